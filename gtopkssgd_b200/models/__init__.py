@@ -7,6 +7,7 @@ from .alexnet import AlexNet
 from .cifar_extras import (caffe_cifar, densenet100_12, preresnet20, preresnet32, preresnet44, preresnet56,
                            preresnet110, resnet_mod20, resnet_mod32, resnet_mod44, resnet_mod56, resnet_mod110,
                            resnext29_8_64, resnext29_16_64)
+from .feed_forward import FeedForward
 from .imagenet_resnet import resnet18, resnet34, resnet50, resnet101, resnet152
 from .lstm import lstm, repackage_hidden
 from .lstman4 import create_net as LSTMAN4
@@ -44,7 +45,8 @@ def create_net(num_classes: int, dnn: str = "resnet20", **kwargs):
         net, ext = LSTMAN4(datapath=kwargs.get("datapath"))
     elif dnn == "lstm":
         net = lstm(vocab_size=kwargs["vocab_size"], batch_size=kwargs["batch_size"],
-                   num_steps=kwargs.get("num_steps", 35))
+                   num_steps=kwargs.get("num_steps", 35),
+                   **{k: kwargs[k] for k in ("ff_layers", "ff_dim", "ff_bits", "ff_dtype") if k in kwargs})
     else:
         raise ValueError("Unsupport neural network %s" % dnn)
     if not hasattr(net, "name"):

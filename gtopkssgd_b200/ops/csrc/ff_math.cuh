@@ -1,0 +1,131 @@
+// What the kernels of the feed-forward operators (K6 layer norm, K7 8-bit activations, K8 matrix products) share:
+// element types, vectors of them, activations with their slopes, and the 8-bit block format.
+//
+// All arithmetic is in f32; a value is rounded once, where it is stored.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <type_traits>
+
+namespace gtk {
+
+enum ElemType : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
+enum Act : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4, kActCount = 5 };
+
+inline int elem_bytes(int type) { return type == kF32 ? 4 : 2; }
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// N elements that move with one access of sizeof(T) * N bytes.
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ void load_f32(const T* p, float (&out)[N]) {
+  const Vec<T, N> x = *reinterpret_cast<const Vec<T, N>*>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = to_f32(x.v[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_f32(T* p, const float (&in)[N]) {
+  Vec<T, N> x;
+#pragma unroll
+  for (int i = 0; i < N; ++i) x.v[i] = from_f32<T>(in[i]);
+  *reinterpret_cast<Vec<T, N>*>(p) = x;
+}
+
+// ---- activations ---------------------------------------------------------------------------------------------
+constexpr float kSqrtHalf = 0.70710678118654752f;        // 1 / sqrt(2)
+constexpr float kInvSqrt2Pi = 0.39894228040143268f;      // 1 / sqrt(2 pi)
+constexpr float kSqrt2OverPi = 0.79788456080286536f;     // sqrt(2 / pi)
+constexpr float kGeluCubic = 0.044715f;
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  if constexpr (ACT == kActRelu) return z < 0.f ? 0.f : z;  // a NaN stays one
+  if constexpr (ACT == kActGelu) return 0.5f * z * (1.f + erff(z * kSqrtHalf));
+  if constexpr (ACT == kActGeluTanh) return 0.5f * z * (1.f + tanhf(kSqrt2OverPi * (z + kGeluCubic * z * z * z)));
+  if constexpr (ACT == kActSilu) return z / (1.f + expf(-z));
+  return z;
+}
+
+// d act(z) / dz, and act(z) itself, which shares its work.
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z, float* value) {
+  if constexpr (ACT == kActRelu) {
+    *value = z < 0.f ? 0.f : z;
+    return z > 0.f ? 1.f : 0.f;
+  }
+  if constexpr (ACT == kActGelu) {
+    const float cdf = 0.5f * (1.f + erff(z * kSqrtHalf));
+    *value = z * cdf;
+    return cdf + z * kInvSqrt2Pi * expf(-0.5f * z * z);
+  }
+  if constexpr (ACT == kActGeluTanh) {
+    const float th = tanhf(kSqrt2OverPi * (z + kGeluCubic * z * z * z));
+    *value = 0.5f * z * (1.f + th);
+    return 0.5f * (1.f + th) + 0.5f * z * (1.f - th * th) * kSqrt2OverPi * (1.f + 3.f * kGeluCubic * z * z);
+  }
+  if constexpr (ACT == kActSilu) {
+    const float sg = 1.f / (1.f + expf(-z));
+    *value = z * sg;
+    return sg * (1.f + z * (1.f - sg));
+  }
+  *value = z;
+  return 1.f;
+}
+
+// Calls f with the activation's number as a type.
+template <int A>
+using ActConst = std::integral_constant<int, A>;
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
+  switch (act) {
+    case kActRelu: f(ActConst<kActRelu>{}); break;
+    case kActGelu: f(ActConst<kActGelu>{}); break;
+    case kActGeluTanh: f(ActConst<kActGeluTanh>{}); break;
+    case kActSilu: f(ActConst<kActSilu>{}); break;
+    default: f(ActConst<kActNone>{}); break;
+  }
+}
+
+// ---- 8 bits: blocks of 32 along a row ----------------------------------------------------------------------------
+// A block stores one byte, e + 127, with e the least integer (at least -127) for which max|x| <= 127 * 2^e; a value
+// is q = rint(x * 2^-e), |q| <= 127, and stands for q * 2^e.  Both scalings are by powers of two, so that only rint
+// rounds and the codes do not depend on the precision they are computed in.  Byte 255: the block held a NaN or an
+// infinity and every value of it stands for NaN.  In the last step, 2^122, codes stop at 63: 64 would stand for 2^128.
+constexpr int kBlock8 = 32;
+constexpr uint32_t kBlock8NaN = 255u, kBlock8Last = 249u;
+
+// abs_bits: the largest bit pattern of |x| in the block.
+__device__ __forceinline__ uint32_t block8_byte(uint32_t abs_bits) {
+  if (abs_bits >= 0x7f800000u) return kBlock8NaN;
+  // |x| = m * 2^E with m in [1, 2): e = E - 6 where m <= 127/64 (mantissa bits up to 0x7e0000), else E - 5
+  const int e = (int)((abs_bits + (0x7fffffu - 0x7e0000u)) >> 23) - 127 - 6;
+  return (uint32_t)(e < -127 ? 0 : e + 127);
+}
+// 2^(byte - 127) for byte 0 .. 254, NaN for 255
+__device__ __forceinline__ float block8_scale(uint32_t byte) {
+  return __uint_as_float(byte == kBlock8NaN ? 0x7fc00000u : byte == 0 ? 0x00400000u : byte << 23);
+}
+// 2^-(byte - 127), for the bytes 0 .. 249 (255: something)
+__device__ __forceinline__ float block8_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+__device__ __forceinline__ int block8_code(float x, uint32_t byte) {
+  const int q = __float2int_rn(x * block8_inverse(byte));
+  return byte < kBlock8Last ? q : byte == kBlock8NaN ? 0 : max(-63, min(63, q));
+}
+
+}  // namespace gtk

@@ -1,0 +1,353 @@
+// K7: element-wise passes over a matrix of activations.
+//
+//   k7_keep          x -> 8-bit codes and one exponent byte per 32 columns of a row (the format is in ff_math.cuh)
+//   k7_stage         a matrix, in its own type or in 8 bits, -> operand or result: restored, with the norm or the
+//                    activation applied again, or split into bf16 pieces for the f32 matrix product
+//   k7_act_backward  dz = dy act'(z) and the sums of dz over the rows (the bias's gradient)
+//
+// Bound by memory.  A warp takes 32 * VEC neighbouring columns of a row, so that a block of 32 lies in 32 / VEC
+// neighbouring lanes and its maximum takes log2(32 / VEC) shuffles; eight warps of a CTA take rows in turn.
+#include "colsum.cuh"
+#include "common.cuh"
+#include "host_api.h"
+#include "launch.cuh"
+
+namespace gtk {
+
+constexpr int kRowWarps = 8;   // warps of a CTA, each with rows of its own
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) k7_keep(const T* x, long long x_ld, signed char* q, long long q_ld, unsigned char* e, long long e_ld, long long rows,
+                                               int cols, int rows_per_warp) {
+  pdl_begin(x);
+  const int c = (int)((blockIdx.x * 32 + threadIdx.x) * VEC);
+  const int padded = (cols + kBlock8 - 1) / kBlock8 * kBlock8;
+  const long long first = ((long long)blockIdx.y * kRowWarps + threadIdx.y) * rows_per_warp;
+  for (int i = 0; i < rows_per_warp; ++i) {
+    const long long row = first + i;
+    if (row >= rows) break;   // the whole warp
+    float v[VEC];
+    uint32_t most = 0;
+    if (c < cols) {
+      load_f32<T, VEC>(x + row * x_ld + c, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = kBlock8 / VEC / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const uint32_t byte = block8_byte(most);
+    if (c < padded) {
+      Vec<signed char, VEC> codes;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) codes.v[j] = (signed char)block8_code(v[j], byte);
+      *reinterpret_cast<Vec<signed char, VEC>*>(q + row * q_ld + c) = codes;
+      if (c % kBlock8 == 0) e[row * e_ld + c / kBlock8] = (unsigned char)byte;
+    }
+  }
+}
+
+// Where an element comes from: a matrix of S, or codes with exponents (S = signed char).
+struct Source {
+  const void* p;
+  long long ld;
+  const unsigned char* e;
+  long long e_ld;
+};
+template <typename S, int VEC>
+__device__ __forceinline__ void load_source(const Source& s, long long row, int c, float (&v)[VEC]) {
+  if constexpr (sizeof(S) == 1) {
+    const Vec<signed char, VEC> q = *reinterpret_cast<const Vec<signed char, VEC>*>((const signed char*)s.p + row * s.ld + c);
+    const float scale = block8_scale(s.e[row * s.e_ld + c / kBlock8]);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = (float)q.v[j] * scale;
+  } else {
+    load_f32<S, VEC>((const S*)s.p + row * s.ld + c, v);
+  }
+}
+
+// What is done to it: (v - mean) rstd g + b where mean is given, then the activation.
+template <typename G>
+struct Apply {
+  const float* mean;
+  const float* rstd;
+  const G* g;
+  const G* b;
+  int act;
+};
+
+// Three bf16 pieces whose sum is v to 24 bits: each is the nearest to what the ones before left.  The first is cut
+// instead of rounded where rounding would overflow; a NaN or an infinity is all in the first.
+__device__ __forceinline__ void split3(float v, __nv_bfloat16 (&p)[3]) {
+  p[0] = __float2bfloat16_rn(v);
+  if (isinf(__bfloat162float(p[0])) && !isinf(v)) p[0] = __float2bfloat16_rz(v);
+  float left = v - __bfloat162float(p[0]);
+  if (!(fabsf(v) <= 3.402823466e38f)) left = 0.f;
+  p[1] = __float2bfloat16_rn(left);
+  p[2] = __float2bfloat16_rn(left - __bfloat162float(p[1]));
+}
+
+// out: `pieces` matrices of rows x out_ld, piece_stride elements apart; columns cols .. pitch - 1 are written as zeros
+// where the pitch is an operand's (a multiple of VEC).
+template <typename S, typename O, typename G, int PIECES, int VEC>
+__global__ void __launch_bounds__(256) k7_stage(Source src, Apply<G> f, O* out, long long out_ld, long long piece_stride, long long rows, int cols, int pitch,
+                                                int rows_per_warp) {
+  pdl_begin(src.p, src.e, f.mean, f.rstd, f.g, f.b);
+  const int c = (int)((blockIdx.x * 32 + threadIdx.x) * VEC);
+  if (c >= pitch) return;
+  const long long first = ((long long)blockIdx.y * kRowWarps + threadIdx.y) * rows_per_warp;
+  for (int i = 0; i < rows_per_warp; ++i) {
+    const long long row = first + i;
+    if (row >= rows) return;
+    float v[VEC];
+    if (c < cols) {
+      load_source<S, VEC>(src, row, c, v);
+      if constexpr (sizeof(S) == 1 && std::is_same_v<O, __half>) {   // a code may stand for 65536, up to half a step above what it was
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (fabsf(v[j]) > 65504.f) v[j] = copysignf(65504.f, v[j]);
+      }
+      if (f.mean) {
+        const float m = f.mean[row], r = f.rstd[row];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          v[j] = (v[j] - m) * r;
+          if (f.g) v[j] *= to_f32(f.g[c + j]);
+          if (f.b) v[j] += to_f32(f.b[c + j]);
+        }
+      }
+      if (f.act != kActNone)
+        with_act(f.act, [&](auto A) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) v[j] = act_value<decltype(A)::value>(v[j]);
+        });
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = 0.f;
+    }
+    O* at = out + row * out_ld + c;
+    if constexpr (PIECES == 3) {
+      Vec<__nv_bfloat16, VEC> o[3];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        __nv_bfloat16 p[3];
+        split3(v[j], p);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) o[k].v[j] = p[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<Vec<__nv_bfloat16, VEC>*>(at + k * piece_stride) = o[k];
+    } else {
+      store_f32<O, VEC>(at, v);
+    }
+  }
+}
+
+// Z: element type of z (signed char: codes).  dz may be null (sums only); partial may be null.
+template <typename T, typename Z, int VEC>
+__global__ void __launch_bounds__(256) k7_act_backward(const T* dy, long long dy_ld, Source z, int act, T* dz, long long dz_ld, float* partial, long long rows,
+                                                       int cols) {
+  __shared__ float joined[kRowWarps][32 * VEC];
+  pdl_begin(dy, z.p, z.e);
+  const int c = (int)((blockIdx.x * 32 + threadIdx.x) * VEC);
+  float sum[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
+  if (c < cols)
+    for (long long row = (long long)blockIdx.y * kRowWarps + threadIdx.y; row < rows; row += (long long)gridDim.y * kRowWarps) {
+      float g[VEC];
+      load_f32<T, VEC>(dy + row * dy_ld + c, g);
+      if (act != kActNone) {
+        float zv[VEC];
+        load_source<Z, VEC>(z, row, c, zv);
+        with_act(act, [&](auto A) {
+          float value;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) g[j] *= act_slope<decltype(A)::value>(zv[j], &value);
+        });
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) sum[j] += g[j];
+      if (dz) store_f32<T, VEC>(dz + row * dz_ld + c, g);
+    }
+  if (!partial) return;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) joined[threadIdx.y][threadIdx.x * VEC + j] = sum[j];
+  __syncthreads();
+  const int t = (int)(threadIdx.y * 32 + threadIdx.x);
+  for (int i = t; i < 32 * VEC; i += 256) {
+    const int col = (int)(blockIdx.x * 32 * VEC) + i;
+    if (col >= cols) break;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < kRowWarps; ++k) s += joined[k][i];
+    partial[(size_t)blockIdx.y * cols + col] = s;
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------
+inline bool aligned(const void* p, long long ld, int elem, int vec) {
+  return (uintptr_t)p % ((uintptr_t)elem * vec) == 0 && (ld * elem) % ((long long)elem * vec) == 0;
+}
+
+// Rows that a warp takes, so that the grid is a few CTAs an SM at least and its y fits.
+inline bool row_grid(long long rows, unsigned strips, int* per_warp, unsigned* y) {
+  long long per = rows * strips / (kRowWarps * 148LL * 8);
+  per = per < 1 ? 1 : per > 8 ? 8 : per;
+  while ((rows + kRowWarps * per - 1) / (kRowWarps * per) > 65535) per *= 2;
+  if (per > 0x3fffffff) return false;
+  *per_warp = (int)per;
+  *y = (unsigned)((rows + kRowWarps * per - 1) / (kRowWarps * per));
+  return true;
+}
+
+template <typename T>
+int keep(const void* x, long long x_ld, signed char* q, long long q_ld, unsigned char* e, long long e_ld, long long rows, int cols, cudaStream_t stream) {
+  auto go = [&](auto V) -> int {
+    constexpr int VEC = decltype(V)::value;
+    const int padded = (cols + kBlock8 - 1) / kBlock8 * kBlock8;
+    const unsigned strips = (unsigned)((padded + 32 * VEC - 1) / (32 * VEC));
+    int per;
+    unsigned y;
+    if (!row_grid(rows, strips, &per, &y)) return GTK_ERR_UNSUPPORTED;
+    const cudaError_t err = launch_pdl(k7_keep<T, VEC>, dim3(strips, y), dim3(32, kRowWarps), stream, (const T*)x, x_ld, q, q_ld, e, e_ld, rows, cols, per);
+    gtk_count_launch(1);
+    return err == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;
+  };
+  constexpr int wide = 16 / sizeof(T);
+  const bool q_ok = aligned(q, q_ld, 1, wide);
+  if (cols % wide == 0 && aligned(x, x_ld, sizeof(T), wide) && q_ok) return go(std::integral_constant<int, wide>{});
+  if (cols % 4 == 0 && aligned(x, x_ld, sizeof(T), 4) && aligned(q, q_ld, 1, 4)) return go(std::integral_constant<int, 4>{});
+  return go(std::integral_constant<int, 1>{});
+}
+
+template <typename S, typename O, typename G, int PIECES>
+int stage(Source src, Apply<G> f, void* out, long long out_ld, long long piece_stride, long long rows, int cols, int pitch, cudaStream_t stream) {
+  auto go = [&](auto V) -> int {
+    constexpr int VEC = decltype(V)::value;
+    const unsigned strips = (unsigned)((pitch + 32 * VEC - 1) / (32 * VEC));
+    int per;
+    unsigned y;
+    if (!row_grid(rows, strips, &per, &y)) return GTK_ERR_UNSUPPORTED;
+    const cudaError_t err = launch_pdl(k7_stage<S, O, G, PIECES, VEC>, dim3(strips, y), dim3(32, kRowWarps), stream, src, f, (O*)out, out_ld, piece_stride,
+                                       rows, cols, pitch, per);
+    gtk_count_launch(1);
+    return err == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;
+  };
+  // a block's scale is read once per vector, so vectors do not cross blocks (they start at multiples of their length)
+  constexpr int wide = sizeof(S) == 4 || sizeof(O) == 4 ? 4 : 8;
+  auto fits = [&](int vec) {
+    return cols % vec == 0 && pitch % vec == 0 && piece_stride % vec == 0 && aligned(src.p, src.ld, sizeof(S), vec) && aligned(out, out_ld, sizeof(O), vec);
+  };
+  if (fits(wide)) return go(std::integral_constant<int, wide>{});
+  if (wide == 8 && fits(4)) return go(std::integral_constant<int, 4>{});
+  return go(std::integral_constant<int, 1>{});
+}
+
+template <typename T, typename Z>
+int act_backward(const void* dy, long long dy_ld, Source z, int act, void* dz, long long dz_ld, void* db, float* partial, int max_lines, long long rows,
+                 int cols, cudaStream_t stream) {
+  unsigned lines = 0;
+  auto go = [&](auto V) {
+    constexpr int VEC = decltype(V)::value;
+    const unsigned strips = (unsigned)((cols + 32 * VEC - 1) / (32 * VEC));
+    long long y = (148LL * 8 + strips - 1) / strips;
+    const long long most = (rows + kRowWarps - 1) / kRowWarps;
+    if (y > most) y = most;
+    if (y > max_lines) y = max_lines;
+    lines = (unsigned)y;
+    return launch_pdl(k7_act_backward<T, Z, VEC>, dim3(strips, lines), dim3(32, kRowWarps), stream, (const T*)dy, dy_ld, z, act, (T*)dz, dz_ld,
+                      db ? partial : (float*)nullptr, rows, cols);
+  };
+  auto fits = [&](int vec) {
+    return cols % vec == 0 && aligned(dy, dy_ld, sizeof(T), vec) && (act == kActNone || aligned(z.p, z.ld, sizeof(Z), vec)) &&
+           (!dz || aligned(dz, dz_ld, sizeof(T), vec));
+  };
+  constexpr int wide = 16 / sizeof(T);
+  cudaError_t err;
+  if (fits(wide)) err = go(std::integral_constant<int, wide>{});
+  else if (wide == 8 && fits(4)) err = go(std::integral_constant<int, 4>{});
+  else err = go(std::integral_constant<int, 1>{});
+  gtk_count_launch(1);
+  if (err != cudaSuccess) return GTK_ERR_CUDA;
+  if (!db) return GTK_OK;
+  err = launch_col_finish<T>(partial, (int)lines, cols, cols, (T*)db, (T*)nullptr, stream);
+  gtk_count_launch(1);
+  return err == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;
+}
+
+constexpr int kActLines = 148;
+
+}  // namespace gtk
+
+using namespace gtk;
+
+// Codes of a matrix: q has q_ld >= cols rounded up to 32 (the rest of the last block is written as zeros).
+extern "C" int gtk_k7_keep(int type, const void* x, long long x_ld, signed char* q, long long q_ld, unsigned char* e, long long e_ld, long long rows,
+                           long long cols, void* stream) {
+  if (rows <= 0 || cols <= 0 || cols > 0x3fffffff || x_ld < 0 || q_ld < (cols + kBlock8 - 1) / kBlock8 * kBlock8 || e_ld < (cols + kBlock8 - 1) / kBlock8)
+    return GTK_ERR_ARG;
+  switch (type) {
+    case kF32: return keep<float>(x, x_ld, q, q_ld, e, e_ld, rows, (int)cols, (cudaStream_t)stream);
+    case kF16: return keep<__half>(x, x_ld, q, q_ld, e, e_ld, rows, (int)cols, (cudaStream_t)stream);
+    case kBF16: return keep<__nv_bfloat16>(x, x_ld, q, q_ld, e, e_ld, rows, (int)cols, (cudaStream_t)stream);
+  }
+  return GTK_ERR_ARG;
+}
+
+// The matrix src (of `type`, or 8-bit codes where e is given), normalised again where mean is given, through the
+// activation, -> out.  out_kind 0: a matrix of `type`; 1: one bf16 piece (f32 codes without a transform, which are
+// exact in it); 3: three bf16 pieces (f32).  Columns up to `pitch` are written, those past `cols` as zeros.
+extern "C" int gtk_k7_stage(int type, const void* src, long long src_ld, const unsigned char* e, long long e_ld, const float* mean, const float* rstd,
+                            const void* g, const void* b, int act, int out_kind, void* out, long long out_ld, long long piece_stride, long long rows,
+                            long long cols, long long pitch, void* stream_) {
+  if (rows <= 0 || cols <= 0 || pitch < cols || out_ld < pitch || pitch > 0x3fffffff || src_ld < 0 || act < 0 || act >= kActCount) return GTK_ERR_ARG;
+  const cudaStream_t stream = (cudaStream_t)stream_;
+  const Source s{src, src_ld, e, e_ld};
+  const int n = (int)cols, p = (int)pitch;
+  auto of = [&](auto t) -> int {
+    using T = decltype(t);
+    const Apply<T> f{mean, rstd, (const T*)g, (const T*)b, act};
+    if (out_kind == 0)
+      return e ? stage<signed char, T, T, 1>(s, f, out, out_ld, piece_stride, rows, n, p, stream)
+               : stage<T, T, T, 1>(s, f, out, out_ld, piece_stride, rows, n, p, stream);
+    if constexpr (sizeof(T) == 4) {
+      if (out_kind == 1 && e && !mean && act == kActNone)
+        return stage<signed char, __nv_bfloat16, T, 1>(s, f, out, out_ld, piece_stride, rows, n, p, stream);
+      if (out_kind == 3)
+        return e ? stage<signed char, __nv_bfloat16, T, 3>(s, f, out, out_ld, piece_stride, rows, n, p, stream)
+                 : stage<T, __nv_bfloat16, T, 3>(s, f, out, out_ld, piece_stride, rows, n, p, stream);
+    }
+    return GTK_ERR_ARG;
+  };
+  switch (type) {
+    case kF32: return of(float{});
+    case kF16: return of(__half{});
+    case kBF16: return of(__nv_bfloat16{});
+  }
+  return GTK_ERR_ARG;
+}
+
+// Lines of `cols` floats that `partial` has to hold.
+extern "C" int gtk_k7_act_lines(void) { return kActLines; }
+
+// dz = dy act'(z), db = sum of dz over the rows; z in `type`, or codes where e is given; dz and db may be null.
+extern "C" int gtk_k7_act_backward(int type, const void* dy, long long dy_ld, const void* z, long long z_ld, const unsigned char* e, long long e_ld, int act,
+                                   void* dz, long long dz_ld, void* db, float* partial, long long rows, long long cols, void* stream_) {
+  if (rows <= 0 || cols <= 0 || cols > 0x3fffffff || act < 0 || act >= kActCount || (act != kActNone && !z) || (!dz && !db)) return GTK_ERR_ARG;
+  const cudaStream_t stream = (cudaStream_t)stream_;
+  const Source s{z, z_ld, e, e_ld};
+  auto of = [&](auto t) {
+    using T = decltype(t);
+    return e ? act_backward<T, signed char>(dy, dy_ld, s, act, dz, dz_ld, db, partial, kActLines, rows, (int)cols, stream)
+             : act_backward<T, T>(dy, dy_ld, s, act, dz, dz_ld, db, partial, kActLines, rows, (int)cols, stream);
+  };
+  switch (type) {
+    case kF32: return of(float{});
+    case kF16: return of(__half{});
+    case kBF16: return of(__nv_bfloat16{});
+  }
+  return GTK_ERR_ARG;
+}

@@ -1,0 +1,132 @@
+"""The feed-forward block of a residual network over sequences (K6, K7, K8 together).
+
+    y = x + W2 act(W1 norm(x) + b1) + b2
+
+``feed_forward`` computes it and what its backward pass reads: x, the norm's mean
+and rstd, and z, the activation's input; with ``bits=8`` x and z are kept as
+``Activation8``, 2.06 bytes a row and column of each together.  The norm's output and the
+hidden layer are made again from them in the backward pass.  Of that one
+(``feed_forward_backward``) the product dy W2 multiplies by the activation's slope,
+makes the hidden layer again and sums b1's gradient in its epilogue.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+
+from . import layers_oracle as oracle
+from .activation8 import Activation8, act_of, bits_of, colsum, matrix, same, shaped, stream_of, type_of, vector
+from .layer_norm import layer_norm_backward, layer_norm_forward
+from .linear import _check, _gradients, linear_forward, operand, product
+
+
+class FeedForwardKept(NamedTuple):
+    """What the forward pass keeps for the backward pass."""
+    x: Union[torch.Tensor, Activation8]
+    mean: torch.Tensor
+    rstd: torch.Tensor
+    z: Union[torch.Tensor, Activation8]
+
+
+def feed_forward(x: torch.Tensor, norm_weight: torch.Tensor, norm_bias: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Tensor,
+                 b2: torch.Tensor, activation: str = "gelu", eps: float = 1e-5, bits: int = 0,
+                 keep: bool = True) -> Tuple[torch.Tensor, Optional[FeedForwardKept]]:
+    """(y, kept); w1 is [hidden, dim], w2 [dim, hidden]."""
+    bits_of(bits)
+    if act_of(activation) == 0:
+        raise ValueError("feed_forward: without an activation the two products are one")
+    _check(x, w1, "feed_forward")
+    shaped("w2", w2, w1.size(1), w1.size(0))
+    a, mean, rstd = layer_norm_forward(x, norm_weight, norm_bias, eps)
+    h, z = linear_forward(a, w1, b1, activation, keep=keep, bits=bits)
+    y, _ = linear_forward(h, w2, b2, residual=x)
+    if not keep:
+        return y, None
+    return y, FeedForwardKept(Activation8.keep(x) if bits else x, mean, rstd, z)
+
+
+def feed_forward_backward(dy: torch.Tensor, kept: FeedForwardKept, norm_weight: torch.Tensor, norm_bias: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor,
+                          activation: str = "gelu"):
+    """(dx, dnorm_weight, dnorm_bias, dw1, db1, dw2, db2)."""
+    type_of(dy, "feed_forward")
+    code = act_of(activation)
+    if code == 0:
+        raise ValueError("feed_forward: without an activation the two products are one")
+    x, mean, rstd, z = kept
+    hidden, dim = w1.shape
+    shape = tuple(dy.shape)
+    shaped("w2", w2, dim, hidden)
+    shaped("norm_weight", norm_weight, dim)
+    shaped("norm_bias", norm_bias, dim)
+    if tuple(x.shape) != shape or shape[-1] != dim:
+        raise ValueError("the gradient has shape %s, x %s, w1 %s" % (shape, tuple(x.shape), tuple(w1.shape)))
+    same(dy, x=x, z=z, w1=w1, w2=w2, norm_weight=norm_weight, norm_bias=norm_bias)
+    g = matrix(dy)
+    rows = g.size(0)
+    z = z if isinstance(z, Activation8) else matrix(z)
+    if (tuple(z.q.shape) if isinstance(z, Activation8) else tuple(z.shape)) != (rows, hidden):
+        raise ValueError("z has shape %s instead of %s" % (tuple(z.shape), (rows, hidden)))
+    if mean.numel() != rows or rstd.numel() != rows:
+        raise ValueError("mean and rstd are the forward pass's, one value for each of %d rows" % rows)
+    if not g.is_cuda:
+        return _backward_plain(g, FeedForwardKept(x, mean.reshape(-1), rstd.reshape(-1), z), norm_weight, norm_bias, w1, w2, activation, shape)
+    new = dict(dtype=dy.dtype, device=dy.device)
+    if rows == 0:
+        return (torch.empty(shape, **new), *(torch.zeros(n, **new) for n in (dim, dim, (hidden, dim), hidden, (dim, hidden), dim)))
+    stream = stream_of(g)
+    mean, rstd = vector(mean), vector(rstd)
+    # dz = (dy W2) act'(z) and h = act(z) again, both in the product's epilogue
+    dz, h = torch.empty((rows, hidden), **new), torch.empty((rows, hidden), **new)
+    db1 = torch.empty(hidden, **new)
+    go = operand(g)
+    product(rows, hidden, dim, go, False, operand(matrix(w2)), True, dz, stream, activation=code, slope=True, z=z, h=h, db=db1)
+    dw2 = torch.empty((dim, hidden), **new)
+    product(dim, hidden, rows, go, True, operand(h), True, dw2, stream)
+    del h
+    _, db2 = colsum(g)
+    xm = x if isinstance(x, Activation8) else matrix(x)
+    a = operand(xm, mean, rstd, vector(norm_weight), vector(norm_bias))   # the norm's output again
+    da, dw1 = _gradients(dz, a, dim, w1, True, True)
+    dx, dg, db = layer_norm_backward(da.view(shape), x.restore() if isinstance(x, Activation8) else x, mean, rstd, norm_weight, add=dy)
+    return dx, dg, db, dw1, db1, dw2, db2
+
+
+def _backward_plain(g, kept, norm_weight, norm_bias, w1, w2, activation, shape):
+    def values(t):
+        return oracle.values8(t.q, t.e, oracle.wide(g).dtype) if isinstance(t, Activation8) else oracle.wide(matrix(t))
+
+    x, mean, rstd, z = values(kept.x), kept.mean, kept.rstd, values(kept.z)
+    t = g.dtype
+    dy = oracle.wide(g)
+    dz, db1 = oracle.act_backward(dy @ oracle.wide(w2), z, activation)
+    a = (x - mean[:, None]) * rstd[:, None] * oracle.wide(norm_weight) + oracle.wide(norm_bias)
+    dx, dg, db = oracle.norm_backward(dz @ oracle.wide(w1), x, mean, rstd, norm_weight, dy)
+    dw1, dw2 = dz.t() @ a, dy.t() @ oracle.act(activation, z)
+    return tuple(v.to(t) for v in (dx.view(shape), dg, db, dw1, db1, dw2, dy.sum(0)))
+
+
+class _FeedForward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, norm_weight, norm_bias, w1, b1, w2, b2, activation, eps, bits):
+        need = any(ctx.needs_input_grad)
+        y, kept = feed_forward(x, norm_weight, norm_bias, w1, b1, w2, b2, activation, eps, bits, need)
+        if need:
+            ctx.activation = activation
+            ctx.codes = (kept.x, kept.z) if bits else None
+            ctx.save_for_backward(kept.mean, kept.rstd, norm_weight, norm_bias, w1, w2, *(() if bits else (kept.x, kept.z)))
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        mean, rstd, norm_weight, norm_bias, w1, w2, *rest = ctx.saved_tensors
+        x, z = ctx.codes or rest
+        got = feed_forward_backward(dy, FeedForwardKept(x, mean, rstd, z), norm_weight, norm_bias, w1, w2, ctx.activation)
+        return (*(g if n else None for g, n in zip(got, ctx.needs_input_grad)), None, None, None)
+
+
+def feed_forward_block(x: torch.Tensor, norm_weight: torch.Tensor, norm_bias: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Tensor,
+                       b2: torch.Tensor, activation: str = "gelu", eps: float = 1e-5, bits: int = 0) -> torch.Tensor:
+    """x + W2 act(W1 norm(x) + b1) + b2 under autograd; with ``bits=8`` x and the activation's input are kept in 8 bits."""
+    return _FeedForward.apply(x, norm_weight, norm_bias, w1, b1, w2, b2, activation, eps, bits_of(bits))

@@ -1,0 +1,105 @@
+"""Layer norm over the last axis, forward and backward (K6).
+
+``layer_norm`` is the operator under autograd; ``layer_norm_forward`` and
+``layer_norm_backward`` are its two directions for code that keeps its own tape.
+x is any shape [..., cols] in f32, f16 or bf16; weight and bias, each optional,
+are vectors of its type.  Statistics and sums are f32.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import layers_oracle as oracle
+from . import lib as _lib
+from .activation8 import TYPES, ld, lines, matrix, same, shaped, stream_of, type_of, vector
+from .select import _ptr
+
+
+def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                       eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, mean, rstd): y = (x - mean) * rstd * weight + bias, rstd = (variance + eps)^-1/2; mean and rstd are f32, of
+    x's shape without its last axis."""
+    code = type_of(x, "layer_norm")
+    m = matrix(x)
+    rows, cols = m.shape
+    if x.size(-1) == 0:
+        raise ValueError("layer_norm: the last axis is empty")
+    same(x, weight=weight, bias=bias)
+    shaped("weight", weight, cols)
+    shaped("bias", bias, cols)
+    lead = x.shape[:-1]
+    if not m.is_cuda:
+        y, mean, rstd = oracle.norm_forward(m, weight, bias, eps)
+        return y.view(x.shape), mean.view(lead), rstd.view(lead)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean, rstd = torch.empty((2, *lead), dtype=torch.float32, device=x.device).unbind(0)
+    if rows:
+        weight, bias = vector(weight), vector(bias)
+        err = _lib.calls().gtk_k6_norm_forward(code, m.data_ptr(), ld(m), _ptr(weight), _ptr(bias), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                               rows, cols, eps, stream_of(m))
+        if err:
+            _lib.check(err, "gtk_k6_norm_forward")
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                        add: Optional[torch.Tensor] = None,
+                        want_parameters: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(dx, dweight, dbias) from the forward pass's x, mean and rstd.  ``add``, of x's shape, is added to dx: the
+    gradient that reaches x past the norm."""
+    type_of(x, "layer_norm")
+    m, g = matrix(x), matrix(dy)
+    rows, cols = m.shape
+    if dy.shape != x.shape:
+        raise ValueError("the gradient has shape %s, x %s" % (tuple(dy.shape), tuple(x.shape)))
+    same(x, dy=dy, weight=weight, add=add)
+    shaped("weight", weight, cols)
+    shaped("add", add, *x.shape)
+    if mean.numel() != rows or rstd.numel() != rows or mean.device != x.device or rstd.device != x.device:
+        raise ValueError("mean and rstd are the forward pass's, one value for each of %d rows" % rows)
+    if not m.is_cuda:
+        dx, dw, db = oracle.norm_backward(g, m, mean.reshape(-1), rstd.reshape(-1), weight, None if add is None else matrix(add))
+        return (dx.view(x.shape), dw, db) if want_parameters else (dx.view(x.shape), None, None)
+    if mean.dtype != torch.float32 or rstd.dtype != torch.float32:
+        raise TypeError("mean and rstd are float32")
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = db = partial = None
+    if want_parameters:
+        dw, db = torch.empty((2, cols), dtype=x.dtype, device=x.device).unbind(0)
+        partial = torch.empty((min(lines("gtk_k6_norm_lines"), max(rows, 1)), 2 * cols), dtype=torch.float32, device=x.device)
+    if rows == 0:
+        if want_parameters:
+            dw.zero_()
+            db.zero_()
+        return dx, dw, db
+    weight, mean, rstd = vector(weight), vector(mean), vector(rstd)
+    a = None if add is None else matrix(add)
+    err = _lib.calls().gtk_k6_norm_backward(TYPES[x.dtype], g.data_ptr(), ld(g), m.data_ptr(), ld(m), mean.data_ptr(), rstd.data_ptr(), _ptr(weight),
+                                            _ptr(a), 0 if a is None else ld(a), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(partial), rows, cols,
+                                            stream_of(m))
+    if err:
+        _lib.check(err, "gtk_k6_norm_backward")
+    return dx, dw, db
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = layer_norm_forward(x, weight, bias, eps)
+        ctx.save_for_backward(x, mean, rstd, weight)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, mean, rstd, weight = ctx.saved_tensors
+        parameters = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dx, dw, db = layer_norm_backward(dy, x, mean, rstd, weight, want_parameters=parameters)
+        return dx, dw if ctx.needs_input_grad[1] else None, db if ctx.needs_input_grad[2] else None, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(variance + eps) * weight + bias over the last axis, under autograd."""
+    return _LayerNorm.apply(x, weight, bias, eps)

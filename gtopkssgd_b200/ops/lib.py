@@ -79,6 +79,7 @@ def _declare(lib):
     lib.gtk_p2p_unmap.restype = i32
     lib.gtk_p2p_enable_peer.argtypes = [i32]
     lib.gtk_p2p_enable_peer.restype = i32
+    lib.gtk_k8_status.restype = u32
     return lib
 
 

@@ -1,0 +1,216 @@
+"""The feed-forward operators on the CPU: the plain forms against independent
+statements in 64 bits, gradients against differences, the 8-bit format's edges,
+refusals, and the block in the language model under the sparse optimizer."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from gtopkssgd_b200.models import FeedForward, create_net
+from gtopkssgd_b200.ops import layers_oracle as oracle
+from gtopkssgd_b200.ops.activation8 import Activation8
+from gtopkssgd_b200.ops.feed_forward import FeedForwardKept, feed_forward, feed_forward_backward, feed_forward_block
+from gtopkssgd_b200.ops.layer_norm import layer_norm, layer_norm_backward, layer_norm_forward
+from gtopkssgd_b200.ops.linear import linear, linear_backward, linear_forward
+
+LIBRARY = {"none": lambda z: z, "relu": F.relu, "gelu": F.gelu, "gelu_tanh": lambda z: F.gelu(z, approximate="tanh"), "silu": F.silu}
+
+
+def _leaf(*shape):
+    return torch.randn(*shape, dtype=torch.float64, requires_grad=True)
+
+
+@pytest.mark.parametrize("name", list(LIBRARY))
+def test_activations_and_slopes(name):
+    z = torch.linspace(-6, 6, 241, dtype=torch.float64, requires_grad=True)
+    y = LIBRARY[name](z)
+    slope, = torch.autograd.grad(y.sum(), z)
+    assert torch.allclose(oracle.act(name, z), y, rtol=1e-12, atol=1e-14)
+    assert torch.allclose(oracle.act_slope(name, z), slope, rtol=1e-12, atol=1e-14)
+
+
+def test_gradients_against_differences():
+    torch.manual_seed(0)
+    assert torch.autograd.gradcheck(lambda *a: layer_norm(*a), (_leaf(3, 2, 7), _leaf(7), _leaf(7)))
+    assert torch.autograd.gradcheck(lambda x: layer_norm(x), (_leaf(4, 5),))
+    for name in ("none", "gelu", "gelu_tanh", "silu"):
+        assert torch.autograd.gradcheck(lambda x, w, b, r: linear(x, w, b, name, r), (_leaf(3, 2, 5), _leaf(4, 5), _leaf(4), _leaf(3, 2, 4)))
+    assert torch.autograd.gradcheck(lambda *a: feed_forward_block(*a), (_leaf(3, 2, 5), _leaf(5), _leaf(5), _leaf(6, 5), _leaf(6), _leaf(5, 6), _leaf(5)))
+
+
+def test_eight_bit_gradients_are_the_formula_at_the_kept_values():
+    """With 8 bits the backward pass is the exact one at the values that the codes stand for."""
+    torch.manual_seed(1)
+    x, w, b = torch.randn(6, 70, dtype=torch.float64), torch.randn(33, 70, dtype=torch.float64), torch.randn(33, dtype=torch.float64)
+    dy = torch.randn(6, 33, dtype=torch.float64)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    linear(*leaves, "gelu", bits=8).backward(dy)
+    z8, x8 = Activation8.keep(x @ w.t() + b).restore(), Activation8.keep(x).restore()
+    dz = dy * oracle.act_slope("gelu", z8)
+    for got, want in zip(leaves, (dz @ w, dz.t() @ x8, dz.sum(0))):
+        assert torch.allclose(got.grad, want, rtol=1e-10, atol=1e-12)
+
+
+# -- the 8-bit format --------------------------------------------------------------
+def test_codes_at_the_edges_of_the_format():
+    block = torch.zeros(1, 32)
+
+    def code(*values):
+        x = block.clone()
+        x[0, :len(values)] = torch.tensor(values)
+        kept = Activation8.keep(x)
+        return kept.q[0, :len(values)].tolist(), int(kept.e[0, 0]) - 127, kept.restore()[0, :len(values)].tolist()
+
+    assert code(127.0, 1.0)[:2] == ([127, 1], 0)              # 127 * 2^0 is the largest that step 1 takes
+    assert code(127.0 + 2 ** -17, 1.0)[:2] == ([64, 0], 1)    # the next f32 above takes step 2; 1 / 2 is a tie, to even
+    assert code(254.0, 3.0)[:2] == ([127, 2], 1)              # 1.5 is a tie, to even
+    assert code(-1.0, 0.5)[:2] == ([-64, 32], -6)
+    assert code(0.0)[:2] == ([0], -127) and code(0.0)[2] == [0.0]
+    tiny = 2.0 ** -149
+    assert code(tiny)[0] == [0] and code(tiny)[2] == [0.0]     # steps end at 2^-127
+    assert code(2.0 ** -126, 2.0 ** -127)[2] == [2.0 ** -126, 2.0 ** -127]
+    big = torch.finfo(torch.float32).max
+    q, e, back = code(big)
+    assert q == [63] and e == 122 and back == [63 * 2.0 ** 122]   # 64 would stand for more than f32 holds
+    half = torch.full((1, 32), 65504.0, dtype=torch.float16)
+    assert torch.equal(Activation8.keep(half).restore(), half)    # 64 * 2^10 in f32
+    for bad in (math.inf, -math.inf, math.nan):
+        q, e, back = code(1.0, bad)
+        assert e == 255 - 127 and all(math.isnan(v) for v in back)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 31), (3, 32), (3, 33), (2, 100), (5, 1021)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+def test_restored_values_are_within_half_a_step(rows, cols, dtype):
+    torch.manual_seed(cols)
+    x = (torch.randn(rows, cols) * torch.exp(torch.randn(rows, 1) * 3)).to(dtype)
+    kept = Activation8.keep(x)
+    assert kept.q.shape == (rows, cols) and kept.e.shape == (rows, -(-cols // 32)) and kept.restore().dtype == dtype
+    step = torch.exp2(kept.e.double() - 127).repeat_interleave(32, 1)[:, :cols]
+    assert torch.all((kept.restore().double() - x.double()).abs() <= step / 2)
+    most = F.pad(x.double().abs(), (0, -cols % 32)).view(rows, -1, 32).amax(2)
+    assert torch.all(most <= 127 * torch.exp2(kept.e.double() - 127))       # large enough
+    assert torch.all(most > 127 * torch.exp2(kept.e.double() - 128))        # and the least such step
+    again = Activation8.keep(kept.restore())                                # what is restored is kept exactly
+    assert torch.equal(again.restore(), kept.restore())
+
+
+def test_shapes_lengths_and_strides():
+    x = torch.randn(5, 3, 24).transpose(0, 1)
+    y, mean, rstd = layer_norm_forward(x)
+    assert y.shape == x.shape and mean.shape == x.shape[:-1]
+    assert torch.allclose(y, F.layer_norm(x, (24,)), atol=1e-5)
+    assert layer_norm(torch.empty(0, 8)).shape == (0, 8)
+    w = torch.randn(8, 24)
+    y, z = linear_forward(x, w, activation="relu", keep=True)
+    assert y.shape == (3, 5, 8) and z.shape == (15, 8)
+    assert linear_forward(x, w)[1] is None and linear_forward(x, w, keep=True)[1] is None
+    assert linear(torch.empty(0, 24), w).shape == (0, 8)
+    dx, dw, db = linear_backward(torch.empty(0, 8), torch.empty(0, 24), w)
+    assert dx.shape == (0, 24) and not dw.any() and not db.any()
+    dx, dw, db = linear_backward(torch.randn(3, 5, 8), x, w, need=(False, True, False))
+    assert dx is None and db is None and dw.shape == w.shape
+    kept = Activation8.keep(x)
+    assert kept.shape == x.shape and kept.restore().shape == x.shape
+
+
+def test_refusals():
+    x, w, b = torch.randn(4, 6), torch.randn(5, 6), torch.randn(5)
+    with pytest.raises(TypeError):
+        layer_norm(torch.zeros(2, 3, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        layer_norm(torch.zeros(2, 0))
+    with pytest.raises(ValueError):
+        layer_norm(x, torch.ones(5))
+    with pytest.raises(ValueError):
+        layer_norm(x, torch.ones(6, dtype=torch.bfloat16))
+    y, mean, rstd = layer_norm_forward(x)
+    with pytest.raises(ValueError):
+        layer_norm_backward(y[:, :5], x, mean, rstd)
+    with pytest.raises(ValueError):
+        layer_norm_backward(y, x, mean[:3], rstd)
+    with pytest.raises(ValueError):
+        linear(x, torch.randn(5, 7))
+    with pytest.raises(ValueError):
+        linear(x, w, torch.randn(6))
+    with pytest.raises(ValueError):
+        linear(x, w, b, "swish")
+    with pytest.raises(ValueError):
+        linear(x, w, b, residual=torch.randn(5))          # a residual is not broadcast
+    with pytest.raises(ValueError):
+        linear(x, w.bfloat16())
+    with pytest.raises(ValueError):
+        linear(x, w, b, "gelu", bits=4)
+    with pytest.raises(ValueError):
+        linear(x, torch.randn(5, 0))
+    with pytest.raises(ValueError):
+        linear_backward(torch.randn(4, 5), x, w, "gelu", None)
+    with pytest.raises(ValueError):
+        linear_backward(torch.randn(4, 5), x, w, "gelu", torch.randn(4, 6))
+    kept = Activation8.keep(x)
+    with pytest.raises(ValueError):
+        Activation8(kept.q.int(), kept.e, torch.float32)
+    with pytest.raises(ValueError):
+        Activation8(kept.q, kept.e[:, :0], torch.float32)
+    with pytest.raises(ValueError):
+        Activation8(kept.q, kept.e, torch.float32, (5, 6))
+    with pytest.raises(TypeError):
+        Activation8(kept.q, kept.e, torch.int32)
+    with pytest.raises(ValueError):
+        kept.backward(torch.randn(4, 5), "gelu")
+    with pytest.raises(ValueError):
+        kept.backward(torch.randn(4, 6), "elu")
+    p = [torch.ones(6), torch.zeros(6), torch.randn(8, 6), torch.zeros(8), torch.randn(6, 8), torch.zeros(6)]
+    with pytest.raises(ValueError):
+        feed_forward(x, *p, activation="none")
+    with pytest.raises(ValueError):
+        feed_forward(x, *p[:4], torch.randn(8, 6), p[5])
+    y, kept = feed_forward(x, *p)
+    with pytest.raises(ValueError):
+        feed_forward_backward(y[:3], kept, p[0], p[1], p[2], p[4])
+    with pytest.raises(ValueError):
+        feed_forward_backward(y, FeedForwardKept(kept.x, kept.mean, kept.rstd, kept.z[:, :7]), p[0], p[1], p[2], p[4])
+    with pytest.raises(ValueError):
+        FeedForward(8, 16, activation="none")
+
+
+def test_block_forward_and_backward_parts_agree_with_autograd():
+    torch.manual_seed(3)
+    x = torch.randn(2, 5, 40, dtype=torch.float64)
+    m = FeedForward(40, 72, activation="silu").double()
+    leaf = x.clone().requires_grad_()
+    dy = torch.randn_like(x)
+    y = m(leaf)
+    y.backward(dy)
+    z = F.linear(F.layer_norm(x, (40,), m.norm_weight, m.norm_bias, 1e-5), m.w1, m.b1)
+    assert torch.allclose(y, x + F.linear(F.silu(z), m.w2, m.b2), rtol=1e-10, atol=1e-12)
+    p = [m.norm_weight, m.norm_bias, m.w1, m.b1, m.w2, m.b2]
+    _, kept = feed_forward(x, *p, activation="silu")
+    got = feed_forward_backward(dy, kept, *p[:3], m.w2, "silu")
+    for a, b in zip(got, [leaf.grad] + [t.grad for t in p]):
+        assert torch.allclose(a, b, rtol=1e-10, atol=1e-12)
+
+
+@pytest.mark.parametrize("bits", [0, 8])
+def test_language_model_with_feed_forward_blocks_trains_sparsely(bits):
+    from gtopkssgd_b200.parallel.compression import compressors
+    from gtopkssgd_b200.parallel.distributed_optimizer import DistributedOptimizer
+    torch.manual_seed(0)
+    plain, _ = create_net(0, "lstm", vocab_size=50, batch_size=4, num_steps=5)
+    assert not any("feed_forward" in n for n in plain.state_dict())
+    from gtopkssgd_b200.models import lstm
+    net = lstm(vocab_size=50, embedding_dim=36, num_steps=5, batch_size=4, ff_layers=2, ff_dim=72, ff_bits=bits)
+    opt = DistributedOptimizer(torch.optim.SGD(net.parameters(), lr=0.5), net.named_parameters(), compression=compressors["gtopk"], is_sparse=True,
+                               density=0.05)
+    tokens = torch.randint(0, 50, (6, 4))
+    losses = []
+    for _ in range(60):
+        opt.zero_grad()
+        logits, _ = net(tokens[:-1], net.init_hidden())
+        loss = F.cross_entropy(logits.view(-1, 50), tokens[1:].reshape(-1))
+        loss.backward()
+        opt.step()
+        losses.append(float(loss.detach()))
+    opt.stop()
+    assert all(math.isfinite(v) for v in losses) and losses[-1] < 0.9 * losses[0]
