@@ -13,10 +13,18 @@
 // product has an accumulator apart from the five small ones, and every 256 of k both are added to f32 registers of the
 // epilogue's warps and begun again.
 //
-// A CTA computes tiles of 128 x bn.  One thread brings operand tiles to shared memory by TMA, one issues tcgen05.mma
-// on them into TMEM, eight warps take finished accumulators out of TMEM and through a padded buffer in shared memory,
-// so that a warp's accesses to global memory run along rows.  Two accumulators alternate: the epilogue of a tile
-// overlaps the products of the next.
+// A pair of CTAs (a cluster of two) computes tiles of 256 x bn: each holds 128 rows of A, half of the columns' B and the
+// accumulators of its 128 rows, and one thread of the first issues tcgen05.mma for both, which reads each half of B
+// once for the two tensor cores.  (One CTA with 128 x 256 reads 96 bytes of shared memory a cycle for its products
+// and has 96 written by TMA, of 128 that there are: 920 TFLOP/s at 8192 x 2048 x 8192 before any epilogue.)  In each
+// CTA one thread brings operand tiles by TMA and eight warps take finished accumulators out of TMEM, a row per lane.
+// Two accumulators alternate: the epilogue of a tile overlaps the products of the next.
+//
+// Where tiles are few and k is long, k is split over the pairs of a larger cluster (`splits`); their sums are joined
+// through distributed shared memory in the order of the pairs, each CTA finishing a share of the columns.
+//
+// Matrices whose rows lie on 16-byte boundaries are read and written by each lane along its row; others go through
+// a padded buffer in shared memory, so that a warp's accesses run along rows.
 //
 // Every wait ends: after a time limit the waiter raises the CTA's abort flag and the status word, everybody leaves
 // after its copies and products in flight, and TMEM is freed.
@@ -29,15 +37,19 @@
 
 namespace gtk {
 
-constexpr int kTileM = 128;
+constexpr int kTileM = 256;           // rows of a pair's tile
+constexpr int kRows = 128;            // of one CTA
 constexpr int kTileK = 64;            // 128 bytes of 16-bit elements: one swizzle span
-constexpr int kGemmThreads = 384;     // warp 0 loads, warp 1 multiplies, warps 4 to 11 are the epilogue
+constexpr int kMaxBn = 256;           // columns of a tile
+constexpr int kGemmThreads = 384;     // warps 0 and 2 load A and B, warp 1 multiplies, warps 4 to 11 are the epilogue
 constexpr int kEpiWarps = 8;
-constexpr int kStagePitch = 33;       // floats a row of the epilogue's buffer: no bank conflict along or across
-constexpr int kEpiBytes = kEpiWarps * 32 * kStagePitch * 4;
+constexpr int kPatchPitch = 33;       // floats a row of the epilogue's buffer: no bank conflict along or across
+constexpr int kPatchBytes = kEpiWarps * 32 * kPatchPitch * 4;
 constexpr int kMaxStages = 8;
 constexpr int kF32Blocks = 4;         // f32: blocks of k that are summed in TMEM before they go to registers
+constexpr int kMaxSplits = 4;         // pairs of a cluster: 8 CTAs are portable
 constexpr int kMaxShared = 227 * 1024;
+constexpr int kStaticShared = 2048;   // room for the kernel's static part
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 
 __device__ unsigned int g_gemm_status;   // not 0: a wait ran out (its place in the code)
@@ -45,7 +57,8 @@ __device__ unsigned int g_gemm_status;   // not 0: a wait ran out (its place in 
 struct GemmShape {
   int m, n, k;
   int tiles_m, tiles_n, blocks_k;
-  int bn, stages;
+  int bn, stages, splits;
+  int wide;                            // the epilogue's matrices have rows on 16-byte boundaries
   int a_pieces, b_pieces;
   int a_mn, b_mn;                      // 1: mn-major
   uint32_t idesc;
@@ -77,8 +90,25 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+// True in one lane of the warp.  The compiler knows that what it guards runs in a single thread, whose operands then are
+// uniform: behind a comparison of the lane's number a product took 75 cycles to issue.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "elect.sync _|p, 0xffffffff;\n"
+      "selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(is));
+  return is != 0;
+}
+// The address of the same variable in another CTA of the cluster.
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {   // a cluster address
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -91,15 +121,20 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // False where the CTA has given up; then nothing may be assumed about what was waited for.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t where) {
-  if (mbar_try(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
+  uint64_t t0 = 0;
   for (uint32_t spins = 1;; ++spins) {
     if (mbar_try(bar, parity)) return true;
-    if ((spins & 63u) == 0u) {
+    if ((spins & 255u) == 0u) {   // the clock is slow to read: not before a wait is a long one
       if (*abort) return false;
-      if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      const uint64_t t = globaltimer_ns();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > kWaitLimitNs) {
         *abort = 1;
         atomicCAS(&g_gemm_status, 0u, where);
         return false;
@@ -107,28 +142,30 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
   }
 }
+// Into this CTA's shared memory; `bar` may be the pair's other CTA's.
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int piece, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
                "r"(x), "r"(y), "r"(piece), "r"(bar)
                : "memory");
 }
 // Shared-memory matrix descriptor, 128-byte swizzle.  k-major: rows of 128 bytes, 8 rows (1024 bytes) to the next
 // group.  mn-major: 64 elements of m or n by 8 of k are 1024 bytes, the next 8 of k follow, the next 64 of m or n
-// are `lead` bytes further.
-__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t lead) {
-  return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ void mma(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// are `lead` bytes further.  The low word holds address / 16, to which offsets / 16 can be added.
+__device__ __forceinline__ uint32_t operand_desc(uint32_t addr, uint32_t lead) { return ((addr & 0x3ffffu) >> 4) | ((lead >> 4) << 16); }
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void mma(uint32_t tmem, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(tmem),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n.reg .pred p;\n.reg .b64 a, b;\n"
+      "setp.ne.b32 p, %5, 0;\n"
+      "mov.b64 a, {%1, %3};\n"
+      "mov.b64 b, {%2, %3};\n"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n}" ::"r"(tmem),
+      "r"(a), "r"(b), "r"(kDescHigh), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// The barrier is arrived on when all products issued before by this thread are done.
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// The barrier, in both CTAs of the pair, is arrived on when all products issued before by this thread are done.
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint16_t pair) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(pair) : "memory");
 }
 __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
   asm volatile(
@@ -185,69 +222,220 @@ __device__ __forceinline__ int piece_products(int a_pieces, int b_pieces, uint32
   return 1;
 }
 
-// ---- epilogue of 32 rows by 32 columns: a warp, whose lanes are columns ---------------------------------------------
+// ---- epilogue: 32 rows by 32 columns a warp, a row per lane ------------------------------------------------------------
 struct Patch {
-  const float* at;      // [32][kStagePitch]
-  int row0, col, rows;  // first row, this lane's column, rows inside the matrix
-  bool inside;          // the lane's column is
+  float* room;          // [32][kPatchPitch] of this warp
+  int row, col0;        // this lane's row, the first column
+  int row0, m, n;
+  bool wide;
 };
 
+// v = the lane's row of a matrix of T, columns col0 .. col0 + 31; what is outside is left alone.
 template <typename T>
-__device__ __forceinline__ void finish_forward(const Patch& p, const GemmShape& s, const GemmEpilogue& e) {
-  const float bias = p.inside && e.bias ? to_f32(((const T*)e.bias)[p.col]) : 0.f;
-  with_act(e.act, [&](auto A) {
-#pragma unroll 4
-    for (int r = 0; r < 32; ++r) {
-      if (r >= p.rows) break;
-      const long long row = p.row0 + r;
-      const float z = p.at[r * kStagePitch + (int)lane_id()] + bias;
-      if (e.q) {
-        const uint32_t bits = p.inside ? __float_as_uint(z) & 0x7fffffffu : 0u;
-        const uint32_t byte = block8_byte(__reduce_max_sync(0xffffffffu, bits));
-        e.q[row * e.q_ld + p.col] = p.inside ? (signed char)block8_code(z, byte) : (signed char)0;
-        if (lane_id() == 0) e.e[row * e.e_ld + p.col / kBlock8] = (unsigned char)byte;
-      }
-      if (p.inside) {
-        if (e.z) ((T*)e.z)[row * e.z_ld + p.col] = from_f32<T>(z);
-        float y = act_value<decltype(A)::value>(z);
-        if (e.add) y += to_f32(((const T*)e.add)[row * e.add_ld + p.col]);
-        ((T*)e.out)[row * e.out_ld + p.col] = from_f32<T>(y);
+__device__ __forceinline__ void read32(const void* base, long long ld, const Patch& p, float (&v)[32]) {
+  constexpr int G = 16 / sizeof(T);
+  if (p.wide) {
+    if (p.row < p.m) {
+      const T* at = (const T*)base + (long long)p.row * ld + p.col0;
+#pragma unroll
+      for (int g = 0; g < 32; g += G) {
+        if (p.col0 + g < p.n) {   // n is a multiple of G
+          float x[G];
+          load_f32<T, G>(at + g, x);
+#pragma unroll
+          for (int i = 0; i < G; ++i) v[g + i] = x[i];
+        }
       }
     }
-  });
+  } else {
+    const int col = p.col0 + (int)lane_id(), rows = min(32, p.m - p.row0);
+    __syncwarp();
+    if (col < p.n) {
+      const T* at = (const T*)base + (long long)p.row0 * ld + col;
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r) p.room[r * kPatchPitch + (int)lane_id()] = to_f32(at[r * ld]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = p.room[(int)lane_id() * kPatchPitch + i];
+  }
 }
 
 template <typename T>
-__device__ __forceinline__ float finish_slope(const Patch& p, const GemmShape& s, const GemmEpilogue& e) {
-  float sum = 0.f;
-  if (p.inside)
-    with_act(e.act, [&](auto A) {
-#pragma unroll 4
-      for (int r = 0; r < 32; ++r) {
-        if (r >= p.rows) break;
-        const long long row = p.row0 + r;
-        const float z = e.q ? (float)e.q[row * e.q_ld + p.col] * block8_scale(e.e[row * e.e_ld + p.col / kBlock8]) : to_f32(((const T*)e.z)[row * e.z_ld + p.col]);
-        float h;
-        const float dz = p.at[r * kStagePitch + (int)lane_id()] * act_slope<decltype(A)::value>(z, &h);
-        sum += dz;
-        ((T*)e.out)[row * e.out_ld + p.col] = from_f32<T>(dz);
-        if (e.h) ((T*)e.h)[row * e.h_ld + p.col] = from_f32<T>(h);
+__device__ __forceinline__ void write32(void* base, long long ld, const Patch& p, const float (&v)[32]) {
+  constexpr int G = 16 / sizeof(T);
+  if (p.wide) {
+    if (p.row < p.m) {
+      T* at = (T*)base + (long long)p.row * ld + p.col0;
+#pragma unroll
+      for (int g = 0; g < 32; g += G) {
+        if (p.col0 + g < p.n) {
+          float x[G];
+#pragma unroll
+          for (int i = 0; i < G; ++i) x[i] = v[g + i];
+          store_f32<T, G>(at + g, x);
+        }
       }
+    }
+  } else {
+    const int col = p.col0 + (int)lane_id(), rows = min(32, p.m - p.row0);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) p.room[(int)lane_id() * kPatchPitch + i] = v[i];
+    __syncwarp();
+    if (col < p.n) {
+      T* at = (T*)base + (long long)p.row0 * ld + col;
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r) at[r * ld] = from_f32<T>(p.room[r * kPatchPitch + (int)lane_id()]);
+    }
+  }
+}
+
+// The 8-bit form of the lane's 32 columns, one block.  Codes past the matrix are zeros.
+__device__ __forceinline__ void write_codes(const GemmEpilogue& e, const Patch& p, const float (&z)[32]) {
+  if (p.row >= p.m) return;
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (p.col0 + i < p.n) most = max(most, __float_as_uint(z[i]) & 0x7fffffffu);
+  const uint32_t byte = block8_byte(most);
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (p.col0 + 4 * i + j < p.n) w[i] |= ((uint32_t)block8_code(z[4 * i + j], byte) & 255u) << (8 * j);
+  }
+  uint4* at = reinterpret_cast<uint4*>(e.q + (long long)p.row * e.q_ld + p.col0);   // rows of whole blocks, 16-byte aligned
+  at[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  at[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  e.e[(long long)p.row * e.e_ld + p.col0 / kBlock8] = (unsigned char)byte;
+}
+
+// What the lane's 32 codes stand for.
+__device__ __forceinline__ void read_codes(const GemmEpilogue& e, const Patch& p, float (&z)[32]) {
+  if (p.wide) {
+    if (p.row < p.m) {
+      const signed char* at = e.q + (long long)p.row * e.q_ld + p.col0;
+      const float scale = block8_scale(e.e[(long long)p.row * e.e_ld + p.col0 / kBlock8]);
+#pragma unroll
+      for (int g = 0; g < 32; g += 16)
+        if (p.col0 + g < p.n) {
+          const Vec<signed char, 16> q = *reinterpret_cast<const Vec<signed char, 16>*>(at + g);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) z[g + i] = (float)q.v[i] * scale;
+        }
+    }
+  } else {
+    const int col = p.col0 + (int)lane_id(), rows = min(32, p.m - p.row0);
+    __syncwarp();
+    if (col < p.n) {
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r) {
+        const long long row = p.row0 + r;
+        p.room[r * kPatchPitch + (int)lane_id()] = (float)e.q[row * e.q_ld + col] * block8_scale(e.e[row * e.e_ld + col / kBlock8]);
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) z[i] = p.room[(int)lane_id() * kPatchPitch + i];
+  }
+}
+
+// Sums of 32 columns over the 32 lanes; lane i gets column i's.  Halves the columns a lane holds at each step.
+__device__ __forceinline__ float transpose_sum(float (&v)[32]) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool upper = (lane_id() & (uint32_t)o) != 0;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float give = upper ? v[i] : v[i + o], keep = upper ? v[i + o] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  return v[0];
+}
+
+// bias: 32 floats of this warp in shared memory.
+template <typename T>
+__device__ __forceinline__ void finish_forward(float (&v)[32], float* bias, const GemmEpilogue& e, const Patch& p) {
+  float r[32];
+  if (e.add) read32<T>(e.add, e.add_ld, p, r);
+  if (e.bias) {
+    const int col = p.col0 + (int)lane_id();
+    __syncwarp();
+    bias[lane_id()] = col < p.n ? to_f32(((const T*)e.bias)[col]) : 0.f;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      const float4 b = *reinterpret_cast<const float4*>(bias + i);
+      v[i] += b.x;
+      v[i + 1] += b.y;
+      v[i + 2] += b.z;
+      v[i + 3] += b.w;
+    }
+  }
+  if (e.q) write_codes(e, p, v);
+  if (e.z) write32<T>(e.z, e.z_ld, p, v);
+  if (e.act != kActNone)
+    with_act(e.act, [&](auto A) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = act_value<decltype(A)::value>(v[i]);
     });
-  return sum;
+  if (e.add) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] += r[i];
+  }
+  write32<T>(e.out, e.out_ld, p, v);
+}
+
+template <typename T>
+__device__ __forceinline__ void finish_slope(float (&v)[32], const GemmEpilogue& e, const Patch& p) {
+  float h[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) h[i] = 0.f;
+  if (e.q) read_codes(e, p, h);
+  else read32<T>(e.z, e.z_ld, p, h);
+  with_act(e.act, [&](auto A) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      float value;
+      v[i] *= act_slope<decltype(A)::value>(h[i], &value);
+      h[i] = value;
+    }
+  });
+  write32<T>(e.out, e.out_ld, p, v);
+  if (e.h) write32<T>(e.h, e.h_ld, p, h);
+  if (e.sums) {
+    if (p.row >= p.m) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0.f;
+    }
+    const float sum = transpose_sum(v);
+    const int col = p.col0 + (int)lane_id();
+    if (col < p.n) e.sums[(long long)(p.row0 >> 5) * p.n + col] = sum;
+  }
 }
 
 // T: type of what the epilogue reads and writes.  SLOPE: the input gradient through the layer before's activation.
+// Clusters of 2 * splits CTAs; with splits 1 the pairs go through tiles in turn, else a cluster has one tile.
 template <typename T, bool SLOPE>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const GemmShape s, GemmEpilogue e) {
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t bars[2 * kMaxStages + 4];
+  __shared__ alignas(16) float bias_room[kEpiWarps][32];
   __shared__ uint32_t tmem_at;
   __shared__ volatile int abort;
   const int warp = (int)(threadIdx.x >> 5);
+  const uint32_t ranks = (uint32_t)(2 * s.splits), rank = blockIdx.x % ranks, half = rank & 1u, split = rank >> 1, leader = rank & ~1u;
+  const uint16_t pair = (uint16_t)(3u << leader);
+  const int first_tile = (int)(blockIdx.x / ranks), step = (int)(gridDim.x / ranks), n_tiles = s.tiles_m * s.tiles_n;
+  const int kb_begin = (int)((long long)s.blocks_k * split / s.splits), kb_end = (int)((long long)s.blocks_k * (split + 1) / s.splits);
+  const int b_rows = s.bn / 2;          // of this CTA's half of B
   uint8_t* base = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
-  const uint32_t a_bytes = (uint32_t)s.a_pieces * kTileM * 128u, stage_bytes = a_bytes + (uint32_t)s.b_pieces * s.bn * 128u;
+  const uint32_t a_bytes = (uint32_t)s.a_pieces * kRows * 128u, stage_bytes = a_bytes + (uint32_t)(s.b_pieces * b_rows) * 128u;
   float* patches = reinterpret_cast<float*>(base + (size_t)stage_bytes * s.stages);
   const uint32_t tiles = smem_addr(base);
   const uint32_t full = smem_addr(bars), empty = full + 8u * kMaxStages, acc_full = empty + 8u * kMaxStages, acc_empty = acc_full + 16u;
@@ -263,45 +451,47 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + 8u * i, 1);
-      mbar_init(acc_empty + 8u * i, kEpiWarps);
+      mbar_init(acc_empty + 8u * i, 2 * kEpiWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&a_map) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&b_map) : "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_at)), "r"(columns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_at)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     tc_fence_before();
   }
   __syncthreads();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_at;
   pdl_begin(e.bias, e.add, e.z, e.q, e.e);
-  const int n_tiles = s.tiles_m * s.tiles_n;
 
-  if (warp == 0) {
-    if (lane_id() == 0) {
+  if (warp == 0 || warp == 2) {   // one for each operand: a copy takes its thread 130 cycles, a block of k 512 with 256 columns
+    if (elect_one()) {
+      const bool is_a = warp == 0;
+      const uint32_t pair_full = mapa(full, leader);
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = (int)blockIdx.x; ok && tile < n_tiles; tile += (int)gridDim.x) {
+      for (int tile = first_tile; ok && tile < n_tiles; tile += step) {
         int tm, tn;
         tile_at(s, tile, &tm, &tn);
-        for (int kb = 0; kb < s.blocks_k; ++kb) {
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
           ok = mbar_wait(empty + 8u * stage, phase ^ 1u, &abort, 1);
           if (!ok) break;
-          mbar_expect(full + 8u * stage, stage_bytes);
-          const uint32_t dst = tiles + (uint32_t)stage * stage_bytes;
-          load_operand(dst, &a_map, s.a_mn, s.a_pieces, kTileM, tm * kTileM, kb * kTileK, full + 8u * stage);
-          load_operand(dst + a_bytes, &b_map, s.b_mn, s.b_pieces, s.bn, tn * s.bn, kb * kTileK, full + 8u * stage);
+          if (is_a && half == 0) mbar_expect(full + 8u * stage, 2u * stage_bytes);   // the pair's
+          const uint32_t dst = tiles + (uint32_t)stage * stage_bytes, bar = pair_full + 8u * stage;
+          if (is_a) load_operand(dst, &a_map, s.a_mn, s.a_pieces, kRows, tm * kTileM + (int)half * kRows, kb * kTileK, bar);
+          else load_operand(dst + a_bytes, &b_map, s.b_mn, s.b_pieces, b_rows, tn * s.bn + (int)half * b_rows, kb * kTileK, bar);
           if (++stage == s.stages) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-      // No arrival is left under way: the consumer has freed every stage.
+      // No copy and no arrival is left under way: the consumer has freed every stage.
       for (int i = 0; ok && i < s.stages; ++i) {
         ok = mbar_wait(empty + 8u * stage, phase ^ 1u, &abort, 5);
         if (++stage == s.stages) {
@@ -309,7 +499,7 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
           phase ^= 1u;
         }
       }
-      if (!ok)   // given up: the copies under way end
+      if (!ok && is_a && half == 0)   // given up: the pair's copies under way end
         for (int i = 0; i < s.stages; ++i) {
           const bool second = i >= stage;   // this stage's last copy belongs to the round before
           const uint64_t t0 = globaltimer_ns();
@@ -318,17 +508,18 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
         }
     }
   } else if (warp == 1) {
-    if (lane_id() == 0) {
+    if (half == 0 && elect_one()) {
       int stage = 0;
       uint32_t phase = 0, list;
       const int products = piece_products(s.a_pieces, s.b_pieces, &list);
-      const uint32_t a_step = s.a_mn ? 2048u : 32u, b_step = s.b_mn ? 2048u : 32u;   // bytes to the next 16 of k
-      const uint32_t a_lead = s.a_mn ? 8192u : 16u, b_lead = s.b_mn ? 8192u : 16u;
+      const uint32_t a_step = s.a_mn ? 2048u / 16 : 32u / 16, b_step = s.b_mn ? 2048u / 16 : 32u / 16;   // to the next 16 of k
+      const uint32_t a_desc = operand_desc(tiles, s.a_mn ? 8192u : 16u), b_desc = operand_desc(tiles + a_bytes, s.b_mn ? 8192u : 16u);
+      const uint32_t a_piece = kRows * 128u / 16, b_piece = (uint32_t)(b_rows * 128) / 16, stage_step = stage_bytes / 16;
       int turn = 0;
       bool ok = true;
-      for (int tile = (int)blockIdx.x; ok && tile < n_tiles; tile += (int)gridDim.x)
-        for (int kb = 0; ok && kb < s.blocks_k; ++turn) {
-          const int acc = turn & 1, stop = min(kb + run, s.blocks_k);
+      for (int tile = first_tile; ok && tile < n_tiles; tile += step)
+        for (int kb = kb_begin; ok && kb < kb_end; ++turn) {
+          const int acc = turn & 1, stop = min(kb + run, kb_end);
           ok = mbar_wait(acc_empty + 8u * acc, ((uint32_t)(turn >> 1) & 1u) ^ 1u, &abort, 2);
           if (!ok) break;
           tc_fence_after();
@@ -338,71 +529,70 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
             ok = mbar_wait(full + 8u * stage, phase, &abort, 3);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t a0 = tiles + (uint32_t)stage * stage_bytes, b0 = a0 + a_bytes;
+            const uint32_t a0 = a_desc + (uint32_t)stage * stage_step, b0 = b_desc + (uint32_t)stage * stage_step;
             for (int i = 0; i < products; ++i) {
-              const uint32_t pair = (list >> (4 * i)) & 15u;
-              const uint32_t a1 = a0 + (pair & 3u) * (kTileM * 128u), b1 = b0 + (pair >> 2) * (uint32_t)(s.bn * 128);
-              const bool to_small = kSplit && pair != 0;
+              const uint32_t at = (list >> (4 * i)) & 15u;
+              const uint32_t a1 = a0 + (at & 3u) * a_piece, b1 = b0 + (at >> 2) * b_piece;
+              const bool to_small = kSplit && at != 0;
               uint32_t on = to_small ? on_small : on_large;
 #pragma unroll
               for (int k = 0; k < kTileK / 16; ++k) {
-                mma(to_small ? small : large, operand_desc(a1 + k * a_step, a_lead), operand_desc(b1 + k * b_step, b_lead), s.idesc, on);
+                mma(to_small ? small : large, a1 + k * a_step, b1 + k * b_step, s.idesc, on);
                 on = 1;
               }
               if (to_small) on_small = 1;
               else on_large = 1;
             }
-            mma_commit(empty + 8u * stage);
+            mma_commit(empty + 8u * stage, pair);
             if (++stage == s.stages) {
               stage = 0;
               phase ^= 1u;
             }
           }
           if (!ok) break;
-          mma_commit(acc_full + 8u * acc);
+          mma_commit(acc_full + 8u * acc, pair);
         }
       if (!ok) {   // products in flight end before TMEM is given back: nobody else arrives on acc_full any more
         const uint32_t last = acc_full + 8u * (turn & 1);
-        mma_commit(last);
+        mma_commit(last, pair);
         const uint64_t t0 = globaltimer_ns();
         while (!mbar_try(last, (uint32_t)(turn >> 1) & 1u) && globaltimer_ns() - t0 < 100000000ull) {
         }
       }
     }
   } else if (warp >= 4) {
-    const int quad = warp & 3, half = (warp - 4) >> 2;
-    float* patch = patches + (size_t)(warp - 4) * 32 * kStagePitch;
-    const int lane = (int)lane_id();
+    const int quad = warp & 3, side = (warp - 4) >> 2, lane = (int)lane_id();
+    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16), pair_acc_empty = mapa(acc_empty, leader);
+    Patch p{patches + (size_t)(warp - 4) * 32 * kPatchPitch, 0, 0, 0, s.m, s.n, s.wide != 0};
     int turn = 0;
     bool ok = true;
-    for (int tile = (int)blockIdx.x; ok && tile < n_tiles; tile += (int)gridDim.x) {
+    for (int tile = first_tile; ok && tile < n_tiles; tile += step) {
       int tm, tn;
       tile_at(s, tile, &tm, &tn);
-      const int row0 = tm * kTileM + quad * 32;
-      // 32 columns of this warp's 32 rows, a row per lane
-      auto finish = [&](int c, const auto& v) {
-        const int col0 = tn * s.bn + c;
-        if (row0 >= s.m || col0 >= s.n) return;
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) patch[lane * kStagePitch + i] = v[i];
-        __syncwarp();
-        const Patch p{patch, row0, col0 + lane, min(32, s.m - row0), col0 + lane < s.n};
-        if constexpr (SLOPE) {
-          const float sum = finish_slope<T>(p, s, e);
-          if (e.sums && p.inside) e.sums[(size_t)(tm * 4 + quad) * s.n + p.col] = sum;
-        } else {
-          finish_forward<T>(p, s, e);
-        }
+      p.row0 = tm * kTileM + (int)half * kRows + quad * 32;
+      p.row = p.row0 + lane;
+      const bool some = p.row0 < s.m;   // rows of this warp
+      auto finish = [&](int c, float (&v)[32]) {
+        p.col0 = tn * s.bn + c;
+        if (!some || p.col0 >= s.n) return;
+        if constexpr (SLOPE) finish_slope<T>(v, e, p);
+        else finish_forward<T>(v, bias_room[warp - 4], e, p);
       };
-      const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+      // Accumulators of one of the splits: 16-byte granules, permuted within a row so that neither the lanes of a write
+      // nor those of a read share banks.
+      float* sums = reinterpret_cast<float*>(base);
+      auto put = [&](int c, const float (&v)[32]) {
+        float4* at = reinterpret_cast<float4*>(sums + (size_t)(c / 32) * kRows * 32 + (quad * 32 + lane) * 32);
+#pragma unroll
+        for (int g = 0; g < 8; ++g) at[g ^ (lane & 7)] = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+      };
       if constexpr (kSplit) {   // bn is 128 at most: two patches a warp
         float sum[2][32];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[j][i] = 0.f;
-        for (int kb = 0; kb < s.blocks_k; kb += run, ++turn) {
+        for (int kb = kb_begin; kb < kb_end; kb += run, ++turn) {
           const int acc = turn & 1;
           ok = mbar_wait(acc_full + 8u * acc, (uint32_t)(turn >> 1) & 1u, &abort, 4);
           if (!ok) break;
@@ -410,7 +600,7 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
           tc_fence_after();
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const int c = half * 32 + j * 64;
+            const int c = side * 32 + j * 64;
             if (c < s.bn) {
               float large[32], small[32];
               tmem_load32(lanes + (uint32_t)acc * acc_columns + (uint32_t)c, large);
@@ -421,26 +611,32 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty + 8u * acc);
+          if (lane == 0) mbar_arrive_remote(pair_acc_empty + 8u * acc);
         }
         if (!ok) break;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (half * 32 + j * 64 < s.bn) finish(half * 32 + j * 64, sum[j]);
+        for (int j = 0; j < 2; ++j) {
+          const int c = side * 32 + j * 64;
+          if (c < s.bn) {
+            if (s.splits > 1) put(c, sum[j]);
+            else finish(c, sum[j]);
+          }
+        }
       } else {
         const int acc = turn & 1;
         ok = mbar_wait(acc_full + 8u * acc, (uint32_t)(turn >> 1) & 1u, &abort, 4);
         if (!ok) break;
         __syncwarp();
         tc_fence_after();
-        for (int c = half * 32; c < s.bn; c += 64) {
+        for (int c = side * 32; c < s.bn; c += 64) {
           float v[32];
           tmem_load32(lanes + (uint32_t)acc * acc_columns + (uint32_t)c, v);
-          finish(c, v);
+          if (s.splits > 1) put(c, v);
+          else finish(c, v);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty + 8u * acc);
+        if (lane == 0) mbar_arrive_remote(pair_acc_empty + 8u * acc);
         ++turn;
       }
     }
@@ -448,8 +644,44 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  cluster_sync();   // every CTA's sums lie in its shared memory; nothing of the pair's products is under way
+  if (s.splits > 1 && warp >= 4 && !abort) {
+    // This CTA finishes every splits-th 32 columns of its rows, adding the pairs' sums up in their order.
+    const int quad = warp & 3, side = (warp - 4) >> 2, lane = (int)lane_id();
+    int tm, tn;
+    tile_at(s, first_tile, &tm, &tn);
+    Patch p{patches + (size_t)(warp - 4) * 32 * kPatchPitch, 0, 0, tm * kTileM + (int)half * kRows + quad * 32, s.m, s.n, s.wide != 0};
+    p.row = p.row0 + lane;
+    if (p.row0 < s.m)
+      for (int c = ((int)split + side * s.splits) * 32; c < s.bn; c += 64 * s.splits) {
+        p.col0 = tn * s.bn + c;
+        if (p.col0 >= s.n) break;
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        const uint32_t at = tiles + (uint32_t)((c / 32) * kRows * 32 + (quad * 32 + lane) * 32) * 4u;
+        for (int k = 0; k < s.splits; ++k) {
+          const uint32_t from = mapa(at, (uint32_t)(2 * k) + half);
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            float4 x;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(from + (uint32_t)(g ^ (lane & 7)) * 16u));
+            v[4 * g] += x.x;
+            v[4 * g + 1] += x.y;
+            v[4 * g + 2] += x.z;
+            v[4 * g + 3] += x.w;
+          }
+        }
+        if constexpr (SLOPE) finish_slope<T>(v, e, p);
+        else finish_forward<T>(v, bias_room[warp - 4], e, p);
+      }
+  }
+  if (s.splits > 1) {   // shared memory stays until all have read it
+    __syncwarp();
+    cluster_sync();
+  }
   tc_fence_after();
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------
@@ -491,37 +723,53 @@ inline bool operand_ok(const Operand& o) {
   return o.p && (uintptr_t)o.p % 16 == 0 && o.ld > 0 && o.ld % 8 == 0 && (o.pieces == 1 || (o.pieces == 3 && o.piece_stride > 0 && o.piece_stride % 8 == 0));
 }
 
-// Columns of a tile: the width with the least work on the longest-running SM.
-inline int pick_bn(long long m, long long n, int most, int sms) {
-  int best = 64;
+// Tiles and splits.  A pair takes about 2 * bn cycles for the products of a block of k (times six with pieces), at
+// least 330 for its copies, and some 24 a column for a tile's last epilogue; more pairs to a tile cost 1500 cycles
+// for joining their sums.  The choice is the one whose busiest pair is done first.
+struct GemmPlan {
+  int bn, splits;
+};
+inline GemmPlan plan_gemm(long long m, long long n, int blocks_k, int products, int most, int sms) {
+  GemmPlan best{128, 1};
   long long least = -1;
-  for (int bn = 64; bn <= most; bn *= 2) {
+  const int pairs = sms / 2;
+  for (int bn = most; bn >= 128; bn /= 2) {
     const long long tiles = ((m + kTileM - 1) / kTileM) * ((n + bn - 1) / bn);
-    const long long cost = ((tiles + sms - 1) / sms) * (bn + 32);
-    if (least < 0 || cost <= least) {
-      least = cost;
-      best = bn;
+    const long long block = 2 * bn * products > 330 ? 2 * bn * products : 330;
+    for (int splits = 1; splits <= kMaxSplits; splits *= 2) {
+      if (splits > 1 && (blocks_k < 4 * splits || tiles * splits > pairs)) break;
+      const long long rounds = (tiles * splits + pairs - 1) / pairs;
+      const long long cost = rounds * ((blocks_k + splits - 1) / splits) * block + bn * 24 / splits + (splits > 1 ? 1500 : 0);
+      if (least < 0 || cost < least) {
+        least = cost;
+        best = GemmPlan{bn, splits};
+      }
     }
   }
   return best;
 }
 
+inline bool on16(const void* p, long long ld, int elem) { return !p || ((uintptr_t)p % 16 == 0 && ld * elem % 16 == 0); }
+
 template <typename T>
 cudaError_t launch_gemm(bool slope, int grid, size_t shared, cudaStream_t stream, const CUtensorMap& a, const CUtensorMap& b, const GemmShape& s,
                         const GemmEpilogue& e) {
   auto go = [&](auto kernel) {
-    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared - 1024);
+    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared - kStaticShared);
     if (err != cudaSuccess) return err;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kGemmThreads);
     cfg.dynamicSmemBytes = shared;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)(2 * s.splits);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kernel, a, b, s, e);
   };
   return slope ? go(k8_gemm<T, true>) : go(k8_gemm<T, false>);
@@ -549,7 +797,7 @@ extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long lo
                            const void* add, long long add_ld, int act, int slope, void* z, long long z_ld, signed char* q, long long q_ld, unsigned char* e8,
                            long long e_ld, void* h, long long h_ld, float* sums, void* db, void* stream_) {
   const Operand oa{a, a_ld, a_pieces, a_stride, a_mn != 0}, ob{b, b_ld, b_pieces, b_stride, b_mn != 0};
-  if (m <= 0 || n <= 0 || k <= 0 || !out || act < 0 || act >= kActCount || !operand_ok(oa) || !operand_ok(ob) || (q && !e8) || (q && !slope && q_ld < (n + kBlock8 - 1) / kBlock8 * kBlock8) || (sums == nullptr) != (db == nullptr))
+  if (m <= 0 || n <= 0 || k <= 0 || !out || act < 0 || act >= kActCount || !operand_ok(oa) || !operand_ok(ob) || (q && !e8) || (q && !slope && (q_ld < (n + kBlock8 - 1) / kBlock8 * kBlock8 || q_ld % 16 || (uintptr_t)q % 16)) || (sums == nullptr) != (db == nullptr))
     return GTK_ERR_ARG;
   if (m > 0x7fffff00LL || n > 0x7fffff00LL || k > 0x7fffff00LL) return GTK_ERR_UNSUPPORTED;
   const DeviceInfo* info = gtk_device_info();
@@ -562,21 +810,27 @@ extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long lo
   s.b_pieces = b_pieces;
   s.a_mn = oa.mn_major;
   s.b_mn = ob.mn_major;
-  s.bn = pick_bn(m, n, a_pieces * b_pieces > 1 ? 128 : 256, info->sms);
   s.tiles_m = (int)((m + kTileM - 1) / kTileM);
-  s.tiles_n = (int)((n + s.bn - 1) / s.bn);
   s.blocks_k = (int)((k + kTileK - 1) / kTileK);
+  const GemmPlan plan = plan_gemm(m, n, s.blocks_k, a_pieces * b_pieces == 9 ? 6 : a_pieces * b_pieces, type == kF32 ? 128 : kMaxBn, info->sms);
+  s.bn = plan.bn;
+  s.splits = plan.splits;
+  s.tiles_n = (int)((n + s.bn - 1) / s.bn);
   if ((long long)s.tiles_m * s.tiles_n > 0x3fffffffLL) return GTK_ERR_UNSUPPORTED;
-  const int stage_bytes = a_pieces * kTileM * 128 + b_pieces * s.bn * 128;
-  const int fixed = 1024 + kEpiBytes;
-  s.stages = (kMaxShared - 1024 - fixed) / stage_bytes;
+  const int elem = elem_bytes(type);
+  s.wide = n * elem % 16 == 0 && on16(out, out_ld, elem) && on16(add, add_ld, elem) && on16(z, z_ld, elem) && on16(h, h_ld, elem) &&
+           (!q || !slope || (n % 16 == 0 && on16(q, q_ld, 1)));
+  const int stage_bytes = a_pieces * kRows * 128 + b_pieces * s.bn / 2 * 128;
+  const int fixed = 1024 + (s.wide ? 0 : kPatchBytes);
+  s.stages = (kMaxShared - kStaticShared - fixed) / stage_bytes;
   if (s.stages > kMaxStages) s.stages = kMaxStages;
   const uint32_t fmt = half ? 0u : 1u;
-  s.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)s.a_mn << 15) | ((uint32_t)s.b_mn << 16) | ((uint32_t)(s.bn >> 3) << 17) | ((kTileM >> 4) << 24);
+  s.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)s.a_mn << 15) | ((uint32_t)s.b_mn << 16) | ((uint32_t)(s.bn >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
   CUtensorMap am, bm;
-  if (!encode(&am, oa, half, m, k, kTileM) || !encode(&bm, ob, half, n, k, s.bn)) return GTK_ERR_CUDA;
+  if (!encode(&am, oa, half, m, k, kRows) || !encode(&bm, ob, half, n, k, s.bn / 2)) return GTK_ERR_CUDA;
   const GemmEpilogue ep{out, out_ld, bias, add, add_ld, act, z, z_ld, q, q_ld, e8, e_ld, h, h_ld, sums};
-  const int tiles = s.tiles_m * s.tiles_n, grid = tiles < info->sms ? tiles : info->sms;
+  const int tiles = s.tiles_m * s.tiles_n, pairs = info->sms / 2;
+  const int grid = 2 * (s.splits > 1 ? tiles * s.splits : tiles < pairs ? tiles : pairs);
   const size_t shared = (size_t)stage_bytes * s.stages + fixed;
   const cudaStream_t stream = (cudaStream_t)stream_;
   cudaError_t err;

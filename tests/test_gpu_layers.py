@@ -401,13 +401,15 @@ def test_matrices_over_2_31_elements():
     del y
     w = _randn(40, 1024, dtype=torch.bfloat16, seed=1)
     y = linear_forward(x, w)[0]
-    assert torch.equal(y[-64:], linear_forward(x[-64:], w)[0])
+    X, W = x[-64:].double(), w.double()
+    _within(y[-64:], X @ W.t(), _c(1024, x.dtype) * (X.abs() @ W.abs().t()), "y")
     del x, y
     a, w = _randn(rows, 8, dtype=torch.bfloat16), _randn(32768, 8, dtype=torch.bfloat16, seed=1)
     y = linear_forward(a, w)[0]
     assert torch.equal(y[-64:], linear_forward(a[-64:], w)[0])
     dx, dw, _ = linear_backward(y, a, w)
-    assert torch.equal(dx[-64:], linear_backward(y[-64:], a[-64:], w)[0])
+    Y, W = y[-64:].double(), w.double()
+    _within(dx[-64:], Y @ W, _c(32768, dx.dtype) * (Y.abs() @ W.abs()), "dx")   # k is split differently over more rows
     want = y[:, -64:].double().t() @ a.double()
     assert float((dw[-64:] - want).norm() / want.norm()) < 1e-2
 
