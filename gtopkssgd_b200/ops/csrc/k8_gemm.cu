@@ -30,6 +30,8 @@
 // after its copies and products in flight, and TMEM is freed.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "colsum.cuh"
 #include "common.cuh"
 #include "host_api.h"
@@ -578,13 +580,12 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
         if constexpr (SLOPE) finish_slope<T>(v, e, p);
         else finish_forward<T>(v, bias_room[warp - 4], e, p);
       };
-      // Accumulators of one of the splits: 16-byte granules, permuted within a row so that neither the lanes of a write
-      // nor those of a read share banks.
-      float* sums = reinterpret_cast<float*>(base);
+      // Accumulators of one of the splits, 16 bytes of every lane side by side: the lanes of a read from another CTA
+      // have to be neighbours (rows 128 bytes apart took 15 us for 128 KB).
       auto put = [&](int c, const float (&v)[32]) {
-        float4* at = reinterpret_cast<float4*>(sums + (size_t)(c / 32) * kRows * 32 + (quad * 32 + lane) * 32);
+        float4* at = reinterpret_cast<float4*>(base) + (size_t)((c / 32) * 4 + quad) * 256 + lane;
 #pragma unroll
-        for (int g = 0; g < 8; ++g) at[g ^ (lane & 7)] = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+        for (int g = 0; g < 8; ++g) at[g * 32] = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
       };
       if constexpr (kSplit) {   // bn is 128 at most: two patches a warp
         float sum[2][32];
@@ -659,17 +660,22 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = 0.f;
-        const uint32_t at = tiles + (uint32_t)((c / 32) * kRows * 32 + (quad * 32 + lane) * 32) * 4u;
+        const uint32_t at = tiles + (uint32_t)(((c / 32) * 4 + quad) * 256 + lane) * 16u;
         for (int k = 0; k < s.splits; ++k) {
           const uint32_t from = mapa(at, (uint32_t)(2 * k) + half);
+          float4 x[8];   // all on their way before the first is used
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(x[g].x), "=f"(x[g].y), "=f"(x[g].z), "=f"(x[g].w)
+                         : "r"(from + (uint32_t)g * 512u)
+                         : "memory");
 #pragma unroll
           for (int g = 0; g < 8; ++g) {
-            float4 x;
-            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(from + (uint32_t)(g ^ (lane & 7)) * 16u));
-            v[4 * g] += x.x;
-            v[4 * g + 1] += x.y;
-            v[4 * g + 2] += x.z;
-            v[4 * g + 3] += x.w;
+            v[4 * g] += x[g].x;
+            v[4 * g + 1] += x[g].y;
+            v[4 * g + 2] += x[g].z;
+            v[4 * g + 3] += x[g].w;
           }
         }
         if constexpr (SLOPE) finish_slope<T>(v, e, p);
@@ -723,23 +729,52 @@ inline bool operand_ok(const Operand& o) {
   return o.p && (uintptr_t)o.p % 16 == 0 && o.ld > 0 && o.ld % 8 == 0 && (o.pieces == 1 || (o.pieces == 3 && o.piece_stride > 0 && o.piece_stride % 8 == 0));
 }
 
-// Tiles and splits.  A pair takes about 2 * bn cycles for the products of a block of k (times six with pieces), at
-// least 330 for its copies, and some 24 a column for a tile's last epilogue; more pairs to a tile cost 1500 cycles
-// for joining their sums.  The choice is the one whose busiest pair is done first.
+// Pairs that run side by side in clusters of `splits` of them (74, 66 and 56 of 1, 2 and 4 on B200: a cluster lies within
+// one group of SMs).  Asked once per device.
+template <typename Kernel>
+int pairs_of(Kernel kernel, int splits, const DeviceInfo* info) {
+  static std::atomic<int> known[64][kMaxSplits + 1];
+  std::atomic<int>& slot = known[info->device][splits];
+  int pairs = slot.load(std::memory_order_relaxed);
+  if (pairs) return pairs;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(info->sms / (2 * splits) * 2 * splits));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = kMaxShared - kStaticShared;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)(2 * splits);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared - kStaticShared) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters <= 0) {
+    cudaGetLastError();
+    clusters = 1;
+  }
+  pairs = clusters * splits;
+  slot.store(pairs, std::memory_order_relaxed);
+  return pairs;
+}
+
+// Tiles and splits.  In cycles, a pair takes about 2 * bn for the products of a block of k (times six with pieces), at
+// least 330 for its copies, 24 a column for a tile's last epilogue and 3000 + 16 a column for joining several pairs'
+// sums (256 x 256: 3.6 us with two, 4.8 with four).  The choice is the one whose busiest pair is done first.
 struct GemmPlan {
   int bn, splits;
 };
-inline GemmPlan plan_gemm(long long m, long long n, int blocks_k, int products, int most, int sms) {
+inline GemmPlan plan_gemm(long long m, long long n, int blocks_k, int products, int most, const DeviceInfo* info) {
   GemmPlan best{128, 1};
   long long least = -1;
-  const int pairs = sms / 2;
   for (int bn = most; bn >= 128; bn /= 2) {
     const long long tiles = ((m + kTileM - 1) / kTileM) * ((n + bn - 1) / bn);
     const long long block = 2 * bn * products > 330 ? 2 * bn * products : 330;
-    for (int splits = 1; splits <= kMaxSplits; splits *= 2) {
+    for (int splits = 1; splits <= kMaxSplits; ++splits) {
+      const int pairs = pairs_of(k8_gemm<__nv_bfloat16, false>, splits, info);
       if (splits > 1 && (blocks_k < 4 * splits || tiles * splits > pairs)) break;
       const long long rounds = (tiles * splits + pairs - 1) / pairs;
-      const long long cost = rounds * ((blocks_k + splits - 1) / splits) * block + bn * 24 / splits + (splits > 1 ? 1500 : 0);
+      const long long cost = rounds * ((blocks_k + splits - 1) / splits) * block + bn * 24 / splits + (splits > 1 ? 3000 + 16 * bn : 0);
       if (least < 0 || cost < least) {
         least = cost;
         best = GemmPlan{bn, splits};
@@ -812,7 +847,7 @@ extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long lo
   s.b_mn = ob.mn_major;
   s.tiles_m = (int)((m + kTileM - 1) / kTileM);
   s.blocks_k = (int)((k + kTileK - 1) / kTileK);
-  const GemmPlan plan = plan_gemm(m, n, s.blocks_k, a_pieces * b_pieces == 9 ? 6 : a_pieces * b_pieces, type == kF32 ? 128 : kMaxBn, info->sms);
+  const GemmPlan plan = plan_gemm(m, n, s.blocks_k, a_pieces * b_pieces == 9 ? 6 : a_pieces * b_pieces, type == kF32 ? 128 : kMaxBn, info);
   s.bn = plan.bn;
   s.splits = plan.splits;
   s.tiles_n = (int)((n + s.bn - 1) / s.bn);
