@@ -16,13 +16,14 @@ import torch
 
 from . import layers_oracle as oracle
 from . import lib as _lib
-from .select import _ptr, _raw_stream
+from .select import _FLOAT, _ptr, _raw_stream
 
 BLOCK = oracle.BLOCK
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # ElemType of the kernels
 
 _lines = {}
+_current_device = getattr(torch._C, "_cuda_getDevice", None)   # (torch.cuda.current_device without its checks)
 
 
 def lines(name: str) -> int:
@@ -60,6 +61,15 @@ def same(like: torch.Tensor, /, **others) -> None:
             raise ValueError("%s is %s on %s instead of %s on %s" % (name, t.dtype, t.device, like.dtype, like.device))
 
 
+def parameter(like: torch.Tensor, name: str, t: Optional[torch.Tensor], n: int) -> Optional[torch.Tensor]:
+    """A vector of n entries of the type and device of ``like``, its entries side by side; None where absent."""
+    if t is None or (t.dtype is like.dtype and t.dim() == 1 and t.size(0) == n and t.is_contiguous() and t.device == like.device):
+        return t
+    same(like, **{name: t})
+    shaped(name, t, n)
+    return t.contiguous()
+
+
 def shaped(name: str, t: Optional[torch.Tensor], *shape: int) -> None:
     if t is not None and tuple(t.shape) != shape:
         raise ValueError("%s has shape %s instead of %s" % (name, tuple(t.shape), shape))
@@ -76,10 +86,6 @@ def matrix(t: torch.Tensor) -> torch.Tensor:
     return m if m.stride(1) == 1 or m.size(1) == 1 else m.contiguous()
 
 
-def vector(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return t if t is None or t.is_contiguous() else t.contiguous()
-
-
 def ld(m: torch.Tensor) -> int:
     """Elements from one row to the next; of a single row, whose stride says nothing, its own length."""
     return m.stride(0) if m.size(0) > 1 else m.size(1)
@@ -88,29 +94,29 @@ def ld(m: torch.Tensor) -> int:
 def stream_of(t: torch.Tensor) -> int:
     """The current stream of the tensor's device, which has to be the current one: launches go there."""
     index = t.get_device()
-    if index != torch._C._cuda_getDevice():
-        raise ValueError("the tensors are on cuda:%d, the current device is cuda:%d" % (index, torch._C._cuda_getDevice()))
+    if index != _current_device():
+        raise ValueError("the tensors are on cuda:%d, the current device is cuda:%d" % (index, _current_device()))
     return _raw_stream(index)
 
 
-def colsum(dy: torch.Tensor, activation: str = "none", z=None, want_dz: bool = False, want_sum: bool = True):
-    """(dz, sum of dz over the rows) with dz = dy * act'(z), over matrices; each None where not wanted."""
-    code = act_of(activation)
+def colsum(dy: torch.Tensor, activation: int = 0, z=None, want_dz: bool = False, want_sum: bool = True):
+    """(dz, sum of dz over the rows) with dz = dy * act'(z), over CUDA matrices; each None where not wanted.
+    ``activation``: its number."""
     rows, cols = dy.shape
-    dz = torch.empty((rows, cols), dtype=dy.dtype, device=dy.device) if want_dz else None
-    db = torch.empty(cols, dtype=dy.dtype, device=dy.device) if want_sum else None
+    dz = dy.new_empty((rows, cols)) if want_dz else None
+    db = dy.new_empty(cols) if want_sum else None
     if rows == 0 or cols == 0:
         if db is not None:
             db.zero_()
         return dz, db
-    if code == 0:
+    if activation == 0:
         zp, zld, e, eld = None, 0, None, 0
-    elif isinstance(z, Activation8):
+    elif type(z) is Activation8:
         zp, zld, e, eld = z.q.data_ptr(), ld(z.q), z.e.data_ptr(), ld(z.e)
     else:
         zp, zld, e, eld = z.data_ptr(), ld(z), None, 0
-    partial = torch.empty((lines("gtk_k7_act_lines"), cols), dtype=torch.float32, device=dy.device) if want_sum else None
-    err = _lib.calls().gtk_k7_act_backward(TYPES[dy.dtype], dy.data_ptr(), ld(dy), zp, zld, e, eld, code, _ptr(dz), cols, _ptr(db),
+    partial = dy.new_empty((min(lines("gtk_k7_act_lines"), rows), cols), dtype=_FLOAT) if want_sum else None
+    err = _lib.calls().gtk_k7_act_backward(TYPES[dy.dtype], dy.data_ptr(), ld(dy), zp, zld, e, eld, activation, _ptr(dz), cols, _ptr(db),
                                            _ptr(partial), rows, cols, stream_of(dy))
     if err:
         _lib.check(err, "gtk_k7_act_backward")
@@ -150,24 +156,31 @@ class Activation8:
         return self.q.size(0) * (ld(self.q) + ld(self.e))
 
     @staticmethod
-    def empty(rows: int, cols: int, dtype: torch.dtype, device, shape=None) -> "Activation8":
-        """Uninitialised; rows are padded to whole blocks, which the kernels store at once."""
+    def empty(like: torch.Tensor, rows: int, cols: int, shape: Tuple[int, ...]) -> "Activation8":
+        """Uninitialised, for a tensor of the type and device of ``like``; rows are padded to whole blocks, which the
+        kernels store at once."""
         blocks = -(-cols // BLOCK)
-        q = torch.empty((rows, blocks * BLOCK), dtype=torch.int8, device=device)[:, :cols]
-        return Activation8(q, torch.empty((rows, blocks), dtype=torch.uint8, device=device), dtype, shape)
+        kept = Activation8.__new__(Activation8)   # consistent by construction
+        q = like.new_empty((rows, blocks * BLOCK), dtype=torch.int8)
+        kept.q = q if cols == blocks * BLOCK else q[:, :cols]
+        kept.e = like.new_empty((rows, blocks), dtype=torch.uint8)
+        kept.dtype, kept.shape = like.dtype, shape
+        return kept
 
     @staticmethod
     def keep(x: torch.Tensor) -> "Activation8":
         """x in 8 bits."""
         code = type_of(x, "Activation8.keep")
-        m = matrix(x.detach())
+        m = matrix(x.detach() if x.requires_grad else x)
         if not m.is_cuda:
             q, e = oracle.keep8(m)
             return Activation8(q, e, x.dtype, x.shape)
-        kept = Activation8.empty(m.size(0), m.size(1), x.dtype, x.device, x.shape)
-        if m.numel():
-            err = _lib.calls().gtk_k7_keep(code, m.data_ptr(), ld(m), kept.q.data_ptr(), kept.e.size(1) * BLOCK, kept.e.data_ptr(), kept.e.size(1),
-                                           m.size(0), m.size(1), stream_of(m))
+        rows, cols = m.shape
+        kept = Activation8.empty(m, rows, cols, tuple(x.shape))
+        if rows and cols:
+            blocks = -(-cols // BLOCK)
+            err = _lib.calls().gtk_k7_keep(code, m.data_ptr(), ld(m), kept.q.data_ptr(), blocks * BLOCK, kept.e.data_ptr(), blocks, rows, cols,
+                                           stream_of(m))
             if err:
                 _lib.check(err, "gtk_k7_keep")
         return kept
@@ -177,7 +190,7 @@ class Activation8:
         rows, cols = self.q.shape
         if not self.q.is_cuda:
             return oracle.restore8(self.q, self.e, self.dtype).view(self.shape)
-        out = torch.empty(self.shape, dtype=self.dtype, device=self.q.device)
+        out = self.q.new_empty(self.shape, dtype=self.dtype)
         if out.numel():
             err = _lib.calls().gtk_k7_stage(TYPES[self.dtype], self.q.data_ptr(), ld(self.q), self.e.data_ptr(), ld(self.e), None, None, None, None, 0,
                                             0, out.data_ptr(), cols, 0, rows, cols, cols, stream_of(self.q))
@@ -188,13 +201,13 @@ class Activation8:
     def backward(self, dy: torch.Tensor, activation: str) -> Tuple[torch.Tensor, torch.Tensor]:
         """The kept tensor is z, an activation's input: (dz, db) with dz = dy * act'(z), and db the sum of dz over
         all but the last axis, the gradient of a bias that was added to make z."""
-        act_of(activation)
-        if tuple(dy.shape) != self.shape or dy.dtype != self.dtype or dy.device != self.device:
+        code = act_of(activation)
+        if dy.shape != self.shape or dy.dtype != self.dtype or dy.device != self.q.device:
             raise ValueError("the gradient is %s %s on %s, what was kept %s %s on %s"
                              % (tuple(dy.shape), dy.dtype, dy.device, self.shape, self.dtype, self.device))
         m = matrix(dy)
         if not m.is_cuda:
             dz, db = oracle.act_backward(m, oracle.values8(self.q, self.e, oracle.wide(m).dtype), activation)
             return dz.to(dy.dtype).view(self.shape), db.to(dy.dtype)
-        dz, db = colsum(m, activation, self, want_dz=True)
-        return dz.view(self.shape), db
+        dz, db = colsum(m, code, self, want_dz=True)
+        return dz if len(self.shape) == 2 else dz.view(self.shape), db

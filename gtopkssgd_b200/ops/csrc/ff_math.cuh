@@ -28,22 +28,56 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// N elements that move with one access of sizeof(T) * N bytes.
+// N elements that move with one access of sizeof(T) * N bytes (two or more of 16 where that is longer).
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Vec {
+struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Vec {
   T v[N];
 };
+// Two neighbours of a 16-bit type at a time: an instruction each to unpack, one for both to pack.
+__device__ __forceinline__ void unpack2(uint32_t u, float* a, float* b, __nv_bfloat16) {
+  *a = __uint_as_float(u << 16);
+  *b = __uint_as_float(u & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack2(uint32_t u, float* a, float* b, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+  *a = f.x;
+  *b = f.y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+template <typename T, int N>
+__device__ __forceinline__ void to_f32(const Vec<T, N>& x, float (&out)[N]) {
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) unpack2(w[i / 2], &out[i], &out[i + 1], T{});
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = to_f32(x.v[i]);
+  }
+}
 template <typename T, int N>
 __device__ __forceinline__ void load_f32(const T* p, float (&out)[N]) {
   const Vec<T, N> x = *reinterpret_cast<const Vec<T, N>*>(p);
-#pragma unroll
-  for (int i = 0; i < N; ++i) out[i] = to_f32(x.v[i]);
+  to_f32<T, N>(x, out);
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_f32(T* p, const float (&in)[N]) {
   Vec<T, N> x;
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
-  for (int i = 0; i < N; ++i) x.v[i] = from_f32<T>(in[i]);
+    for (int i = 0; i < N; i += 2) w[i / 2] = pack2(in[i], in[i + 1], T{});
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x.v[i] = from_f32<T>(in[i]);
+  }
   *reinterpret_cast<Vec<T, N>*>(p) = x;
 }
 

@@ -101,6 +101,7 @@ int gtk_k7_stage(int type, const void* src, long long src_ld, const unsigned cha
                  const float* mean, const float* rstd, const void* g, const void* b, int act, int out_kind, void* out,
                  long long out_ld, long long piece_stride, long long rows, long long cols, long long pitch,
                  void* stream);
+int gtk_k7_pack(gtk_addresses list, void* stream);
 int gtk_k7_act_lines(void);
 int gtk_k7_act_backward(int type, const void* dy, long long dy_ld, const void* z, long long z_ld,
                         const unsigned char* e, long long e_ld, int act, void* dz, long long dz_ld, void* db,

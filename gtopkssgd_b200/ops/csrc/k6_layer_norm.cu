@@ -5,8 +5,11 @@
 //
 // Bound by memory: the forward pass reads x and writes y, the backward pass reads dy and x and writes dx.  A row is
 // read once and stays in registers (the variance is summed over the centred values, not from sums of squares).  A
-// group of warps takes a row.  In the backward pass the groups go through rows in turn, the column sums of a
-// thread's own columns stay in its registers all along, the groups of a CTA join theirs in shared memory, and
+// group of warps takes a row, 16 elements a thread (8 where rows are few), and goes through rows in turn; the rows to
+// come are copied to shared memory meanwhile, every thread its own elements (no thread waits for another's copies).
+// With 8 elements a thread the work per thread and row - sums across lanes and warps, addresses - took 37
+// instructions an element forward and 70 backward, and their issue, not memory, set the time.  In the backward pass the column sums of
+// a thread's own columns stay in its registers all along, the groups of a CTA join theirs in shared memory, and
 // col_finish adds up one line per CTA.
 #include "colsum.cuh"
 #include "common.cuh"
@@ -17,10 +20,11 @@ namespace gtk {
 
 constexpr int kNormMaxWarps = 32;
 
-// Sum of N values over the threads of a group of `warps` warps (named barrier `bar`; scratch: 2 x N x 32 floats per
-// group, used in turn so that one barrier per sum is enough).
+// Sums of N values over the threads of a group of warps.  All groups of the CTA take part at the same time: a barrier
+// whose number is known only at run time makes the compiler reserve all 16, and four such CTAs fill an SM.  Scratch:
+// N floats a warp, zeros past the last warp up to a multiple of 4; used in turn, so that one barrier a sum is enough.
 template <int N>
-__device__ __forceinline__ void group_sum(float (&v)[N], int warps, int warp, int bar, float* scratch) {
+__device__ __forceinline__ void group_sum(float (&v)[N], int warps, int warp, float* scratch) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
@@ -28,14 +32,14 @@ __device__ __forceinline__ void group_sum(float (&v)[N], int warps, int warp, in
   if (warps == 1) return;
   if (lane_id() == 0)
 #pragma unroll
-    for (int i = 0; i < N; ++i) scratch[i * kNormMaxWarps + warp] = v[i];
-  asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(warps * 32) : "memory");
+    for (int i = 0; i < N; ++i) scratch[warp * N + i] = v[i];
+  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float s = (int)lane_id() < warps ? scratch[i * kNormMaxWarps + lane_id()] : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    v[i] = s;
+  for (int i = 0; i < N; ++i) v[i] = 0.f;
+  for (int k = 0; k < warps * N; k += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(scratch + k);
+    v[0] += N == 1 ? (x.x + x.y) + (x.z + x.w) : x.x + x.z;
+    if constexpr (N == 2) v[1] += x.y + x.w;
   }
 }
 
@@ -43,68 +47,151 @@ struct NormShape {
   long long rows, x_ld, dy_ld, add_ld;   // leading dimensions in elements
   int cols;
   int warps;                             // of a group
+  int depth;                             // rows of a group under way
   float eps;
 };
 
-// blockDim = (32 * warps, groups).  NV vectors of VEC elements per thread cover the row.
+// A thread's part of a row, as it lies in memory: NV vectors of VEC elements.
 template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(1024) k6_norm_forward(const T* x, const T* w, const T* b, T* y, float* mean, float* rstd, NormShape s) {
-  __shared__ float scratch[8][2][kNormMaxWarps];
-  pdl_begin(x, w, b);
-  const int threads = s.warps * 32, at = (int)threadIdx.x, group = (int)threadIdx.y;
-  const long long row = (long long)blockIdx.x * blockDim.y + group;
-  if (row >= s.rows) return;   // the whole group
-  const T* xr = x + row * s.x_ld;
-  float v[NV][VEC];
-  float sum[1] = {0.f};
+struct RowRaw {
+  Vec<T, VEC> v[NV];
+};
+
+// The rows to come.  Vectors of less than 4 bytes have no asynchronous copy: of those rows the next one waits in
+// registers (depth 1).
+template <typename T, int VEC, int NV>
+struct RowRing {
+  static constexpr int kBytes = VEC * (int)sizeof(T);
+  static constexpr bool kAsync = kBytes >= 4;
+  uint8_t* mine;      // [depth][NV][threads of the CTA] vectors
+  uint32_t stride;    // bytes between the vectors of a thread
+  uint32_t slot;      // bytes of a row of all groups
+  RowRaw<T, VEC, kAsync ? 1 : NV> held;
+
+  __device__ __forceinline__ RowRing(uint8_t* base, int cta_threads, int thread)
+      : mine(base + thread * kBytes), stride((uint32_t)(cta_threads * kBytes)), slot((uint32_t)(NV * cta_threads * kBytes)) {}
+  __device__ __forceinline__ void copy(int at, const T* row, int first, int threads, int cols) {
+    if constexpr (kAsync) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (at + i * threads) * VEC;
-    if (c < s.cols) {
-      load_f32<T, VEC>(xr + c, v[i]);
+      for (int i = 0; i < NV; ++i) {
+        const int c = (first + i * threads) * VEC;
+        const uint32_t to = (uint32_t)__cvta_generic_to_shared(mine) + (uint32_t)at * slot + (uint32_t)i * stride;
+        if (c < cols) {
+          if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row + c) : "memory");
+          else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(row + c), "n"(kBytes) : "memory");
+        }
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
+      for (int i = 0; i < NV; ++i) {
+        const int c = (first + i * threads) * VEC;
+        if (c < cols) held.v[i] = *reinterpret_cast<const Vec<T, VEC>*>(row + c);
+      }
     }
   }
+  __device__ __forceinline__ void take(int at, int first, int threads, int cols, RowRaw<T, VEC, NV>* out) const {
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) sum[0] += v[i][j];
-  group_sum<1>(sum, s.warps, at >> 5, 1 + group, scratch[group][0]);
-  const float m = sum[0] / (float)s.cols;
-  float sq[1] = {0.f};
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if ((at + i * threads) * VEC < s.cols)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        v[i][j] -= m;
-        sq[0] += v[i][j] * v[i][j];
+    for (int i = 0; i < NV; ++i) {
+      const int c = (first + i * threads) * VEC;
+      if (c < cols) {
+        if constexpr (kAsync) out->v[i] = *reinterpret_cast<const Vec<T, VEC>*>(mine + (size_t)at * slot + (size_t)i * stride);
+        else out->v[i] = held.v[i];
       }
-  group_sum<1>(sq, s.warps, at >> 5, 1 + group, scratch[group][1]);
-  const float r = 1.f / sqrtf(sq[0] / (float)s.cols + s.eps);
-  if (at == 0) {
-    mean[row] = m;
-    rstd[row] = r;
+    }
   }
+};
+__device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void ring_wait(int newer) {   // all but the `newer` last groups have arrived
+  switch (newer) {
+    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+    default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+  }
+}
+constexpr int kRingDepth = 4;   // at most; ring_wait knows these
+
+// blockDim = (32 * warps, groups).  Dynamic shared memory: `depth` rows of every group.
+template <typename T, int VEC, int NV>
+__global__ void __launch_bounds__(1024) k6_norm_forward(const T* x, const T* w, const T* b, T* y, float* mean, float* rstd, NormShape s) {
+  extern __shared__ uint4 dynamic[];
+  __shared__ alignas(16) float scratch[8][2][kNormMaxWarps];
+  pdl_begin(x, w, b);
+  const int threads = s.warps * 32, at = (int)threadIdx.x, group = (int)threadIdx.y;
+  for (int i = group * threads + at; i < 8 * 2 * kNormMaxWarps; i += threads * (int)blockDim.y) (&scratch[0][0][0])[i] = 0.f;
+  __syncthreads();
+  const long long step = (long long)gridDim.x * blockDim.y;
+  RowRing<T, VEC, NV> ring(reinterpret_cast<uint8_t*>(dynamic), threads * (int)blockDim.y, group * threads + at);
+  long long row = (long long)blockIdx.x * blockDim.y + group;
+  const T* coming = x + row * s.x_ld;   // the row to be copied next, and its number
+  long long coming_row = row;
+  for (int i = 0; i < s.depth; ++i) {
+    if (coming_row < s.rows) ring.copy(i, coming, at, threads, s.cols);
+    ring_commit();
+    coming += step * s.x_ld;
+    coming_row += step;
+  }
+  const float inv = 1.f / (float)s.cols;
   T* yr = y + row * s.cols;
+  int slot = 0;
+  for (long long left = s.rows - (long long)blockIdx.x * blockDim.y; left > 0; left -= step) {   // the whole CTA
+    const bool mine = row < s.rows;
+    RowRaw<T, VEC, NV> raw;
+    ring_wait(s.depth - 1);
+    if (mine) ring.take(slot, at, threads, s.cols, &raw);
+    float v[NV][VEC];
+    float sum[1] = {0.f};
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (at + i * threads) * VEC;
-    if (c < s.cols) {
-      float wv[VEC], bv[VEC];
-      if (w) load_f32<T, VEC>(w + c, wv);
-      if (b) load_f32<T, VEC>(b + c, bv);
+    for (int i = 0; i < NV; ++i)
+      if ((at + i * threads) * VEC < s.cols) {
+        to_f32<T, VEC>(raw.v[i], v[i]);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float o = v[i][j] * r;
-        if (w) o *= wv[j];
-        if (b) o += bv[j];
-        v[i][j] = o;
+        for (int j = 0; j < VEC; ++j) sum[0] += v[i][j];
       }
-      store_f32<T, VEC>(yr + c, v[i]);
+    group_sum<1>(sum, s.warps, at >> 5, scratch[group][0]);
+    if (coming_row < s.rows) ring.copy(slot, coming, at, threads, s.cols);
+    ring_commit();
+    coming += step * s.x_ld;
+    coming_row += step;
+    slot = slot + 1 == s.depth ? 0 : slot + 1;
+    const float m = sum[0] * inv;
+    float sq[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((at + i * threads) * VEC < s.cols) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          v[i][j] -= m;
+          sq[0] = fmaf(v[i][j], v[i][j], sq[0]);
+        }
+      }
+    group_sum<1>(sq, s.warps, at >> 5, scratch[group][1]);
+    const float r = rsqrtf(fmaf(sq[0], inv, s.eps));
+    if (mine) {
+      if (at == 0) {
+        mean[row] = m;
+        rstd[row] = r;
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (at + i * threads) * VEC;
+        if (c < s.cols) {
+          float wv[VEC], bv[VEC];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            wv[j] = 1.f;
+            bv[j] = 0.f;
+          }
+          if (w) load_f32<T, VEC>(w + c, wv);
+          if (b) load_f32<T, VEC>(b + c, bv);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) v[i][j] = fmaf(v[i][j] * r, wv[j], bv[j]);
+          store_f32<T, VEC>(yr + c, v[i]);
+        }
+      }
     }
+    row += step;
+    yr += step * s.cols;
   }
 }
 
@@ -117,14 +204,14 @@ __global__ void __launch_bounds__(1024) k6_norm_forward_long(const T* x, const T
     const T* xr = x + row * s.x_ld;
     float sum[1] = {0.f};
     for (int c = (int)threadIdx.x; c < s.cols; c += 1024) sum[0] += to_f32(xr[c]);
-    group_sum<1>(sum, 32, (int)threadIdx.x >> 5, 1, scratch[0]);
+    group_sum<1>(sum, 32, (int)threadIdx.x >> 5, scratch[0]);
     const float m = sum[0] / (float)s.cols;
     float sq[1] = {0.f};
     for (int c = (int)threadIdx.x; c < s.cols; c += 1024) {
       const float d = to_f32(xr[c]) - m;
       sq[0] += d * d;
     }
-    group_sum<1>(sq, 32, (int)threadIdx.x >> 5, 1, scratch[1]);
+    group_sum<1>(sq, 32, (int)threadIdx.x >> 5, scratch[1]);
     const float r = 1.f / sqrtf(sq[0] / (float)s.cols + s.eps);
     if (threadIdx.x == 0) {
       mean[row] = m;
@@ -139,102 +226,154 @@ __global__ void __launch_bounds__(1024) k6_norm_forward_long(const T* x, const T
   }
 }
 
-// partial: [gridDim.x][2 * cols], sums of dy xh, then of dy.  blockDim = (32 * warps, groups).  THREADS: the most that it
-// is launched with; with 1024 (rows over 8192 elements) the column sums do not fit the registers and lie in shared memory.
+// partial: [gridDim.x][2 * cols], sums of dy xh, then of dy.  blockDim = (32 * warps, groups).  Dynamic shared memory:
+// `depth` rows of x, as many of dy, of every group; afterwards the groups' column sums.  THREADS: the most that it is
+// launched with; with 1024 (rows over 8192 elements) the column sums lie in shared memory all along, and rows are
+// loaded when they are used.
 template <typename T, int VEC, int NV, int THREADS>
 __global__ void __launch_bounds__(THREADS)
 k6_norm_backward(const T* dy, const T* x, const float* mean, const float* rstd, const T* w, const T* add, T* dx, float* partial, NormShape s) {
   constexpr bool kShared = THREADS > 512;
-  extern __shared__ float joined[];   // [groups - 1][2 * cols], or [2 * cols]
-  __shared__ float scratch[8][2][2][kNormMaxWarps];
+  extern __shared__ uint4 dynamic[];   // then [groups - 1][2 * cols], or [2 * cols], of floats
+  __shared__ alignas(16) float scratch[8][2][2 * kNormMaxWarps];
   pdl_begin(dy, x, mean, rstd, w, add);
+  float* joined = reinterpret_cast<float*>(dynamic);
   const int threads = s.warps * 32, at = (int)threadIdx.x, group = (int)threadIdx.y, groups = (int)blockDim.y;
+  for (int i = group * threads + at; i < 8 * 2 * 2 * kNormMaxWarps; i += threads * groups) (&scratch[0][0][0])[i] = 0.f;
+  RowRing<T, VEC, NV> xs(reinterpret_cast<uint8_t*>(dynamic), threads * groups, group * threads + at);
+  RowRing<T, VEC, NV> gs(reinterpret_cast<uint8_t*>(dynamic) + (size_t)s.depth * xs.slot, threads * groups, group * threads + at);
   float dw[kShared ? 1 : NV][VEC], db[kShared ? 1 : NV][VEC];
   if constexpr (kShared) {
     if (partial)
       for (int c = at; c < 2 * s.cols; c += threads) joined[c] = 0.f;
-    __syncthreads();
   } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) dw[i][j] = db[i][j] = 0.f;
   }
+  __syncthreads();
   const float inv = 1.f / (float)s.cols;
-  int turn = 0;
-  for (long long row = (long long)blockIdx.x * groups + group; row < s.rows; row += (long long)gridDim.x * groups) {
-    const T* xr = x + row * s.x_ld;
-    const T* gr = dy + row * s.dy_ld;
-    const float m = mean[row], r = rstd[row];
+  const long long step = (long long)gridDim.x * groups;
+  long long row = (long long)blockIdx.x * groups + group;
+  long long coming = row;   // the row to be copied next
+  if constexpr (!kShared)
+    for (int i = 0; i < s.depth; ++i) {
+      if (coming < s.rows) {
+        xs.copy(i, x + coming * s.x_ld, at, threads, s.cols);
+        gs.copy(i, dy + coming * s.dy_ld, at, threads, s.cols);
+      }
+      ring_commit();
+      coming += step;
+    }
+  float nm = row < s.rows ? mean[row] : 0.f, nr = row < s.rows ? rstd[row] : 0.f;
+  int turn = 0, slot = 0;
+  for (long long left = s.rows - (long long)blockIdx.x * groups; left > 0; left -= step) {   // the whole CTA
+    const bool mine = row < s.rows;
+    const float r = nr, mr = -nm * nr;
     float xh[NV][VEC], t[NV][VEC];
     float sums[2] = {0.f, 0.f};
+    {
+      RowRaw<T, VEC, NV> rx, rg;
+      if constexpr (kShared) {
+        const T* xr = x + row * s.x_ld;
+        const T* gr = dy + row * s.dy_ld;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (at + i * threads) * VEC;
-      if (c < s.cols) {
-        load_f32<T, VEC>(xr + c, xh[i]);
-        load_f32<T, VEC>(gr + c, t[i]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (at + i * threads) * VEC;
-      if (c < s.cols) {
-        float wv[VEC];
-        if (w) load_f32<T, VEC>(w + c, wv);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          xh[i][j] = (xh[i][j] - m) * r;
-          if constexpr (kShared) {
-            if (partial) {   // this thread's own columns
-              joined[c + j] += t[i][j] * xh[i][j];
-              joined[s.cols + c + j] += t[i][j];
-            }
-          } else {
-            dw[i][j] += t[i][j] * xh[i][j];
-            db[i][j] += t[i][j];
+        for (int i = 0; i < NV; ++i) {
+          const int c = (at + i * threads) * VEC;
+          if (c < s.cols && mine) {
+            rx.v[i] = *reinterpret_cast<const Vec<T, VEC>*>(xr + c);
+            rg.v[i] = *reinterpret_cast<const Vec<T, VEC>*>(gr + c);
           }
-          if (w) t[i][j] *= wv[j];
-          sums[0] += t[i][j];
-          sums[1] += t[i][j] * xh[i][j];
+        }
+      } else {
+        ring_wait(s.depth - 1);
+        if (mine) {
+          xs.take(slot, at, threads, s.cols, &rx);
+          gs.take(slot, at, threads, s.cols, &rg);
+        }
+      }
+      if (mine) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int c = (at + i * threads) * VEC;
+          if (c < s.cols) {
+            float wv[VEC];
+            if (w) load_f32<T, VEC>(w + c, wv);
+            to_f32<T, VEC>(rx.v[i], xh[i]);
+            to_f32<T, VEC>(rg.v[i], t[i]);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              const float h = fmaf(xh[i][j], r, mr), g = t[i][j];
+              if constexpr (kShared) {
+                if (partial) {   // this thread's own columns
+                  joined[c + j] += g * h;
+                  joined[s.cols + c + j] += g;
+                }
+              } else {
+                dw[i][j] = fmaf(g, h, dw[i][j]);
+                db[i][j] += g;
+              }
+              xh[i][j] = h;
+              t[i][j] = w ? g * wv[j] : g;
+              sums[0] += t[i][j];
+              sums[1] = fmaf(t[i][j], h, sums[1]);
+            }
+          }
         }
       }
     }
-    group_sum<2>(sums, s.warps, at >> 5, 1 + group, scratch[group][turn][0]);
+    row += step;
+    if (row < s.rows) {
+      nm = mean[row];
+      nr = rstd[row];
+    }
+    group_sum<2>(sums, s.warps, at >> 5, scratch[group][turn]);
     turn ^= 1;
-    const float c1 = sums[0] * inv, c2 = sums[1] * inv;
+    if constexpr (!kShared) {
+      if (coming < s.rows) {
+        xs.copy(slot, x + coming * s.x_ld, at, threads, s.cols);
+        gs.copy(slot, dy + coming * s.dy_ld, at, threads, s.cols);
+      }
+      ring_commit();
+      coming += step;
+      slot = slot + 1 == s.depth ? 0 : slot + 1;
+    }
+    if (mine) {
+      const float c1 = -r * sums[0] * inv, c2 = -r * sums[1] * inv;   // dx = r t + c1 + c2 xh
+      T* out = dx + (row - step) * s.cols;
+      const T* ar = add + (row - step) * s.add_ld;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (at + i * threads) * VEC;
-      if (c < s.cols) {
-        float o[VEC];
-        if (add) load_f32<T, VEC>(add + row * s.add_ld + c, o);
+      for (int i = 0; i < NV; ++i) {
+        const int c = (at + i * threads) * VEC;
+        if (c < s.cols) {
+          float o[VEC];
+          if (add) load_f32<T, VEC>(ar + c, o);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float g = r * (t[i][j] - c1 - xh[i][j] * c2);
-          o[j] = add ? g + o[j] : g;
+          for (int j = 0; j < VEC; ++j) {
+            const float g = fmaf(t[i][j], r, fmaf(xh[i][j], c2, c1));
+            o[j] = add ? g + o[j] : g;
+          }
+          store_f32<T, VEC>(out + c, o);
         }
-        store_f32<T, VEC>(dx + row * s.cols + c, o);
       }
     }
   }
   if (!partial) return;
   float* line = partial + (size_t)blockIdx.x * 2 * s.cols;
+  __syncthreads();
   if constexpr (kShared) {
-    __syncthreads();
     for (int c = at; c < 2 * s.cols; c += threads) line[c] = joined[c];
   } else {
     if (group) {
-      float* mine = joined + (size_t)(group - 1) * 2 * s.cols;
+      float* own = joined + (size_t)(group - 1) * 2 * s.cols;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (at + i * threads) * VEC;
-        if (c < s.cols)
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            mine[c + j] = dw[i][j];
-            mine[s.cols + c + j] = db[i][j];
-          }
+        if (c < s.cols) {
+          store_f32<float, VEC>(own + c, dw[i]);
+          store_f32<float, VEC>(own + s.cols + c, db[i]);
+        }
       }
     }
     __syncthreads();
@@ -242,17 +381,20 @@ k6_norm_backward(const T* dy, const T* x, const float* mean, const float* rstd, 
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (at + i * threads) * VEC;
-        if (c < s.cols)
+        if (c < s.cols) {
+          for (int g = 0; g + 1 < groups; ++g) {
+            float a[VEC], d[VEC];
+            load_f32<float, VEC>(joined + (size_t)g * 2 * s.cols + c, a);
+            load_f32<float, VEC>(joined + (size_t)g * 2 * s.cols + s.cols + c, d);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            float a = dw[i][j], d = db[i][j];
-            for (int g = 1; g < groups; ++g) {
-              a += joined[(size_t)(g - 1) * 2 * s.cols + c + j];
-              d += joined[(size_t)(g - 1) * 2 * s.cols + s.cols + c + j];
+            for (int j = 0; j < VEC; ++j) {
+              dw[i][j] += a[j];
+              db[i][j] += d[j];
             }
-            line[c + j] = a;
-            line[s.cols + c + j] = d;
           }
+          store_f32<float, VEC>(line + c, dw[i]);
+          store_f32<float, VEC>(line + s.cols + c, db[i]);
+        }
       }
     }
   }
@@ -275,7 +417,7 @@ __global__ void __launch_bounds__(1024) k6_norm_backward_long(const T* dy, const
       sums[0] += t;
       sums[1] += t * ((to_f32(xr[c]) - m) * r);
     }
-    group_sum<2>(sums, 32, (int)threadIdx.x >> 5, 1, scratch[turn][0]);
+    group_sum<2>(sums, 32, (int)threadIdx.x >> 5, scratch[turn][0]);
     turn ^= 1;
     const float c1 = sums[0] / (float)s.cols, c2 = sums[1] / (float)s.cols;
     for (int c = (int)threadIdx.x; c < s.cols; c += 1024) {
@@ -302,42 +444,33 @@ __global__ void __launch_bounds__(256) k6_norm_columns_long(const T* dy, const T
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------
-// How a row is spread over a group: `nv` vectors of `vec` elements per thread.  About 8 elements a thread where that
-// needs no more than 8 warps; longer rows take more warps, then more vectors.
+// How a row is spread over a group: `nv` vectors of `vec` elements per thread.  16 elements where there are rows for two
+// groups of every SM and the rows to come can be copied to shared memory, else 8; at most `most` warps; longer rows take another form (nv 0).
 struct NormPlan {
-  int vec, nv, warps, groups;   // nv 0: the form for long rows
+  int vec, nv, warps;
 };
 
 inline bool divides(long long bytes, const void* p, long long ld_bytes) {
   return p == nullptr || ((uintptr_t)p % bytes == 0 && ld_bytes % bytes == 0);
 }
 
-inline NormPlan norm_plan(int cols, int vec) {
-  NormPlan p{vec, 1, 1, 1};
+inline NormPlan norm_plan(long long rows, int cols, int vec, int vec_bytes, int most) {
   const int vectors = (cols + vec - 1) / vec;
-  const int per = 8 / vec > 0 ? 8 / vec : 1;
-  int warps = (vectors + 32 * per - 1) / (32 * per);
-  if (warps > 8) warps = 8;
-  for (;;) {
-    const int need = (vectors + 32 * warps - 1) / (32 * warps);
-    const int cap = 16 / vec;   // vectors per thread: 16 elements at most
-    if (need <= (cap > 1 ? cap : 1)) {
-      p.nv = need;
-      break;
+  for (int each = rows >= 296 && vec_bytes >= 4 ? 16 : 8; each <= 16; each *= 2) {
+    const int warps = (vectors + 32 * (each / vec) - 1) / (32 * (each / vec));
+    if (warps <= most) {
+      int nv = 1;
+      while (nv * 32 * warps < vectors) nv *= 2;
+      return NormPlan{vec, nv, warps};
     }
-    if (warps == 32) {
-      p.nv = 0;
-      break;
-    }
-    warps = warps <= 8 ? 16 : 32;
   }
-  p.warps = warps;
-  int groups = 8 / warps;
-  p.groups = groups < 1 ? 1 : groups;
-  int nv = 1;
-  while (p.nv > nv) nv *= 2;
-  p.nv = p.nv ? nv : 0;
-  return p;
+  return NormPlan{vec, 0, 32};
+}
+
+// Rows under way: as many as the rest of the shared memory holds.
+inline int ring_depth(size_t bytes_a_row, size_t room) {
+  const size_t d = room / bytes_a_row;
+  return d < 1 ? 1 : d > (size_t)kRingDepth ? kRingDepth : (int)d;
 }
 
 template <typename T, typename F>
@@ -369,22 +502,48 @@ int pick_vec(long long cols, std::initializer_list<std::pair<const void*, long l
   return 1;
 }
 
+constexpr int kNormShared = 200 * 1024;   // dynamic shared memory of an SM that the rows under way may take
+
+template <typename... K, typename... A>
+cudaError_t launch_norm(void (*kernel)(K...), long long grid, int warps, int groups, size_t shared, cudaStream_t stream, A... args) {
+  if (shared > 32 * 1024) {
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormShared);
+    if (err != cudaSuccess) return err;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(32 * warps, groups);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(args)...);
+}
+
 template <typename T>
 int norm_forward(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, NormShape s, cudaStream_t stream) {
   const int vec = pick_vec<T>(s.cols, {{x, s.x_ld}, {w, 0}, {b, 0}, {y, s.cols}});
-  NormPlan p = norm_plan(s.cols, vec);
+  const NormPlan p = norm_plan(s.rows, s.cols, vec, vec * (int)sizeof(T), 32);
   s.warps = p.warps;
   cudaError_t e = cudaSuccess;
   if (p.nv == 0) {
     const long long grid = s.rows < 65535 ? s.rows : 65535;
     e = launch_pdl(k6_norm_forward_long<T>, dim3((unsigned)grid), dim3(1024), stream, (const T*)x, (const T*)w, (const T*)b, (T*)y, mean, rstd, s);
   } else {
-    while (p.groups > 1 && s.rows < 148 * p.groups) p.groups /= 2;   // few rows: one row a CTA spreads them over the SMs
-    const long long grid = (s.rows + p.groups - 1) / p.groups;
-    if (grid > 0x7fffffffLL) return GTK_ERR_UNSUPPORTED;
+    // CTAs of 512 threads, two of which fill an SM's registers; few rows: one a CTA, to spread them over the SMs
+    int groups = 16 / p.warps > 8 ? 8 : 16 / p.warps > 1 ? 16 / p.warps : 1;
+    while (groups > 1 && s.rows < 148LL * groups) --groups;
+    const int ctas = 32 / (p.warps * groups);
+    const size_t slot = (size_t)groups * p.warps * 32 * p.nv * p.vec * sizeof(T);
+    s.depth = ring_depth(slot, (size_t)kNormShared / ctas);
+    const long long all = (s.rows + groups - 1) / groups, grid = all < 148LL * ctas ? all : 148LL * ctas;
+    while (s.depth > 1 && ((s.depth - 1) * grid >= all || vec * sizeof(T) < 4)) --s.depth;
     if (!with_plan<T>(p, [&](auto V, auto N) {
-          e = launch_pdl(k6_norm_forward<T, decltype(V)::value, decltype(N)::value>, dim3((unsigned)grid), dim3(32 * p.warps, p.groups), stream,
-                         (const T*)x, (const T*)w, (const T*)b, (T*)y, mean, rstd, s);
+          e = launch_norm(k6_norm_forward<T, decltype(V)::value, decltype(N)::value>, grid, p.warps, groups, slot * s.depth, stream, (const T*)x,
+                          (const T*)w, (const T*)b, (T*)y, mean, rstd, s);
         }))
       return GTK_ERR_UNSUPPORTED;
   }
@@ -398,7 +557,9 @@ template <typename T>
 int norm_backward(const void* dy, const void* x, const float* mean, const float* rstd, const void* w, const void* add, void* dx, void* dw, void* db,
                   float* partial, NormShape s, cudaStream_t stream) {
   const int vec = pick_vec<T>(s.cols, {{x, s.x_ld}, {dy, s.dy_ld}, {w, 0}, {add, s.add_ld}, {dx, s.cols}});
-  NormPlan p = norm_plan(s.cols, vec);
+  NormPlan p = norm_plan(s.rows, s.cols, vec, vec * (int)sizeof(T), 16);   // 512 threads of 128 registers
+  const bool shared = p.nv == 0;
+  if (shared) p = norm_plan(296, s.cols, vec, 4, 32);
   s.warps = p.warps;
   cudaError_t e = cudaSuccess;
   int lines;
@@ -415,34 +576,24 @@ int norm_backward(const void* dy, const void* x, const float* mean, const float*
                    rstd, sums, s);
   } else {
     const size_t line_bytes = 2 * (size_t)s.cols * 4;
-    while (p.groups > 1 && (p.groups - 1) * line_bytes > 32768) p.groups /= 2;
-    const bool shared = p.warps > 16;
-    const size_t dynamic = !sums ? 0 : shared ? line_bytes : (p.groups - 1) * line_bytes;
-    const long long need = (s.rows + p.groups - 1) / p.groups;
+    int groups = shared ? 1 : 16 / p.warps > 8 ? 8 : 16 / p.warps;
+    while (groups > 1 && s.rows < 148LL * groups) --groups;
+    const size_t slot = (size_t)groups * p.warps * 32 * p.nv * p.vec * sizeof(T) * 2;   // of x and dy
+    const long long need = (s.rows + groups - 1) / groups;
     lines = need < kNormLines ? (int)need : kNormLines;
+    s.depth = ring_depth(slot, kNormShared);
+    while (s.depth > 1 && ((long long)(s.depth - 1) * lines >= need || vec * sizeof(T) < 4)) --s.depth;
+    size_t dynamic = shared ? 0 : slot * s.depth;
+    const size_t join = !sums ? 0 : shared ? line_bytes : (groups - 1) * line_bytes;
+    dynamic = dynamic > join ? dynamic : join;
     if (!with_plan<T>(p, [&](auto V, auto N) {
-          cudaLaunchConfig_t cfg = {};
-          cfg.gridDim = dim3((unsigned)lines);
-          cfg.blockDim = dim3(32 * p.warps, p.groups);
-          cfg.dynamicSmemBytes = dynamic;
-          cfg.stream = stream;
-          cudaLaunchAttribute attr[1];
-          attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-          attr[0].val.programmaticStreamSerializationAllowed = 1;
-          cfg.attrs = attr;
-          cfg.numAttrs = 1;
           constexpr int kV = decltype(V)::value, kN = decltype(N)::value;
           auto go = [&](auto kernel) {
-            e = cudaLaunchKernelEx(&cfg, kernel, (const T*)dy, (const T*)x, mean, rstd, (const T*)w, (const T*)add, (T*)dx, sums, s);
+            e = launch_norm(kernel, lines, p.warps, groups, dynamic, stream, (const T*)dy, (const T*)x, mean, rstd, (const T*)w, (const T*)add, (T*)dx, sums, s);
           };
-          if (!shared) {
-            go(k6_norm_backward<T, kV, kN, 512>);
-          } else if constexpr (kV * kN > 8) {
-            e = cudaFuncSetAttribute(k6_norm_backward<T, kV, kN, 1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, 16384 * 8);
-            if (e == cudaSuccess) go(k6_norm_backward<T, kV, kN, 1024>);
-          } else {
-            e = cudaErrorInvalidConfiguration;   // rows for which 17 warps and more are taken give a thread over 8 elements
-          }
+          if (!shared) go(k6_norm_backward<T, kV, kN, 512>);
+          else if constexpr (kV * kN == 16) go(k6_norm_backward<T, kV, kN, 1024>);   // over 8192 elements of 32 warps
+          else e = cudaErrorInvalidConfiguration;
         }))
       return GTK_ERR_UNSUPPORTED;
     if (!sums) {
@@ -465,7 +616,7 @@ using namespace gtk;
 extern "C" int gtk_k6_norm_forward(int type, const void* x, long long x_ld, const void* w, const void* b, void* y, float* mean, float* rstd, long long rows,
                                    long long cols, float eps, void* stream) {
   if (rows <= 0 || cols <= 0 || cols > 0x3fffffff || x_ld < 0) return GTK_ERR_ARG;
-  const NormShape s{rows, x_ld, 0, 0, (int)cols, 1, eps};
+  const NormShape s{rows, x_ld, 0, 0, (int)cols, 1, 1, eps};
   switch (type) {
     case kF32: return norm_forward<float>(x, w, b, y, mean, rstd, s, (cudaStream_t)stream);
     case kF16: return norm_forward<__half>(x, w, b, y, mean, rstd, s, (cudaStream_t)stream);
@@ -482,7 +633,7 @@ extern "C" int gtk_k6_norm_backward(int type, const void* dy, long long dy_ld, c
                                     const void* w, const void* add, long long add_ld, void* dx, void* dw, void* db, float* partial, long long rows,
                                     long long cols, void* stream) {
   if (rows <= 0 || cols <= 0 || cols > 0x3fffffff || x_ld < 0 || dy_ld < 0 || add_ld < 0) return GTK_ERR_ARG;
-  const NormShape s{rows, x_ld, dy_ld, add_ld, (int)cols, 1, 0.f};
+  const NormShape s{rows, x_ld, dy_ld, add_ld, (int)cols, 1, 1, 0.f};
   switch (type) {
     case kF32: return norm_backward<float>(dy, x, mean, rstd, w, add, dx, dw, db, partial, s, (cudaStream_t)stream);
     case kF16: return norm_backward<__half>(dy, x, mean, rstd, w, add, dx, dw, db, partial, s, (cudaStream_t)stream);

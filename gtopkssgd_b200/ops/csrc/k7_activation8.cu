@@ -68,6 +68,14 @@ __device__ __forceinline__ void load_source(const Source& s, long long row, int 
   }
 }
 
+// Codes of f16 values may stand for 65536, up to half a step above what was kept.
+template <int VEC>
+__device__ __forceinline__ void hold_f16(float (&v)[VEC]) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j)
+    if (fabsf(v[j]) > 65504.f) v[j] = copysignf(65504.f, v[j]);
+}
+
 // What is done to it: (v - mean) rstd g + b where mean is given, then the activation.
 template <typename G>
 struct Apply {
@@ -104,11 +112,7 @@ __global__ void __launch_bounds__(256) k7_stage(Source src, Apply<G> f, O* out, 
     float v[VEC];
     if (c < cols) {
       load_source<S, VEC>(src, row, c, v);
-      if constexpr (sizeof(S) == 1 && std::is_same_v<O, __half>) {   // a code may stand for 65536, up to half a step above what it was
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          if (fabsf(v[j]) > 65504.f) v[j] = copysignf(65504.f, v[j]);
-      }
+      if constexpr (sizeof(S) == 1 && std::is_same_v<O, __half>) hold_f16<VEC>(v);
       if (f.mean) {
         const float m = f.mean[row], r = f.rstd[row];
 #pragma unroll
@@ -142,6 +146,86 @@ __global__ void __launch_bounds__(256) k7_stage(Source src, Apply<G> f, O* out, 
     } else {
       store_f32<O, VEC>(at, v);
     }
+  }
+}
+
+// Matrices that are made operands of a matrix product by one launch: up to three, CTAs in the order of the matrices.
+// Rows get a pitch of a multiple of 8 elements, zeros behind the columns.
+enum PackKind : int { kPackPieces = 0, kPackCopy = 1, kPackCodesF16 = 2, kPackCodesBF16 = 3 };
+struct PackItem {
+  Source src;
+  void* out;
+  long long rows;
+  int cols, pitch, kind, vec, per;
+  unsigned strips, first;      // strips of columns; the matrix's first CTA
+};
+struct PackList {
+  PackItem item[3];
+  int count;
+};
+
+template <int KIND, int VEC>
+__device__ __forceinline__ void pack_rows(const PackItem& p, unsigned block) {
+  const int c = (int)((block % p.strips * 32 + threadIdx.x) * VEC);
+  if (c >= p.pitch) return;
+  const long long first = ((long long)(block / p.strips) * kRowWarps + threadIdx.y) * p.per, stride = p.rows * p.pitch;
+  for (int i = 0; i < p.per; ++i) {
+    const long long row = first + i;
+    if (row >= p.rows) return;
+    const long long to = row * p.pitch + c;
+    if constexpr (KIND == kPackCopy) {
+      Vec<uint16_t, VEC> v = {};
+      if (c < p.cols) v = *reinterpret_cast<const Vec<uint16_t, VEC>*>((const uint16_t*)p.src.p + row * p.src.ld + c);
+      *reinterpret_cast<Vec<uint16_t, VEC>*>((uint16_t*)p.out + to) = v;
+    } else {
+      float v[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = 0.f;
+      if constexpr (KIND == kPackPieces) {
+        if (c < p.cols) load_source<float, VEC>(p.src, row, c, v);
+        float left[3][VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          __nv_bfloat16 b[3];
+          split3(v[j], b);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) left[k][j] = __bfloat162float(b[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) store_f32<__nv_bfloat16, VEC>((__nv_bfloat16*)p.out + k * stride + to, left[k]);
+      } else {
+        if (c < p.cols) load_source<signed char, VEC>(p.src, row, c, v);
+        if constexpr (KIND == kPackCodesF16) {
+          hold_f16<VEC>(v);
+          store_f32<__half, VEC>((__half*)p.out + to, v);
+        } else {
+          store_f32<__nv_bfloat16, VEC>((__nv_bfloat16*)p.out + to, v);
+        }
+      }
+    }
+  }
+}
+
+template <int KIND>
+__device__ __forceinline__ void pack_of(const PackItem& p, unsigned block) {
+  constexpr int wide = KIND == kPackPieces ? 4 : 8;
+  if (p.vec == wide) pack_rows<KIND, wide>(p, block);
+  else if (p.vec == 4) pack_rows<KIND, 4>(p, block);
+  else pack_rows<KIND, 1>(p, block);
+}
+
+__global__ void __launch_bounds__(256) k7_pack(const __grid_constant__ PackList list) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int k = 0;
+  while (k + 1 < list.count && blockIdx.x >= list.item[k + 1].first) ++k;
+  const PackItem& p = list.item[k];
+  const unsigned block = blockIdx.x - p.first;
+  switch (p.kind) {
+    case kPackPieces: pack_of<kPackPieces>(p, block); break;
+    case kPackCopy: pack_of<kPackCopy>(p, block); break;
+    case kPackCodesF16: pack_of<kPackCodesF16>(p, block); break;
+    default: pack_of<kPackCodesBF16>(p, block); break;
   }
 }
 
@@ -328,6 +412,44 @@ extern "C" int gtk_k7_stage(int type, const void* src, long long src_ld, const u
     case kBF16: return of(__nv_bfloat16{});
   }
   return GTK_ERR_ARG;
+}
+
+// Up to three matrices to operands by one launch.  list: for each of them eight words - kind (0: f32 to three bf16 pieces,
+// 1: 16 bits as they are, 2 and 3: codes to f16 and bf16), address, leading dimension, exponents and their leading
+// dimension (codes), rows, columns, address of the operand (pitch: the columns rounded up to 8; pieces follow one
+// another), on 16 bytes.
+extern "C" int gtk_k7_pack(gtk_addresses list, void* stream) {
+  if (list.n == 0 || list.n % 8 || list.n > 24) return GTK_ERR_ARG;
+  PackList l{};
+  unsigned long long blocks = 0;
+  for (unsigned i = 0; i < list.n / 8; ++i) {
+    const unsigned long long* w = list.p + 8 * i;
+    PackItem& p = l.item[i];
+    p.kind = (int)w[0];
+    p.src = Source{(const void*)w[1], (long long)w[2], (const unsigned char*)w[3], (long long)w[4]};
+    p.rows = (long long)w[5];
+    p.out = (void*)w[7];
+    const long long cols = (long long)w[6];
+    if (w[0] > 3 || !p.src.p || !p.out || p.rows <= 0 || cols <= 0 || cols > 0x3ffffff0 || p.src.ld < 0 || (uintptr_t)p.out % 16 ||
+        (w[0] >= 2 && !p.src.e))
+      return GTK_ERR_ARG;
+    p.cols = (int)cols;
+    p.pitch = (p.cols + 7) / 8 * 8;
+    const int elem = p.kind == kPackPieces ? 4 : p.kind == kPackCopy ? 2 : 1, wide = p.kind == kPackPieces ? 4 : 8;
+    p.vec = 1;
+    for (int vec : {wide, 4})
+      if (p.vec == 1 && p.cols % vec == 0 && aligned(p.src.p, p.src.ld, elem, vec)) p.vec = vec;
+    p.strips = (unsigned)((p.pitch + 32 * p.vec - 1) / (32 * p.vec));
+    unsigned y;
+    if (!row_grid(p.rows, p.strips, &p.per, &y)) return GTK_ERR_UNSUPPORTED;
+    p.first = (unsigned)blocks;
+    blocks += (unsigned long long)p.strips * y;
+  }
+  if (blocks > 0x7fffffffull) return GTK_ERR_UNSUPPORTED;
+  l.count = (int)(list.n / 8);
+  const cudaError_t err = launch_pdl(k7_pack, dim3((unsigned)blocks), dim3(32, kRowWarps), (cudaStream_t)stream, l);
+  gtk_count_launch(1);
+  return err == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;
 }
 
 // Lines of `cols` floats that `partial` has to hold.

@@ -787,10 +787,14 @@ inline GemmPlan plan_gemm(long long m, long long n, int blocks_k, int products, 
 inline bool on16(const void* p, long long ld, int elem) { return !p || ((uintptr_t)p % 16 == 0 && ld * elem % 16 == 0); }
 
 template <typename T>
-cudaError_t launch_gemm(bool slope, int grid, size_t shared, cudaStream_t stream, const CUtensorMap& a, const CUtensorMap& b, const GemmShape& s,
+cudaError_t launch_gemm(int device, bool slope, int grid, size_t shared, cudaStream_t stream, const CUtensorMap& a, const CUtensorMap& b, const GemmShape& s,
                         const GemmEpilogue& e) {
+  static std::atomic<unsigned long long> devices[2];   // whose kernel has been given its shared memory
+  const unsigned long long bit = 1ull << device;
+  const bool allowed = devices[slope].load(std::memory_order_relaxed) & bit;
   auto go = [&](auto kernel) {
-    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared - kStaticShared);
+    cudaError_t err = cudaSuccess;
+    if (!allowed) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared - kStaticShared);
     if (err != cudaSuccess) return err;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
@@ -805,6 +809,7 @@ cudaError_t launch_gemm(bool slope, int grid, size_t shared, cudaStream_t stream
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
+    if (!allowed) devices[slope].fetch_or(bit, std::memory_order_relaxed);
     return cudaLaunchKernelEx(&cfg, kernel, a, b, s, e);
   };
   return slope ? go(k8_gemm<T, true>) : go(k8_gemm<T, false>);
@@ -870,9 +875,9 @@ extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long lo
   const cudaStream_t stream = (cudaStream_t)stream_;
   cudaError_t err;
   switch (type) {
-    case kF32: err = launch_gemm<float>(slope, grid, shared, stream, am, bm, s, ep); break;
-    case kF16: err = launch_gemm<__half>(slope, grid, shared, stream, am, bm, s, ep); break;
-    case kBF16: err = launch_gemm<__nv_bfloat16>(slope, grid, shared, stream, am, bm, s, ep); break;
+    case kF32: err = launch_gemm<float>(info->device, slope, grid, shared, stream, am, bm, s, ep); break;
+    case kF16: err = launch_gemm<__half>(info->device, slope, grid, shared, stream, am, bm, s, ep); break;
+    case kBF16: err = launch_gemm<__nv_bfloat16>(info->device, slope, grid, shared, stream, am, bm, s, ep); break;
     default: return GTK_ERR_ARG;
   }
   gtk_count_launch(1);

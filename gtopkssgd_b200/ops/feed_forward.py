@@ -16,9 +16,9 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 
 from . import layers_oracle as oracle
-from .activation8 import Activation8, act_of, bits_of, colsum, matrix, same, shaped, stream_of, type_of, vector
+from .activation8 import Activation8, act_of, bits_of, colsum, matrix, parameter, same, shaped, stream_of, type_of
 from .layer_norm import layer_norm_backward, layer_norm_forward
-from .linear import _check, _gradients, linear_forward, operand, product
+from .linear import _check, _gradients, linear_forward, normed_operand, operands, product
 
 
 class FeedForwardKept(NamedTuple):
@@ -57,11 +57,11 @@ def feed_forward_backward(dy: torch.Tensor, kept: FeedForwardKept, norm_weight: 
     hidden, dim = w1.shape
     shape = tuple(dy.shape)
     shaped("w2", w2, dim, hidden)
-    shaped("norm_weight", norm_weight, dim)
-    shaped("norm_bias", norm_bias, dim)
+    norm_weight = parameter(dy, "norm_weight", norm_weight, dim)
+    norm_bias = parameter(dy, "norm_bias", norm_bias, dim)
     if tuple(x.shape) != shape or shape[-1] != dim:
         raise ValueError("the gradient has shape %s, x %s, w1 %s" % (shape, tuple(x.shape), tuple(w1.shape)))
-    same(dy, x=x, z=z, w1=w1, w2=w2, norm_weight=norm_weight, norm_bias=norm_bias)
+    same(dy, x=x, z=z, w1=w1, w2=w2)
     g = matrix(dy)
     rows = g.size(0)
     z = z if isinstance(z, Activation8) else matrix(z)
@@ -71,23 +71,22 @@ def feed_forward_backward(dy: torch.Tensor, kept: FeedForwardKept, norm_weight: 
         raise ValueError("mean and rstd are the forward pass's, one value for each of %d rows" % rows)
     if not g.is_cuda:
         return _backward_plain(g, FeedForwardKept(x, mean.reshape(-1), rstd.reshape(-1), z), norm_weight, norm_bias, w1, w2, activation, shape)
-    new = dict(dtype=dy.dtype, device=dy.device)
+    new = dy.new_empty
     if rows == 0:
-        return (torch.empty(shape, **new), *(torch.zeros(n, **new) for n in (dim, dim, (hidden, dim), hidden, (dim, hidden), dim)))
+        return (new(shape), *(new(n).zero_() for n in (dim, dim, (hidden, dim), hidden, (dim, hidden), dim)))
     stream = stream_of(g)
-    mean, rstd = vector(mean), vector(rstd)
+    mean, rstd = mean.contiguous(), rstd.contiguous()
     # dz = (dy W2) act'(z) and h = act(z) again, both in the product's epilogue
-    dz, h = torch.empty((rows, hidden), **new), torch.empty((rows, hidden), **new)
-    db1 = torch.empty(hidden, **new)
-    go = operand(g)
-    product(rows, hidden, dim, go, False, operand(matrix(w2)), True, dz, stream, activation=code, slope=True, z=z, h=h, db=db1)
-    dw2 = torch.empty((dim, hidden), **new)
-    product(dim, hidden, rows, go, True, operand(h), True, dw2, stream)
-    del h
+    dz, h, db1 = new((rows, hidden)), new((rows, hidden)), new(hidden)
+    go, w2o = operands(g, matrix(w2))
+    product(rows, hidden, dim, go, False, w2o, True, dz, stream, activation=code, slope=True, z=z, h=h, db=db1)
+    del w2o
+    dw2 = new((dim, hidden))
+    product(dim, hidden, rows, go, True, operands(h)[0], True, dw2, stream)
+    del h, go
     _, db2 = colsum(g)
-    xm = x if isinstance(x, Activation8) else matrix(x)
-    a = operand(xm, mean, rstd, vector(norm_weight), vector(norm_bias))   # the norm's output again
-    da, dw1 = _gradients(dz, a, dim, w1, True, True)
+    a = normed_operand(x if isinstance(x, Activation8) else matrix(x), mean, rstd, norm_weight, norm_bias)   # the norm's output again
+    da, dw1 = _gradients(dz, a, w1, True, True)
     dx, dg, db = layer_norm_backward(da.view(shape), x.restore() if isinstance(x, Activation8) else x, mean, rstd, norm_weight, add=dy)
     return dx, dg, db, dw1, db1, dw2, db2
 

@@ -13,8 +13,8 @@ import torch
 
 from . import layers_oracle as oracle
 from . import lib as _lib
-from .activation8 import TYPES, ld, lines, matrix, same, shaped, stream_of, type_of, vector
-from .select import _ptr
+from .activation8 import ld, lines, matrix, parameter, same, shaped, stream_of, type_of
+from .select import _FLOAT, _ptr
 
 
 def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -26,17 +26,16 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
     rows, cols = m.shape
     if x.size(-1) == 0:
         raise ValueError("layer_norm: the last axis is empty")
-    same(x, weight=weight, bias=bias)
-    shaped("weight", weight, cols)
-    shaped("bias", bias, cols)
+    weight = parameter(x, "weight", weight, cols)
+    bias = parameter(x, "bias", bias, cols)
     lead = x.shape[:-1]
     if not m.is_cuda:
         y, mean, rstd = oracle.norm_forward(m, weight, bias, eps)
         return y.view(x.shape), mean.view(lead), rstd.view(lead)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean, rstd = torch.empty((2, *lead), dtype=torch.float32, device=x.device).unbind(0)
+    y = x.new_empty(x.shape)
+    mean = x.new_empty(lead, dtype=_FLOAT)
+    rstd = torch.empty_like(mean)
     if rows:
-        weight, bias = vector(weight), vector(bias)
         err = _lib.calls().gtk_k6_norm_forward(code, m.data_ptr(), ld(m), _ptr(weight), _ptr(bias), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
                                                rows, cols, eps, stream_of(m))
         if err:
@@ -49,35 +48,39 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
                         want_parameters: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx, dweight, dbias) from the forward pass's x, mean and rstd.  ``add``, of x's shape, is added to dx: the
     gradient that reaches x past the norm."""
-    type_of(x, "layer_norm")
+    code = type_of(x, "layer_norm")
     m, g = matrix(x), matrix(dy)
     rows, cols = m.shape
     if dy.shape != x.shape:
         raise ValueError("the gradient has shape %s, x %s" % (tuple(dy.shape), tuple(x.shape)))
-    same(x, dy=dy, weight=weight, add=add)
-    shaped("weight", weight, cols)
-    shaped("add", add, *x.shape)
+    if x.size(-1) == 0:
+        raise ValueError("layer_norm: the last axis is empty")
+    weight = parameter(x, "weight", weight, cols)
+    same(x, dy=dy, add=add)
+    if add is not None:
+        shaped("add", add, *x.shape)
+        add = matrix(add)
     if mean.numel() != rows or rstd.numel() != rows or mean.device != x.device or rstd.device != x.device:
         raise ValueError("mean and rstd are the forward pass's, one value for each of %d rows" % rows)
     if not m.is_cuda:
-        dx, dw, db = oracle.norm_backward(g, m, mean.reshape(-1), rstd.reshape(-1), weight, None if add is None else matrix(add))
+        dx, dw, db = oracle.norm_backward(g, m, mean.reshape(-1), rstd.reshape(-1), weight, add)
         return (dx.view(x.shape), dw, db) if want_parameters else (dx.view(x.shape), None, None)
-    if mean.dtype != torch.float32 or rstd.dtype != torch.float32:
+    if mean.dtype is not _FLOAT or rstd.dtype is not _FLOAT:
         raise TypeError("mean and rstd are float32")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = x.new_empty(x.shape)
     dw = db = partial = None
     if want_parameters:
-        dw, db = torch.empty((2, cols), dtype=x.dtype, device=x.device).unbind(0)
-        partial = torch.empty((min(lines("gtk_k6_norm_lines"), max(rows, 1)), 2 * cols), dtype=torch.float32, device=x.device)
+        dw = x.new_empty(cols)
+        db = torch.empty_like(dw)
+        partial = x.new_empty((min(lines("gtk_k6_norm_lines"), rows), 2 * cols), dtype=_FLOAT)
     if rows == 0:
         if want_parameters:
             dw.zero_()
             db.zero_()
         return dx, dw, db
-    weight, mean, rstd = vector(weight), vector(mean), vector(rstd)
-    a = None if add is None else matrix(add)
-    err = _lib.calls().gtk_k6_norm_backward(TYPES[x.dtype], g.data_ptr(), ld(g), m.data_ptr(), ld(m), mean.data_ptr(), rstd.data_ptr(), _ptr(weight),
-                                            _ptr(a), 0 if a is None else ld(a), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(partial), rows, cols,
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    err = _lib.calls().gtk_k6_norm_backward(code, g.data_ptr(), ld(g), m.data_ptr(), ld(m), mean.data_ptr(), rstd.data_ptr(), _ptr(weight), _ptr(add),
+                                            0 if add is None else ld(add), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(partial), rows, cols,
                                             stream_of(m))
     if err:
         _lib.check(err, "gtk_k6_norm_backward")

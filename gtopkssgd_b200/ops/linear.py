@@ -15,8 +15,8 @@ import torch
 
 from . import layers_oracle as oracle
 from . import lib as _lib
-from .activation8 import TYPES, Activation8, act_of, bits_of, colsum, ld, matrix, same, shaped, stream_of, type_of, vector
-from .select import _ptr
+from .activation8 import TYPES, Activation8, act_of, bits_of, colsum, ld, matrix, parameter, same, shaped, stream_of, type_of
+from .select import _FLOAT, _ptr
 
 Kept = Union[None, torch.Tensor, Activation8]
 
@@ -35,22 +35,51 @@ class Operand:
         self.at, self.ld, self.pieces, self.stride, self.held = at, row, pieces, stride, held
 
 
-def operand(src, mean=None, rstd=None, weight=None, bias=None, activation: str = "none") -> Operand:
-    """The operand of a matrix or of codes, after (v - mean) * rstd * weight + bias where mean is given and the
-    activation.  A 16-bit matrix whose rows lie on 16-byte boundaries is read where it is."""
-    codes = isinstance(src, Activation8)
+def operands(*sources) -> list:
+    """Matrices or codes (``Activation8``), up to three, as operands.  A 16-bit matrix whose rows lie on 16-byte
+    boundaries is read where it is; one launch makes all the others."""
+    made, words, size = [], [], 0
+    for src in sources:
+        codes = type(src) is Activation8
+        m = src.q if codes else src
+        rows, cols = m.shape
+        row = ld(m)
+        f32 = src.dtype is _FLOAT
+        if not codes and not f32 and row % 8 == 0 and row >= cols and m.data_ptr() % 16 == 0:
+            made.append(Operand(m.data_ptr(), row, 1, 0, m))
+            continue
+        pitch = (cols + 7) & ~7
+        pieces = 3 if f32 and not codes else 1
+        kind = (2 if src.dtype is torch.float16 else 3) if codes else 0 if f32 else 1
+        words += (kind, m.data_ptr(), row, src.e.data_ptr() if codes else 0, ld(src.e) if codes else 0, rows, cols, size)
+        made.append(Operand(size, pitch, pieces, rows * pitch, None))
+        size += pieces * rows * pitch * 2
+    if words:
+        src = sources[0]
+        room = (src.q if type(src) is Activation8 else src).new_empty(size, dtype=torch.uint8)
+        base = room.data_ptr()
+        for i in range(7, len(words), 8):
+            words[i] += base
+        for o in made:
+            if o.held is None:
+                o.at, o.held = o.at + base, room
+        err = _lib.calls().gtk_k7_pack(words, stream_of(room))
+        if err:
+            _lib.check(err, "gtk_k7_pack")
+    return made
+
+
+def normed_operand(src, mean, rstd, weight, bias) -> Operand:
+    """The operand (v - mean) * rstd * weight + bias of a matrix or of codes."""
+    codes = type(src) is Activation8
     m = src.q if codes else src
     rows, cols = m.shape
-    f32 = src.dtype == torch.float32
-    plain = mean is None and activation == "none"
-    if not codes and not f32 and plain and ld(m) % 8 == 0 and m.data_ptr() % 16 == 0 and ld(m) >= cols:
-        return Operand(m.data_ptr(), ld(m), 1, 0, m)
-    pieces = 1 if not f32 or (codes and plain) else 3
-    pitch = -(-cols // 8) * 8
-    out = torch.empty((pieces, rows, pitch), dtype=torch.bfloat16 if f32 else src.dtype, device=m.device)
-    err = _lib.calls().gtk_k7_stage(TYPES[src.dtype], m.data_ptr(), ld(m), src.e.data_ptr() if codes else None, ld(src.e) if codes else 0, _ptr(mean),
-                                    _ptr(rstd), _ptr(weight), _ptr(bias), act_of(activation), (1 if codes and plain else 3) if f32 else 0,
-                                    out.data_ptr(), pitch, rows * pitch, rows, cols, pitch, stream_of(m))
+    f32 = src.dtype is _FLOAT
+    pieces, pitch = 3 if f32 else 1, (cols + 7) & ~7
+    out = m.new_empty((pieces, rows, pitch), dtype=torch.bfloat16 if f32 else src.dtype)
+    err = _lib.calls().gtk_k7_stage(TYPES[src.dtype], m.data_ptr(), ld(m), src.e.data_ptr() if codes else None, ld(src.e) if codes else 0,
+                                    mean.data_ptr(), rstd.data_ptr(), _ptr(weight), _ptr(bias), 0, 3 if f32 else 0, out.data_ptr(), pitch,
+                                    rows * pitch, rows, cols, pitch, stream_of(m))
     if err:
         _lib.check(err, "gtk_k7_stage")
     return Operand(out.data_ptr(), pitch, pieces, rows * pitch, out)
@@ -58,15 +87,23 @@ def operand(src, mean=None, rstd=None, weight=None, bias=None, activation: str =
 
 def product(m: int, n: int, k: int, a: Operand, a_mn: bool, b: Operand, b_mn: bool, out: torch.Tensor, stream: int, bias=None, add=None,
             activation: int = 0, slope: bool = False, z: Kept = None, h: Optional[torch.Tensor] = None, db: Optional[torch.Tensor] = None) -> None:
-    """out[m, n] = epilogue(sum_k a[m, k] b[n, k]); ``a_mn``, ``b_mn``: the operand's matrix is [k, m] or [k, n]."""
-    sums = torch.empty((-(-m // 32), n), dtype=torch.float32, device=out.device) if db is not None else None
-    if isinstance(z, Activation8):
-        zp, zld, q, qld, e, eld = None, 0, z.q.data_ptr(), ld(z.q) if slope else z.e.size(1) * 32, z.e.data_ptr(), ld(z.e)
+    """out[m, n] = epilogue(sum_k a[m, k] b[n, k]); ``a_mn``, ``b_mn``: the operand's matrix is [k, m] or [k, n].  out and
+    h are dense."""
+    sums = None
+    zp = zld = q = qld = e = eld = None
+    if z is None:
+        zld = qld = eld = 0
+    elif type(z) is Activation8:
+        zld = 0
+        q, qld, e, eld = z.q.data_ptr(), ld(z.q) if slope else z.e.size(1) * 32, z.e.data_ptr(), ld(z.e)
     else:
-        zp, zld, q, qld, e, eld = _ptr(z), 0 if z is None else ld(z), None, 0, None, 0
-    err = _lib.calls().gtk_k8_gemm(TYPES[out.dtype], out.dtype == torch.float16, m, n, k, a.at, a.ld, a.pieces, a.stride, a_mn, b.at, b.ld, b.pieces,
-                                   b.stride, b_mn, out.data_ptr(), ld(out), _ptr(bias), _ptr(add), 0 if add is None else ld(add), activation, slope, zp,
-                                   zld, q, qld, e, eld, _ptr(h), 0 if h is None else ld(h), _ptr(sums), _ptr(db), stream)
+        qld = eld = 0
+        zp, zld = z.data_ptr(), ld(z)
+    if db is not None:
+        sums = out.new_empty((-(-m // 32), n), dtype=_FLOAT)
+    err = _lib.calls().gtk_k8_gemm(TYPES[out.dtype], out.dtype is torch.float16, m, n, k, a.at, a.ld, a.pieces, a.stride, a_mn, b.at, b.ld, b.pieces,
+                                   b.stride, b_mn, out.data_ptr(), n, _ptr(bias), _ptr(add), 0 if add is None else ld(add), activation, slope, zp,
+                                   zld, q, qld, e, eld, _ptr(h), n, _ptr(sums), _ptr(db), stream)
     if err:
         _lib.check(err, "gtk_k8_gemm")
 
@@ -84,44 +121,49 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
     x's type or, with ``bits=8``, as ``Activation8``; None where there is no activation."""
     type_of(x, "linear")
     code = act_of(activation)
-    bits_of(bits)
+    if bits:
+        bits_of(bits)
     _check(x, weight, "linear")
-    same(x, weight=weight, bias=bias, residual=residual)
+    same(x, weight=weight, residual=residual)
     outer, inner = weight.shape
     shape = (*x.shape[:-1], outer)
-    shaped("bias", bias, outer)
-    shaped("residual", residual, *shape)
+    bias = parameter(x, "bias", bias, outer)
+    if residual is not None:
+        shaped("residual", residual, *shape)
+        residual = matrix(residual)
     keep = keep and code != 0
     m = matrix(x)
     rows = m.size(0)
     if not m.is_cuda:
-        y, z = oracle.linear_forward(m, weight, bias, activation, None if residual is None else matrix(residual))
+        y, z = oracle.linear_forward(m, weight, bias, activation, residual)
         z = None if not keep else Activation8(*oracle.keep8(z), x.dtype) if bits else z.to(x.dtype)
         return y.view(shape), z
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(shape)
     z = None
     if keep:
-        z = Activation8.empty(rows, outer, x.dtype, x.device) if bits else torch.empty((rows, outer), dtype=x.dtype, device=x.device)
+        z = Activation8.empty(x, rows, outer, (rows, outer)) if bits else x.new_empty((rows, outer))
     if rows and outer:
-        product(rows, outer, inner, operand(m), False, operand(matrix(weight)), False, y.view(rows, outer), stream_of(m), vector(bias),
-                None if residual is None else matrix(residual), code, z=z)
+        a, b = operands(m, matrix(weight))
+        product(rows, outer, inner, a, False, b, False, y, stream_of(m), bias, residual, code, z=z)
     return y, z
 
 
-def _gradients(dz: torch.Tensor, x: Union[torch.Tensor, Activation8, Operand], inner: int, weight: torch.Tensor, need_dx: bool, need_dw: bool):
-    """(dz W, dz^T x) over CUDA matrices; x may come as an operand."""
+def _gradients(dz: torch.Tensor, x, weight: torch.Tensor, need_dx: bool, need_dw: bool):
+    """(dz W, dz^T x) over CUDA matrices; x may be codes, or an operand already."""
     rows, outer = dz.shape
-    stream = stream_of(dz)
+    inner = weight.size(1)
     dx = dw = None
     if not (need_dx or need_dw):
         return dx, dw
-    a = operand(dz)
+    stream = stream_of(dz)
+    made = type(x) is Operand
+    a, *rest = operands(dz, *((matrix(weight),) if need_dx else ()), *((x,) if need_dw and not made else ()))
     if need_dx:
-        dx = torch.empty((rows, inner), dtype=dz.dtype, device=dz.device)
-        product(rows, inner, outer, a, False, operand(matrix(weight)), True, dx, stream)
+        dx = dz.new_empty((rows, inner))
+        product(rows, inner, outer, a, False, rest[0], True, dx, stream)
     if need_dw:
-        dw = torch.empty((outer, inner), dtype=dz.dtype, device=dz.device)
-        product(outer, inner, rows, a, True, x if isinstance(x, Operand) else operand(x), True, dw, stream)
+        dw = dz.new_empty((outer, inner))
+        product(outer, inner, rows, a, True, x if made else rest[-1], True, dw, stream)
     return dx, dw
 
 
@@ -158,10 +200,10 @@ def linear_backward(dy: torch.Tensor, x: Union[torch.Tensor, Activation8], weigh
     products = need[0] or need[1]
     db = None
     if (code and products) or need[2]:
-        dz, db = colsum(g, activation, z, want_dz=bool(code and products), want_sum=need[2])
+        dz, db = colsum(g, code, z, want_dz=bool(code and products), want_sum=need[2])
         g = dz if code and products else g
-    dx, dw = _gradients(g, x if isinstance(x, Activation8) or not need[1] else matrix(x), inner, weight, need[0], need[1])
-    return dx if dx is None else dx.view(shape), dw, db
+    dx, dw = _gradients(g, x if isinstance(x, Activation8) or not need[1] else matrix(x), weight, need[0], need[1])
+    return dx if dx is None or len(shape) == 2 else dx.view(shape), dw, db
 
 
 class _Linear(torch.autograd.Function):
