@@ -192,9 +192,31 @@ __device__ __forceinline__ float block8_scale(uint32_t byte) {
 }
 // 2^-(byte - 127), for the bytes 0 .. 249 (255: something)
 __device__ __forceinline__ float block8_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+// The largest magnitude of three, NaN where one is.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Four codes in a word, for bytes below kBlock8Last: adding 1.5 * 2^23 rounds to an integer, whose low byte it leaves in
+// the low byte of the sum.
+__device__ __forceinline__ uint32_t block8_codes(float a, float b, float c, float d, float inverse) {
+  constexpr float kMagic = 12582912.f;
+  const uint32_t ia = __float_as_uint(fmaf(a, inverse, kMagic)), ib = __float_as_uint(fmaf(b, inverse, kMagic));
+  const uint32_t ic = __float_as_uint(fmaf(c, inverse, kMagic)), id = __float_as_uint(fmaf(d, inverse, kMagic));
+  return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
+}
 __device__ __forceinline__ int block8_code(float x, uint32_t byte) {
   const int q = __float2int_rn(x * block8_inverse(byte));
   return byte < kBlock8Last ? q : byte == kBlock8NaN ? 0 : max(-63, min(63, q));
+}
+
+// ---- f32 as two f16 pieces -----------------------------------------------------------------------------------------
+// The power of two by which values whose largest magnitude has these bits are scaled: it then lies in [2^14, 2^15).
+// Values down to 2^-17 of the largest keep 22 bits, smaller ones are off by 2^-40 of it at most.
+__device__ __forceinline__ int pair_shift(uint32_t most) {
+  const int shift = 14 + 127 - (int)(most >> 23);
+  return most == 0u || most >= 0x7f800000u ? 0 : shift > 126 ? 126 : shift;
 }
 
 }  // namespace gtk

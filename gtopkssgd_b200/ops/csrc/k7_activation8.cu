@@ -149,18 +149,20 @@ __global__ void __launch_bounds__(256) k7_stage(Source src, Apply<G> f, O* out, 
   }
 }
 
-// Matrices that are made operands of a matrix product by one launch: up to three, CTAs in the order of the matrices.
+// Matrices that are made operands of a matrix product by one launch: up to four, CTAs in the order of the matrices.
 // Rows get a pitch of a multiple of 8 elements, zeros behind the columns.
-enum PackKind : int { kPackPieces = 0, kPackCopy = 1, kPackCodesF16 = 2, kPackCodesBF16 = 3 };
+enum PackKind : int { kPackPieces = 0, kPackCopy = 1, kPackCodesF16 = 2, kPackCodesBF16 = 3, kPackPairsOfRows = 4, kPackPairsOfColumns = 5 };
 struct PackItem {
   Source src;
   void* out;
   long long rows;
   int cols, pitch, kind, vec, per;
   unsigned strips, first;      // strips of columns; the matrix's first CTA
+  unsigned int* most;          // pairs: the largest magnitudes (bits) of the rows (written) or of the columns (read)
 };
+constexpr int kPackItems = 4;
 struct PackList {
-  PackItem item[3];
+  PackItem item[kPackItems];
   int count;
 };
 
@@ -206,6 +208,116 @@ __device__ __forceinline__ void pack_rows(const PackItem& p, unsigned block) {
   }
 }
 
+// Two f16 pieces of scaled f32 values.
+template <int VEC>
+__device__ __forceinline__ void store_pairs(__half* out, long long stride, const float (&v)[VEC], const float (&scale)[VEC]) {
+  float high[VEC], low[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    const float x = v[j] * scale[j];
+    high[j] = __half2float(__float2half_rn(x));
+    low[j] = isinf(high[j]) || isnan(high[j]) ? 0.f : x - high[j];
+  }
+  store_f32<__half, VEC>(out, high);
+  store_f32<__half, VEC>(out + stride, low);
+}
+
+// Rows scaled by their own largest magnitude: a warp takes a row of up to 1024 columns (strips 1: eight rows a CTA),
+// the CTA's eight warps one of more.
+template <int VEC>
+__device__ __forceinline__ void pack_pairs_of_rows(const PackItem& p, unsigned block, unsigned int* room) {
+  const bool shared = p.strips != 1;
+  const long long row = shared ? block : (long long)block * kRowWarps + threadIdx.y, stride = p.rows * p.pitch;
+  const int first = (int)((shared ? threadIdx.y * 32 + threadIdx.x : threadIdx.x) * VEC), step = (shared ? 256 : 32) * VEC;
+  if (row >= p.rows) return;   // the whole warp, or the whole CTA
+  const float* x = (const float*)p.src.p + row * p.src.ld;
+  unsigned int most = 0;
+  for (int c = first; c < p.cols; c += step) {
+    float v[VEC];
+    load_f32<float, VEC>(x + c, v);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (shared) {
+    if (threadIdx.x == 0) room[threadIdx.y] = most;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kRowWarps; ++k) most = max(most, room[k]);
+  }
+  if (first == 0) p.most[row] = most;
+  float scale[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) scale[j] = __uint_as_float((uint32_t)(pair_shift(most) + 127) << 23);
+  for (int c = first; c < p.pitch; c += step) {
+    float v[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = 0.f;
+    if (c < p.cols) load_f32<float, VEC>(x + c, v);
+    store_pairs<VEC>((__half*)p.out + row * p.pitch + c, stride, v, scale);
+  }
+}
+
+template <int VEC>
+__device__ __forceinline__ void pack_pairs_of_columns(const PackItem& p, unsigned block) {
+  const int c = (int)((block % p.strips * 32 + threadIdx.x) * VEC);
+  if (c >= p.pitch) return;
+  const long long first = ((long long)(block / p.strips) * kRowWarps + threadIdx.y) * p.per, stride = p.rows * p.pitch;
+  float scale[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) scale[j] = c + j < p.cols ? __uint_as_float((uint32_t)(pair_shift(p.most[c + j]) + 127) << 23) : 0.f;
+  for (int i = 0; i < p.per; ++i) {
+    const long long row = first + i;
+    if (row >= p.rows) return;
+    float v[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = 0.f;
+    if (c < p.cols) load_f32<float, VEC>((const float*)p.src.p + row * p.src.ld + c, v);
+    store_pairs<VEC>((__half*)p.out + row * p.pitch + c, stride, v, scale);
+  }
+}
+
+// The largest magnitudes of the columns of the list's kPackPairsOfColumns matrices, by atomic maxima over zeros: whatever
+// their order, the result is the same.
+template <int VEC>
+__device__ __forceinline__ void column_most(const PackItem& p, unsigned block, unsigned int (*room)[32 * 4]) {
+  const int c = (int)((block % p.strips * 32 + threadIdx.x) * VEC);
+  const long long first = ((long long)(block / p.strips) * kRowWarps + threadIdx.y) * p.per;
+  unsigned int most[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) most[j] = 0;
+  if (c < p.cols)
+    for (int i = 0; i < p.per; ++i) {
+      const long long row = first + i;
+      if (row >= p.rows) break;
+      float v[VEC];
+      load_f32<float, VEC>((const float*)p.src.p + row * p.src.ld + c, v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) most[j] = max(most[j], __float_as_uint(v[j]) & 0x7fffffffu);
+    }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) room[threadIdx.y][threadIdx.x * VEC + j] = most[j];
+  __syncthreads();
+  for (int i = (int)(threadIdx.y * 32 + threadIdx.x); i < 32 * VEC; i += 256) {
+    const int col = (int)(block % p.strips * 32 * VEC) + i;
+    if (col >= p.cols) break;
+    unsigned int m = 0;
+#pragma unroll
+    for (int k = 0; k < kRowWarps; ++k) m = max(m, room[k][i]);
+    if (m) atomicMax(p.most + col, m);
+  }
+}
+__global__ void __launch_bounds__(256) k7_column_most(const __grid_constant__ PackList list) {
+  __shared__ unsigned int room[kRowWarps][32 * 4];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int k = 0;
+  while (k + 1 < list.count && blockIdx.x >= list.item[k + 1].first) ++k;
+  const PackItem& p = list.item[k];
+  if (p.vec == 4) column_most<4>(p, blockIdx.x - p.first, room);
+  else column_most<1>(p, blockIdx.x - p.first, room);
+}
+
 template <int KIND>
 __device__ __forceinline__ void pack_of(const PackItem& p, unsigned block) {
   constexpr int wide = KIND == kPackPieces ? 4 : 8;
@@ -215,6 +327,7 @@ __device__ __forceinline__ void pack_of(const PackItem& p, unsigned block) {
 }
 
 __global__ void __launch_bounds__(256) k7_pack(const __grid_constant__ PackList list) {
+  __shared__ unsigned int room[kRowWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int k = 0;
@@ -225,6 +338,14 @@ __global__ void __launch_bounds__(256) k7_pack(const __grid_constant__ PackList 
     case kPackPieces: pack_of<kPackPieces>(p, block); break;
     case kPackCopy: pack_of<kPackCopy>(p, block); break;
     case kPackCodesF16: pack_of<kPackCodesF16>(p, block); break;
+    case kPackPairsOfRows:
+      if (p.vec == 4) pack_pairs_of_rows<4>(p, block, room);
+      else pack_pairs_of_rows<1>(p, block, room);
+      break;
+    case kPackPairsOfColumns:
+      if (p.vec == 4) pack_pairs_of_columns<4>(p, block);
+      else pack_pairs_of_columns<1>(p, block);
+      break;
     default: pack_of<kPackCodesBF16>(p, block); break;
   }
 }
@@ -414,14 +535,15 @@ extern "C" int gtk_k7_stage(int type, const void* src, long long src_ld, const u
   return GTK_ERR_ARG;
 }
 
-// Up to three matrices to operands by one launch.  list: for each of them eight words - kind (0: f32 to three bf16 pieces,
-// 1: 16 bits as they are, 2 and 3: codes to f16 and bf16), address, leading dimension, exponents and their leading
-// dimension (codes), rows, columns, address of the operand (pitch: the columns rounded up to 8; pieces follow one
-// another), on 16 bytes.
+// Up to four matrices to operands by one launch.  list: for each of them eight words - kind (0: f32 to three bf16 pieces,
+// 1: 16 bits as they are, 2 and 3: codes to f16 and bf16, 4 and 5: f32 to two f16 pieces scaled by rows and by columns),
+// address, leading dimension, exponents (codes) or largest magnitudes (pairs: an unsigned int for each row, written
+// here, or for each column, zeros before the call), the exponents' leading dimension, rows, columns, address of the
+// operand (pitch: the columns rounded up to 8; pieces follow one another), on 16 bytes.
 extern "C" int gtk_k7_pack(gtk_addresses list, void* stream) {
-  if (list.n == 0 || list.n % 8 || list.n > 24) return GTK_ERR_ARG;
-  PackList l{};
-  unsigned long long blocks = 0;
+  if (list.n == 0 || list.n % 8 || list.n > 8 * kPackItems) return GTK_ERR_ARG;
+  PackList l{}, columns{};
+  unsigned long long blocks = 0, column_blocks = 0;
   for (unsigned i = 0; i < list.n / 8; ++i) {
     const unsigned long long* w = list.p + 8 * i;
     PackItem& p = l.item[i];
@@ -429,25 +551,43 @@ extern "C" int gtk_k7_pack(gtk_addresses list, void* stream) {
     p.src = Source{(const void*)w[1], (long long)w[2], (const unsigned char*)w[3], (long long)w[4]};
     p.rows = (long long)w[5];
     p.out = (void*)w[7];
+    p.most = (unsigned int*)w[3];
     const long long cols = (long long)w[6];
-    if (w[0] > 3 || !p.src.p || !p.out || p.rows <= 0 || cols <= 0 || cols > 0x3ffffff0 || p.src.ld < 0 || (uintptr_t)p.out % 16 ||
-        (w[0] >= 2 && !p.src.e))
+    if (w[0] > 5 || !p.src.p || !p.out || p.rows <= 0 || cols <= 0 || cols > 0x3ffffff0 || p.src.ld < 0 || (uintptr_t)p.out % 16 || (w[0] >= 2 && !w[3]))
       return GTK_ERR_ARG;
     p.cols = (int)cols;
     p.pitch = (p.cols + 7) / 8 * 8;
-    const int elem = p.kind == kPackPieces ? 4 : p.kind == kPackCopy ? 2 : 1, wide = p.kind == kPackPieces ? 4 : 8;
+    const bool f32 = p.kind == kPackPieces || p.kind >= kPackPairsOfRows;
+    const int elem = f32 ? 4 : p.kind == kPackCopy ? 2 : 1, wide = f32 ? 4 : 8;
     p.vec = 1;
     for (int vec : {wide, 4})
       if (p.vec == 1 && p.cols % vec == 0 && aligned(p.src.p, p.src.ld, elem, vec)) p.vec = vec;
-    p.strips = (unsigned)((p.pitch + 32 * p.vec - 1) / (32 * p.vec));
-    unsigned y;
-    if (!row_grid(p.rows, p.strips, &p.per, &y)) return GTK_ERR_UNSUPPORTED;
     p.first = (unsigned)blocks;
-    blocks += (unsigned long long)p.strips * y;
+    if (p.kind == kPackPairsOfRows) {
+      p.strips = p.cols <= 1024 ? 1u : 2u;
+      blocks += (unsigned long long)(p.strips == 1 ? (p.rows + kRowWarps - 1) / kRowWarps : p.rows);
+    } else {
+      p.strips = (unsigned)((p.pitch + 32 * p.vec - 1) / (32 * p.vec));
+      unsigned y;
+      if (!row_grid(p.rows, p.strips, &p.per, &y)) return GTK_ERR_UNSUPPORTED;
+      blocks += (unsigned long long)p.strips * y;
+      if (p.kind == kPackPairsOfColumns) {
+        PackItem& q = columns.item[columns.count++];
+        q = p;
+        q.first = (unsigned)column_blocks;
+        column_blocks += (unsigned long long)p.strips * y;
+      }
+    }
+    if (blocks > 0x7fffffffull) return GTK_ERR_UNSUPPORTED;
   }
-  if (blocks > 0x7fffffffull) return GTK_ERR_UNSUPPORTED;
   l.count = (int)(list.n / 8);
-  const cudaError_t err = launch_pdl(k7_pack, dim3((unsigned)blocks), dim3(32, kRowWarps), (cudaStream_t)stream, l);
+  cudaError_t err = cudaSuccess;
+  if (columns.count) {
+    err = launch_pdl(k7_column_most, dim3((unsigned)column_blocks), dim3(32, kRowWarps), (cudaStream_t)stream, columns);
+    gtk_count_launch(1);
+    if (err != cudaSuccess) return GTK_ERR_CUDA;
+  }
+  err = launch_pdl(k7_pack, dim3((unsigned)blocks), dim3(32, kRowWarps), (cudaStream_t)stream, l);
   gtk_count_launch(1);
   return err == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;
 }

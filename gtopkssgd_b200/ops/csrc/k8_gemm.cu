@@ -8,7 +8,9 @@
 // its matrix ("k-major": x and W forward) or the outer one ("mn-major": W for dx, both for dW); the tensor cores
 // take both, so nothing is transposed in memory.  f32 operands come as three bf16 pieces a value (8 + 8 + 8 bits of
 // the significand) and are multiplied piece by piece: the six products down to 2^-18 of the largest; what is left
-// out is below 2^-26.  The tensor cores cut a sum to 24 bits where they add to it instead of rounding it, which over
+// out is below 2^-26.  Or, where the products are long enough to pay for finding the largest magnitude of each row of
+// A and B, as two f16 pieces of 11 + 11 bits, scaled by a power of two so that the row's largest is just under 2^15:
+// three products, and what is left out is below 2^-24.  The tensor cores cut a sum to 24 bits where they add to it instead of rounding it, which over
 // the 6 * 1500 / 16 additions of K = 1500 took 1e-5 off the result (measured; f32 summed in order: 7e-7).  So the large
 // product has an accumulator apart from the five small ones, and every 256 of k both are added to f32 registers of the
 // epilogue's warps and begun again.
@@ -45,7 +47,7 @@ constexpr int kTileK = 64;            // 128 bytes of 16-bit elements: one swizz
 constexpr int kMaxBn = 256;           // columns of a tile
 constexpr int kGemmThreads = 384;     // warps 0 and 2 load A and B, warp 1 multiplies, warps 4 to 11 are the epilogue
 constexpr int kEpiWarps = 8;
-constexpr int kPatchPitch = 33;       // floats a row of the epilogue's buffer: no bank conflict along or across
+constexpr int kPatchPitch = 36;       // floats a row of the epilogue's buffer: no bank conflicts, 16 bytes a lane along rows or 4 across
 constexpr int kPatchBytes = kEpiWarps * 32 * kPatchPitch * 4;
 constexpr int kMaxStages = 8;
 constexpr int kF32Blocks = 4;         // f32: blocks of k that are summed in TMEM before they go to registers
@@ -60,7 +62,7 @@ struct GemmShape {
   int m, n, k;
   int tiles_m, tiles_n, blocks_k;
   int bn, stages, splits;
-  int wide;                            // the epilogue's matrices have rows on 16-byte boundaries
+  int wide;                            // the epilogue's matrices have rows on boundaries of 32 bytes (2), of 16 (1) or of neither (0)
   int a_pieces, b_pieces;
   int a_mn, b_mn;                      // 1: mn-major
   uint32_t idesc;
@@ -82,6 +84,8 @@ struct GemmEpilogue {
   void* h;                // slope: act(z') is stored here
   long long h_ld;
   float* sums;            // slope: [rows / 32, rounded up][n], sums of dz' over 32 rows each
+  const unsigned int* a_most;   // operands of two f16 pieces: the largest magnitudes (bits) of A's m and B's n, from
+  const unsigned int* b_most;   // which their scales follow
 };
 
 // ---- PTX ----------------------------------------------------------------------------------------------------------
@@ -220,6 +224,10 @@ __device__ __forceinline__ int piece_products(int a_pieces, int b_pieces, uint32
     *list = 0x048u;      // (0,2), (0,1), (0,0)
     return 3;
   }
+  if (a_pieces == 2) {
+    *list = 0x014u;      // (0,1), (1,0), (0,0); what is left out is below 2^-24
+    return 3;
+  }
   *list = 0;
   return 1;
 }
@@ -228,15 +236,61 @@ __device__ __forceinline__ int piece_products(int a_pieces, int b_pieces, uint32
 struct Patch {
   float* room;          // [32][kPatchPitch] of this warp
   int row, col0;        // this lane's row, the first column
-  int row0, m, n;
-  bool wide;
+  int row0, m, n, wide;
 };
+
+// The lane's row to and from the warp's buffer.
+__device__ __forceinline__ void patch_put(const Patch& p, const float (&v)[32]) {
+  __syncwarp();
+#pragma unroll
+  for (int g = 0; g < 8; ++g) *reinterpret_cast<float4*>(p.room + (int)lane_id() * kPatchPitch + 4 * g) = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+  __syncwarp();
+}
+__device__ __forceinline__ void patch_get(const Patch& p, float (&v)[32]) {
+  __syncwarp();
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {
+    const float4 x = *reinterpret_cast<const float4*>(p.room + (int)lane_id() * kPatchPitch + 4 * g);
+    v[4 * g] = x.x;
+    v[4 * g + 1] = x.y;
+    v[4 * g + 2] = x.z;
+    v[4 * g + 3] = x.w;
+  }
+}
+
+// 32 bytes at once: a lane's access touches a line of its own, so that half as many accesses take half the time.
+__device__ __forceinline__ void load32b(const void* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void store32b(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+               "r"(w[6]), "r"(w[7])
+               : "memory");
+}
 
 // v = the lane's row of a matrix of T, columns col0 .. col0 + 31; what is outside is left alone.
 template <typename T>
 __device__ __forceinline__ void read32(const void* base, long long ld, const Patch& p, float (&v)[32]) {
   constexpr int G = 16 / sizeof(T);
-  if (p.wide) {
+  if (p.wide == 2) {
+    if (p.row < p.m) {
+      const T* at = (const T*)base + (long long)p.row * ld + p.col0;
+#pragma unroll
+      for (int g = 0; g < 32; g += 2 * G) {
+        if (p.col0 + g < p.n) {   // n is a multiple of 2 G
+          uint32_t w[8];
+          load32b(at + g, w);
+          float x[2 * G];
+          to_f32<T, 2 * G>(*reinterpret_cast<const Vec<T, 2 * G>*>(w), x);
+#pragma unroll
+          for (int i = 0; i < 2 * G; ++i) v[g + i] = x[i];
+        }
+      }
+    }
+  } else if (p.wide) {
     if (p.row < p.m) {
       const T* at = (const T*)base + (long long)p.row * ld + p.col0;
 #pragma unroll
@@ -257,16 +311,32 @@ __device__ __forceinline__ void read32(const void* base, long long ld, const Pat
 #pragma unroll 8
       for (int r = 0; r < rows; ++r) p.room[r * kPatchPitch + (int)lane_id()] = to_f32(at[r * ld]);
     }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = p.room[(int)lane_id() * kPatchPitch + i];
+    patch_get(p, v);
   }
 }
 
 template <typename T>
 __device__ __forceinline__ void write32(void* base, long long ld, const Patch& p, const float (&v)[32]) {
   constexpr int G = 16 / sizeof(T);
-  if (p.wide) {
+  if (p.wide == 2) {
+    if (p.row < p.m) {
+      T* at = (T*)base + (long long)p.row * ld + p.col0;
+#pragma unroll
+      for (int g = 0; g < 32; g += 2 * G) {
+        if (p.col0 + g < p.n) {
+          uint32_t w[8];
+          if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = pack2(v[g + 2 * i], v[g + 2 * i + 1], T{});
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[g + i]);
+          }
+          store32b(at + g, w);
+        }
+      }
+    }
+  } else if (p.wide) {
     if (p.row < p.m) {
       T* at = (T*)base + (long long)p.row * ld + p.col0;
 #pragma unroll
@@ -281,10 +351,7 @@ __device__ __forceinline__ void write32(void* base, long long ld, const Patch& p
     }
   } else {
     const int col = p.col0 + (int)lane_id(), rows = min(32, p.m - p.row0);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) p.room[(int)lane_id() * kPatchPitch + i] = v[i];
-    __syncwarp();
+    patch_put(p, v);
     if (col < p.n) {
       T* at = (T*)base + (long long)p.row0 * ld + col;
 #pragma unroll 8
@@ -296,22 +363,33 @@ __device__ __forceinline__ void write32(void* base, long long ld, const Patch& p
 // The 8-bit form of the lane's 32 columns, one block.  Codes past the matrix are zeros.
 __device__ __forceinline__ void write_codes(const GemmEpilogue& e, const Patch& p, const float (&z)[32]) {
   if (p.row >= p.m) return;
-  uint32_t most = 0;
+  const bool whole = p.col0 + 32 <= p.n;
+  float most = 0.f;
+  uint32_t w[8], byte;
+  if (whole) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (p.col0 + i < p.n) most = max(most, __float_as_uint(z[i]) & 0x7fffffffu);
-  const uint32_t byte = block8_byte(most);
-  uint32_t w[8];
+    for (int i = 0; i < 32; i += 2) most = max_abs(most, z[i], z[i + 1]);
+    byte = block8_byte(__float_as_uint(most));
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    w[i] = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (p.col0 + 4 * i + j < p.n) w[i] |= ((uint32_t)block8_code(z[4 * i + j], byte) & 255u) << (8 * j);
+    for (int i = 0; i < 32; ++i)
+      if (p.col0 + i < p.n) most = max_abs(most, most, z[i]);
+    byte = block8_byte(__float_as_uint(most));
   }
-  uint4* at = reinterpret_cast<uint4*>(e.q + (long long)p.row * e.q_ld + p.col0);   // rows of whole blocks, 16-byte aligned
-  at[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  at[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  if (whole && byte < kBlock8Last) {
+    const float inverse = block8_inverse(byte);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = block8_codes(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3], inverse);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (p.col0 + 4 * i + j < p.n) w[i] |= ((uint32_t)block8_code(z[4 * i + j], byte) & 255u) << (8 * j);
+    }
+  }
+  store32b(e.q + (long long)p.row * e.q_ld + p.col0, w);   // rows of whole blocks
   e.e[(long long)p.row * e.e_ld + p.col0 / kBlock8] = (unsigned char)byte;
 }
 
@@ -321,6 +399,14 @@ __device__ __forceinline__ void read_codes(const GemmEpilogue& e, const Patch& p
     if (p.row < p.m) {
       const signed char* at = e.q + (long long)p.row * e.q_ld + p.col0;
       const float scale = block8_scale(e.e[(long long)p.row * e.e_ld + p.col0 / kBlock8]);
+      if (p.wide == 2) {   // n is a multiple of 32
+        uint32_t w[8];
+        load32b(at, w);
+        const Vec<signed char, 32>& q = *reinterpret_cast<const Vec<signed char, 32>*>(w);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z[i] = (float)q.v[i] * scale;
+        return;
+      }
 #pragma unroll
       for (int g = 0; g < 32; g += 16)
         if (p.col0 + g < p.n) {
@@ -339,13 +425,12 @@ __device__ __forceinline__ void read_codes(const GemmEpilogue& e, const Patch& p
         p.room[r * kPatchPitch + (int)lane_id()] = (float)e.q[row * e.q_ld + col] * block8_scale(e.e[row * e.e_ld + col / kBlock8]);
       }
     }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) z[i] = p.room[(int)lane_id() * kPatchPitch + i];
+    patch_get(p, z);
   }
 }
 
-// Sums of 32 columns over the 32 lanes; lane i gets column i's.  Halves the columns a lane holds at each step.
+// Sums of 32 columns over the 32 lanes; lane i gets column i's.  Halves the columns a lane holds at each step.  (Through
+// the warp's buffer instead it is half the instructions, but two stages of operands less: no faster.)
 __device__ __forceinline__ float transpose_sum(float (&v)[32]) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -420,6 +505,22 @@ __device__ __forceinline__ void finish_slope(float (&v)[32], const GemmEpilogue&
   }
 }
 
+// Takes the operands' scales out of the lane's 32 sums: times 2^-(shift of the row + shift of the column), in two steps,
+// neither of which leaves f32's range where the result does not.
+__device__ __forceinline__ void unscale(float (&v)[32], float* room, const GemmEpilogue& e, const Patch& p) {
+  int* shifts = reinterpret_cast<int*>(room);
+  const int col = p.col0 + (int)lane_id(), row = p.row < p.m ? pair_shift(e.a_most[p.row]) : 0;
+  __syncwarp();
+  shifts[lane_id()] = col < p.n ? pair_shift(e.b_most[col]) : 0;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const int t = -(row + shifts[i]), half = t >> 1;   // -252 .. 228
+    v[i] = v[i] * __uint_as_float((uint32_t)(half + 127) << 23) * __uint_as_float((uint32_t)(t - half + 127) << 23);
+  }
+  __syncwarp();
+}
+
 // T: type of what the epilogue reads and writes.  SLOPE: the input gradient through the layer before's activation.
 // Clusters of 2 * splits CTAs; with splits 1 the pairs go through tiles in turn, else a cluster has one tile.
 template <typename T, bool SLOPE>
@@ -468,7 +569,7 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_at;
-  pdl_begin(e.bias, e.add, e.z, e.q, e.e);
+  pdl_begin(e.bias, e.add, e.z, e.q, e.e, e.a_most, e.b_most);
 
   if (warp == 0 || warp == 2) {   // one for each operand: a copy takes its thread 130 cycles, a block of k 512 with 256 columns
     if (elect_one()) {
@@ -565,7 +666,7 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
   } else if (warp >= 4) {
     const int quad = warp & 3, side = (warp - 4) >> 2, lane = (int)lane_id();
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16), pair_acc_empty = mapa(acc_empty, leader);
-    Patch p{patches + (size_t)(warp - 4) * 32 * kPatchPitch, 0, 0, 0, s.m, s.n, s.wide != 0};
+    Patch p{patches + (size_t)(warp - 4) * 32 * kPatchPitch, 0, 0, 0, s.m, s.n, s.wide};
     int turn = 0;
     bool ok = true;
     for (int tile = first_tile; ok && tile < n_tiles; tile += step) {
@@ -577,6 +678,7 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
       auto finish = [&](int c, float (&v)[32]) {
         p.col0 = tn * s.bn + c;
         if (!some || p.col0 >= s.n) return;
+        if (kSplit && e.a_most) unscale(v, bias_room[warp - 4], e, p);
         if constexpr (SLOPE) finish_slope<T>(v, e, p);
         else finish_forward<T>(v, bias_room[warp - 4], e, p);
       };
@@ -651,7 +753,7 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
     const int quad = warp & 3, side = (warp - 4) >> 2, lane = (int)lane_id();
     int tm, tn;
     tile_at(s, first_tile, &tm, &tn);
-    Patch p{patches + (size_t)(warp - 4) * 32 * kPatchPitch, 0, 0, tm * kTileM + (int)half * kRows + quad * 32, s.m, s.n, s.wide != 0};
+    Patch p{patches + (size_t)(warp - 4) * 32 * kPatchPitch, 0, 0, tm * kTileM + (int)half * kRows + quad * 32, s.m, s.n, s.wide};
     p.row = p.row0 + lane;
     if (p.row0 < s.m)
       for (int c = ((int)split + side * s.splits) * 32; c < s.bn; c += 64 * s.splits) {
@@ -678,6 +780,7 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
             v[4 * g + 3] += x[g].w;
           }
         }
+        if (kSplit && e.a_most) unscale(v, bias_room[warp - 4], e, p);
         if constexpr (SLOPE) finish_slope<T>(v, e, p);
         else finish_forward<T>(v, bias_room[warp - 4], e, p);
       }
@@ -711,6 +814,7 @@ struct Operand {
   int pieces;
   long long piece_stride;
   int mn_major;
+  const unsigned int* most;   // two pieces: the largest magnitudes
 };
 
 inline bool encode(CUtensorMap* map, const Operand& o, int half, long long rows, long long k, int box_rows) {
@@ -726,7 +830,7 @@ inline bool encode(CUtensorMap* map, const Operand& o, int half, long long rows,
 }
 
 inline bool operand_ok(const Operand& o) {
-  return o.p && (uintptr_t)o.p % 16 == 0 && o.ld > 0 && o.ld % 8 == 0 && (o.pieces == 1 || (o.pieces == 3 && o.piece_stride > 0 && o.piece_stride % 8 == 0));
+  return o.p && (uintptr_t)o.p % 16 == 0 && o.ld > 0 && o.ld % 8 == 0 && (o.pieces == 1 || ((o.pieces == 3 || (o.pieces == 2 && o.most)) && o.piece_stride > 0 && o.piece_stride % 8 == 0));
 }
 
 // Pairs that run side by side in clusters of `splits` of them (74, 66 and 56 of 1, 2 and 4 on B200: a cluster lies within
@@ -759,8 +863,9 @@ int pairs_of(Kernel kernel, int splits, const DeviceInfo* info) {
 }
 
 // Tiles and splits.  In cycles, a pair takes about 2 * bn for the products of a block of k (times six with pieces), at
-// least 330 for its copies, 24 a column for a tile's last epilogue and 3000 + 16 a column for joining several pairs'
-// sums (256 x 256: 3.6 us with two, 4.8 with four).  The choice is the one whose busiest pair is done first.
+// least 330 for its copies (pieces: 5/4 of it, as shared memory is read faster than it can be), 24 a column for a tile's
+// last epilogue and 3000 + 16 a column for joining several pairs' sums (256 x 256: 3.6 us with two, 4.8 with four) and
+// as much again where clusters follow one another.  The choice is the one whose busiest pair is done first.
 struct GemmPlan {
   int bn, splits;
 };
@@ -769,12 +874,12 @@ inline GemmPlan plan_gemm(long long m, long long n, int blocks_k, int products, 
   long long least = -1;
   for (int bn = most; bn >= 128; bn /= 2) {
     const long long tiles = ((m + kTileM - 1) / kTileM) * ((n + bn - 1) / bn);
-    const long long block = 2 * bn * products > 330 ? 2 * bn * products : 330;
+    const long long block = products > 1 ? 2 * bn * products * 5 / 4 : 2 * bn > 330 ? 2 * bn : 330;
     for (int splits = 1; splits <= kMaxSplits; ++splits) {
       const int pairs = pairs_of(k8_gemm<__nv_bfloat16, false>, splits, info);
-      if (splits > 1 && (blocks_k < 4 * splits || tiles * splits > pairs)) break;
+      if (splits > 1 && blocks_k < 4 * splits) break;
       const long long rounds = (tiles * splits + pairs - 1) / pairs;
-      const long long cost = rounds * ((blocks_k + splits - 1) / splits) * block + bn * 24 / splits + (splits > 1 ? 3000 + 16 * bn : 0);
+      const long long cost = rounds * ((blocks_k + splits - 1) / splits) * block + bn * 24 / splits + (splits > 1 ? rounds * (3000 + 16 * bn) : 0);
       if (least < 0 || cost < least) {
         least = cost;
         best = GemmPlan{bn, splits};
@@ -784,7 +889,7 @@ inline GemmPlan plan_gemm(long long m, long long n, int blocks_k, int products, 
   return best;
 }
 
-inline bool on16(const void* p, long long ld, int elem) { return !p || ((uintptr_t)p % 16 == 0 && ld * elem % 16 == 0); }
+inline bool on(int bytes, const void* p, long long ld, int elem) { return !p || ((uintptr_t)p % bytes == 0 && ld * elem % bytes == 0); }
 
 template <typename T>
 cudaError_t launch_gemm(int device, bool slope, int grid, size_t shared, cudaStream_t stream, const CUtensorMap& a, const CUtensorMap& b, const GemmShape& s,
@@ -833,11 +938,13 @@ extern "C" unsigned int gtk_k8_status(void) {
 // f16, else bf16.  Leading dimensions and piece strides of operands are multiples of 8 elements, their addresses of
 // 16 bytes.  slope: see the top of this file.  sums with db: the sums over all rows of what the slope form stores.
 extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long long k, const void* a, long long a_ld, int a_pieces, long long a_stride, int a_mn,
-                           const void* b, long long b_ld, int b_pieces, long long b_stride, int b_mn, void* out, long long out_ld, const void* bias,
+                           const unsigned int* a_most, const void* b, long long b_ld, int b_pieces, long long b_stride, int b_mn, const unsigned int* b_most,
+                           void* out, long long out_ld, const void* bias,
                            const void* add, long long add_ld, int act, int slope, void* z, long long z_ld, signed char* q, long long q_ld, unsigned char* e8,
                            long long e_ld, void* h, long long h_ld, float* sums, void* db, void* stream_) {
-  const Operand oa{a, a_ld, a_pieces, a_stride, a_mn != 0}, ob{b, b_ld, b_pieces, b_stride, b_mn != 0};
-  if (m <= 0 || n <= 0 || k <= 0 || !out || act < 0 || act >= kActCount || !operand_ok(oa) || !operand_ok(ob) || (q && !e8) || (q && !slope && (q_ld < (n + kBlock8 - 1) / kBlock8 * kBlock8 || q_ld % 16 || (uintptr_t)q % 16)) || (sums == nullptr) != (db == nullptr))
+  const Operand oa{a, a_ld, a_pieces, a_stride, a_mn != 0, a_most}, ob{b, b_ld, b_pieces, b_stride, b_mn != 0, b_most};
+  if (m <= 0 || n <= 0 || k <= 0 || !out || act < 0 || act >= kActCount || !operand_ok(oa) || !operand_ok(ob) || (q && !e8) || (q && !slope && (q_ld < (n + kBlock8 - 1) / kBlock8 * kBlock8 || q_ld % 32 || (uintptr_t)q % 32)) || (sums == nullptr) != (db == nullptr) ||
+      ((a_pieces == 2) != (b_pieces == 2)) || (a_pieces == 2 && (!half || type != kF32)) || ((a_pieces == 3 || b_pieces == 3) && (half || type != kF32)))
     return GTK_ERR_ARG;
   if (m > 0x7fffff00LL || n > 0x7fffff00LL || k > 0x7fffff00LL) return GTK_ERR_UNSUPPORTED;
   const DeviceInfo* info = gtk_device_info();
@@ -852,14 +959,16 @@ extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long lo
   s.b_mn = ob.mn_major;
   s.tiles_m = (int)((m + kTileM - 1) / kTileM);
   s.blocks_k = (int)((k + kTileK - 1) / kTileK);
-  const GemmPlan plan = plan_gemm(m, n, s.blocks_k, a_pieces * b_pieces == 9 ? 6 : a_pieces * b_pieces, type == kF32 ? 128 : kMaxBn, info);
+  const GemmPlan plan = plan_gemm(m, n, s.blocks_k, a_pieces * b_pieces == 9 ? 6 : a_pieces == 2 ? 3 : a_pieces * b_pieces, type == kF32 ? 128 : kMaxBn, info);
   s.bn = plan.bn;
   s.splits = plan.splits;
   s.tiles_n = (int)((n + s.bn - 1) / s.bn);
   if ((long long)s.tiles_m * s.tiles_n > 0x3fffffffLL) return GTK_ERR_UNSUPPORTED;
   const int elem = elem_bytes(type);
-  s.wide = n * elem % 16 == 0 && on16(out, out_ld, elem) && on16(add, add_ld, elem) && on16(z, z_ld, elem) && on16(h, h_ld, elem) &&
-           (!q || !slope || (n % 16 == 0 && on16(q, q_ld, 1)));
+  for (const int bytes : {16, 32})
+    if (n * elem % bytes == 0 && on(bytes, out, out_ld, elem) && on(bytes, add, add_ld, elem) && on(bytes, z, z_ld, elem) && on(bytes, h, h_ld, elem) &&
+        (!q || !slope || (n % bytes == 0 && on(bytes, q, q_ld, 1))))
+      s.wide = bytes / 16;
   const int stage_bytes = a_pieces * kRows * 128 + b_pieces * s.bn / 2 * 128;
   const int fixed = 1024 + (s.wide ? 0 : kPatchBytes);
   s.stages = (kMaxShared - kStaticShared - fixed) / stage_bytes;
@@ -868,7 +977,7 @@ extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long lo
   s.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)s.a_mn << 15) | ((uint32_t)s.b_mn << 16) | ((uint32_t)(s.bn >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
   CUtensorMap am, bm;
   if (!encode(&am, oa, half, m, k, kRows) || !encode(&bm, ob, half, n, k, s.bn / 2)) return GTK_ERR_CUDA;
-  const GemmEpilogue ep{out, out_ld, bias, add, add_ld, act, z, z_ld, q, q_ld, e8, e_ld, h, h_ld, sums};
+  const GemmEpilogue ep{out, out_ld, bias, add, add_ld, act, z, z_ld, q, q_ld, e8, e_ld, h, h_ld, sums, a_pieces == 2 ? a_most : nullptr, b_most};
   const int tiles = s.tiles_m * s.tiles_n, pairs = info->sms / 2;
   const int grid = 2 * (s.splits > 1 ? tiles * s.splits : tiles < pairs ? tiles : pairs);
   const size_t shared = (size_t)stage_bytes * s.stages + fixed;

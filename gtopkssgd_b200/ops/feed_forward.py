@@ -18,7 +18,7 @@ import torch
 from . import layers_oracle as oracle
 from .activation8 import Activation8, act_of, bits_of, colsum, matrix, parameter, same, shaped, stream_of, type_of
 from .layer_norm import layer_norm_backward, layer_norm_forward
-from .linear import _check, _gradients, linear_forward, normed_operand, operands, product
+from .linear import _check, _gradients, linear_forward, normed, operands, pairs_for, product
 
 
 class FeedForwardKept(NamedTuple):
@@ -76,16 +76,21 @@ def feed_forward_backward(dy: torch.Tensor, kept: FeedForwardKept, norm_weight: 
         return (new(shape), *(new(n).zero_() for n in (dim, dim, (hidden, dim), hidden, (dim, hidden), dim)))
     stream = stream_of(g)
     mean, rstd = mean.contiguous(), rstd.contiguous()
+    pairs = pairs_for(dy.dtype, True, rows, hidden, dim)
     # dz = (dy W2) act'(z) and h = act(z) again, both in the product's epilogue
     dz, h, db1 = new((rows, hidden)), new((rows, hidden)), new(hidden)
-    go, w2o = operands(g, matrix(w2))
+    go, w2o = operands(pairs, (g, 1), (matrix(w2), 0))
     product(rows, hidden, dim, go, False, w2o, True, dz, stream, activation=code, slope=True, z=z, h=h, db=db1)
     del w2o
     dw2 = new((dim, hidden))
-    product(dim, hidden, rows, go, True, operands(h)[0], True, dw2, stream)
-    del h, go
+    if pairs:
+        go, ho = operands(True, (g, 0), (h, 0))
+    else:
+        ho, = operands(False, (h, 0))
+    product(dim, hidden, rows, go, True, ho, True, dw2, stream)
+    del h, go, ho
     _, db2 = colsum(g)
-    a = normed_operand(x if isinstance(x, Activation8) else matrix(x), mean, rstd, norm_weight, norm_bias)   # the norm's output again
+    a = normed(x if isinstance(x, Activation8) else matrix(x), mean, rstd, norm_weight, norm_bias, pairs)   # the norm's output again
     da, dw1 = _gradients(dz, a, w1, True, True)
     dx, dg, db = layer_norm_backward(da.view(shape), x.restore() if isinstance(x, Activation8) else x, mean, rstd, norm_weight, add=dy)
     return dx, dg, db, dw1, db1, dw2, db2

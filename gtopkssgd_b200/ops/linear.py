@@ -4,7 +4,7 @@
 ``linear_backward`` are its two directions.  y = act(x W^T + bias) + residual, x
 any shape [..., inner], weight [outer, inner] as in ``nn.Linear``; f32, f16 or bf16,
 one type for all.  Products are summed in f32.  f32 operands are multiplied as three
-bf16 pieces a value, which keeps f32's accuracy.  In the 16-bit types the gradient
+bf16 pieces a value, or two scaled f16 ones, which keeps f32's accuracy.  In the 16-bit types the gradient
 dz = dy * act'(z) is rounded to the type between the products, as their operand.
 """
 from __future__ import annotations
@@ -27,62 +27,100 @@ def status() -> int:
 
 
 class Operand:
-    """A matrix as the tensor cores read it: 16-bit pieces with rows on 16-byte boundaries."""
+    """A matrix as the tensor cores read it: 16-bit pieces with rows on 16-byte boundaries.  ``most``: the largest
+    magnitudes that two f16 pieces were scaled by, else 0."""
 
-    __slots__ = ("at", "ld", "pieces", "stride", "held")
+    __slots__ = ("at", "ld", "pieces", "stride", "most", "held")
 
-    def __init__(self, at, row, pieces, stride, held):
-        self.at, self.ld, self.pieces, self.stride, self.held = at, row, pieces, stride, held
+    def __init__(self, at, row, pieces, stride, most, held):
+        self.at, self.ld, self.pieces, self.stride, self.most, self.held = at, row, pieces, stride, most, held
 
 
-def operands(*sources) -> list:
-    """Matrices or codes (``Activation8``), up to three, as operands.  A 16-bit matrix whose rows lie on 16-byte
-    boundaries is read where it is; one launch makes all the others."""
-    made, words, size = [], [], 0
-    for src in sources:
+# f32 operands as two scaled f16 pieces (three products) from this many multiplications a product on, as three bf16 pieces
+# (six products) below.  Forward the scales are found where the pieces are made; a backward pass's operands, scaled by
+# columns, take two launches more and are read once more.  Both ways, us a pass forward and backward: 512 x 1024 x 1024
+# 18 and 42 against 20 and 38; 2048 x 1024 x 1024 25 and 66 against 31 and 66; 700 x 1500 x 10000 111 and 246 against 132
+# and 292.
+PAIRS_FROM_FORWARD = 500_000_000
+PAIRS_FROM_BACKWARD = 2_200_000_000
+
+
+def pairs_for(dtype: torch.dtype, backward: bool, m: int, n: int, k: int) -> bool:
+    return dtype is _FLOAT and m * n * k >= (PAIRS_FROM_BACKWARD if backward else PAIRS_FROM_FORWARD)
+
+
+def operands(pairs: bool, *specs) -> list:
+    """Up to four matrices or codes (``Activation8``) as operands; each comes as (matrix, contracted), ``contracted`` the
+    axis of it that the product sums over.  A 16-bit matrix whose rows lie on 16-byte boundaries is read where it is;
+    one launch makes all the others (``pairs``: f32 as two f16 pieces)."""
+    made, words, size, row_most, column_most = [], [], 0, 0, 0
+    for src, contracted in specs:
         codes = type(src) is Activation8
+        f32 = src.dtype is _FLOAT
+        if codes and pairs:
+            src, codes = src.restore().view(src.q.shape), False
         m = src.q if codes else src
         rows, cols = m.shape
         row = ld(m)
-        f32 = src.dtype is _FLOAT
         if not codes and not f32 and row % 8 == 0 and row >= cols and m.data_ptr() % 16 == 0:
-            made.append(Operand(m.data_ptr(), row, 1, 0, m))
+            made.append(Operand(m.data_ptr(), row, 1, 0, 0, m))
             continue
         pitch = (cols + 7) & ~7
-        pieces = 3 if f32 and not codes else 1
-        kind = (2 if src.dtype is torch.float16 else 3) if codes else 0 if f32 else 1
-        words += (kind, m.data_ptr(), row, src.e.data_ptr() if codes else 0, ld(src.e) if codes else 0, rows, cols, size)
-        made.append(Operand(size, pitch, pieces, rows * pitch, None))
+        if codes:
+            kind, pieces, scale = 2 if src.dtype is torch.float16 else 3, 1, src.e.data_ptr()
+        elif not f32:
+            kind, pieces, scale = 1, 1, 0
+        elif not pairs:
+            kind, pieces, scale = 0, 3, 0
+        elif contracted == 1:
+            kind, pieces, scale = 4, 2, row_most
+            row_most += rows
+        else:
+            kind, pieces, scale = 5, 2, column_most
+            column_most += cols
+        words += (kind, m.data_ptr(), row, scale, ld(src.e) if codes else 0, rows, cols, size)
+        made.append(Operand(size, pitch, pieces, rows * pitch, scale if kind >= 4 else 0, (m, kind)))
         size += pieces * rows * pitch * 2
     if words:
-        src = sources[0]
-        room = (src.q if type(src) is Activation8 else src).new_empty(size, dtype=torch.uint8)
-        base = room.data_ptr()
-        for i in range(7, len(words), 8):
-            words[i] += base
-        for o in made:
-            if o.held is None:
-                o.at, o.held = o.at + base, room
+        src = specs[0][0]
+        like = src.q if type(src) is Activation8 else src
+        room = like.new_empty(size + 4 * row_most, dtype=torch.uint8)
+        zeros = like.new_zeros(column_most, dtype=torch.int32) if column_most else None
+        base, rows_at, columns_at = room.data_ptr(), room.data_ptr() + size, zeros.data_ptr() if column_most else 0
+        for i in range(0, len(words), 8):
+            words[i + 7] += base
+            if words[i] == 4:
+                words[i + 3] = rows_at + 4 * words[i + 3]
+            elif words[i] == 5:
+                words[i + 3] = columns_at + 4 * words[i + 3]
         err = _lib.calls().gtk_k7_pack(words, stream_of(room))
         if err:
             _lib.check(err, "gtk_k7_pack")
+        for o in made:
+            if type(o.held) is tuple:
+                kind = o.held[1]
+                o.at += base
+                if kind >= 4:
+                    o.most = (rows_at if kind == 4 else columns_at) + 4 * o.most
+                o.held = (room, zeros)
     return made
 
 
-def normed_operand(src, mean, rstd, weight, bias) -> Operand:
-    """The operand (v - mean) * rstd * weight + bias of a matrix or of codes."""
+def normed(src, mean, rstd, weight, bias, pairs: bool):
+    """The matrix (v - mean) * rstd * weight + bias of a matrix or of codes, as an operand (f32 with ``pairs``: as a
+    matrix, for ``operands``)."""
     codes = type(src) is Activation8
     m = src.q if codes else src
     rows, cols = m.shape
-    f32 = src.dtype is _FLOAT
-    pieces, pitch = 3 if f32 else 1, (cols + 7) & ~7
-    out = m.new_empty((pieces, rows, pitch), dtype=torch.bfloat16 if f32 else src.dtype)
+    split = src.dtype is _FLOAT and not pairs
+    pieces, pitch = (3, (cols + 7) & ~7) if split else (1, cols if pairs else (cols + 7) & ~7)
+    out = m.new_empty((pieces, rows, pitch), dtype=torch.bfloat16 if split else src.dtype)
     err = _lib.calls().gtk_k7_stage(TYPES[src.dtype], m.data_ptr(), ld(m), src.e.data_ptr() if codes else None, ld(src.e) if codes else 0,
-                                    mean.data_ptr(), rstd.data_ptr(), _ptr(weight), _ptr(bias), 0, 3 if f32 else 0, out.data_ptr(), pitch,
+                                    mean.data_ptr(), rstd.data_ptr(), _ptr(weight), _ptr(bias), 0, 3 if split else 0, out.data_ptr(), pitch,
                                     rows * pitch, rows, cols, pitch, stream_of(m))
     if err:
         _lib.check(err, "gtk_k7_stage")
-    return Operand(out.data_ptr(), pitch, pieces, rows * pitch, out)
+    return out[0] if pairs else Operand(out.data_ptr(), pitch, pieces, rows * pitch, 0, out)
 
 
 def product(m: int, n: int, k: int, a: Operand, a_mn: bool, b: Operand, b_mn: bool, out: torch.Tensor, stream: int, bias=None, add=None,
@@ -101,8 +139,8 @@ def product(m: int, n: int, k: int, a: Operand, a_mn: bool, b: Operand, b_mn: bo
         zp, zld = z.data_ptr(), ld(z)
     if db is not None:
         sums = out.new_empty((-(-m // 32), n), dtype=_FLOAT)
-    err = _lib.calls().gtk_k8_gemm(TYPES[out.dtype], out.dtype is torch.float16, m, n, k, a.at, a.ld, a.pieces, a.stride, a_mn, b.at, b.ld, b.pieces,
-                                   b.stride, b_mn, out.data_ptr(), n, _ptr(bias), _ptr(add), 0 if add is None else ld(add), activation, slope, zp,
+    err = _lib.calls().gtk_k8_gemm(TYPES[out.dtype], out.dtype is torch.float16 or a.pieces == 2, m, n, k, a.at, a.ld, a.pieces, a.stride, a_mn,
+                                   a.most or None, b.at, b.ld, b.pieces, b.stride, b_mn, b.most or None, out.data_ptr(), n, _ptr(bias), _ptr(add), 0 if add is None else ld(add), activation, slope, zp,
                                    zld, q, qld, e, eld, _ptr(h), n, _ptr(sums), _ptr(db), stream)
     if err:
         _lib.check(err, "gtk_k8_gemm")
@@ -143,27 +181,35 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
     if keep:
         z = Activation8.empty(x, rows, outer, (rows, outer)) if bits else x.new_empty((rows, outer))
     if rows and outer:
-        a, b = operands(m, matrix(weight))
+        a, b = operands(pairs_for(x.dtype, False, rows, outer, inner), (m, 1), (matrix(weight), 1))
         product(rows, outer, inner, a, False, b, False, y, stream_of(m), bias, residual, code, z=z)
     return y, z
 
 
 def _gradients(dz: torch.Tensor, x, weight: torch.Tensor, need_dx: bool, need_dw: bool):
-    """(dz W, dz^T x) over CUDA matrices; x may be codes, or an operand already."""
+    """(dz W, dz^T x) over CUDA matrices; x may be codes, or (not for ``pairs_for``) an operand already."""
     rows, outer = dz.shape
     inner = weight.size(1)
     dx = dw = None
     if not (need_dx or need_dw):
         return dx, dw
     stream = stream_of(dz)
-    made = type(x) is Operand
-    a, *rest = operands(dz, *((matrix(weight),) if need_dx else ()), *((x,) if need_dw and not made else ()))
+    pairs = pairs_for(dz.dtype, True, rows, outer, inner)
+    specs = [(dz, 1)] if need_dx or not pairs else []
+    if need_dx:
+        specs.append((matrix(weight), 0))
+    if need_dw and pairs:
+        specs.append((dz, 0))
+    if need_dw and type(x) is not Operand:
+        specs.append((x, 0))
+    made = operands(pairs, *specs)
     if need_dx:
         dx = dz.new_empty((rows, inner))
-        product(rows, inner, outer, a, False, rest[0], True, dx, stream)
+        product(rows, inner, outer, made[0], False, made[1], True, dx, stream)
     if need_dw:
         dw = dz.new_empty((outer, inner))
-        product(outer, inner, rows, a, True, x if made else rest[-1], True, dw, stream)
+        a, b = (made[-2], made[-1]) if pairs else (made[0], x if type(x) is Operand else made[-1])
+        product(outer, inner, rows, a, True, b, True, dw, stream)
     return dx, dw
 
 
