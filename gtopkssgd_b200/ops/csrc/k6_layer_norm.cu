@@ -11,6 +11,8 @@
 // instructions an element forward and 70 backward, and their issue, not memory, set the time.  In the backward pass the column sums of
 // a thread's own columns stay in its registers all along, the groups of a CTA join theirs in shared memory, and
 // col_finish adds up one line per CTA.
+#include <atomic>
+
 #include "colsum.cuh"
 #include "common.cuh"
 #include "host_api.h"
@@ -229,10 +231,11 @@ __global__ void __launch_bounds__(1024) k6_norm_forward_long(const T* x, const T
 // partial: [gridDim.x][2 * cols], sums of dy xh, then of dy.  blockDim = (32 * warps, groups).  Dynamic shared memory:
 // `depth` rows of x, as many of dy, of every group; afterwards the groups' column sums.  THREADS: the most that it is
 // launched with; with 1024 (rows over 8192 elements) the column sums lie in shared memory all along, and rows are
-// loaded when they are used.
+// loaded when they are used.  A single CTA stores the gradients of weight and bias itself.
 template <typename T, int VEC, int NV, int THREADS>
 __global__ void __launch_bounds__(THREADS)
-k6_norm_backward(const T* dy, const T* x, const float* mean, const float* rstd, const T* w, const T* add, T* dx, float* partial, NormShape s) {
+k6_norm_backward(const T* dy, const T* x, const float* mean, const float* rstd, const T* w, const T* add, T* dx, T* dw_out, T* db_out, float* partial,
+                 NormShape s) {
   constexpr bool kShared = THREADS > 512;
   extern __shared__ uint4 dynamic[];   // then [groups - 1][2 * cols], or [2 * cols], of floats
   __shared__ alignas(16) float scratch[8][2][2 * kNormMaxWarps];
@@ -363,7 +366,7 @@ k6_norm_backward(const T* dy, const T* x, const float* mean, const float* rstd, 
   float* line = partial + (size_t)blockIdx.x * 2 * s.cols;
   __syncthreads();
   if constexpr (kShared) {
-    for (int c = at; c < 2 * s.cols; c += threads) line[c] = joined[c];
+    for (int c = at; c < 2 * s.cols; c += threads) line[c] = joined[c];   // (never a single CTA)
   } else {
     if (group) {
       float* own = joined + (size_t)(group - 1) * 2 * s.cols;
@@ -392,8 +395,16 @@ k6_norm_backward(const T* dy, const T* x, const float* mean, const float* rstd, 
               db[i][j] += d[j];
             }
           }
-          store_f32<float, VEC>(line + c, dw[i]);
-          store_f32<float, VEC>(line + s.cols + c, db[i]);
+          if (gridDim.x == 1) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {   // (no vector: the two may lie anywhere)
+              if (dw_out) dw_out[c + j] = from_f32<T>(dw[i][j]);
+              if (db_out) db_out[c + j] = from_f32<T>(db[i][j]);
+            }
+          } else {
+            store_f32<float, VEC>(line + c, dw[i]);
+            store_f32<float, VEC>(line + s.cols + c, db[i]);
+          }
         }
       }
     }
@@ -504,11 +515,18 @@ int pick_vec(long long cols, std::initializer_list<std::pair<const void*, long l
 
 constexpr int kNormShared = 200 * 1024;   // dynamic shared memory of an SM that the rows under way may take
 
-template <typename... K, typename... A>
-cudaError_t launch_norm(void (*kernel)(K...), long long grid, int warps, int groups, size_t shared, cudaStream_t stream, A... args) {
+template <auto Kernel, typename... A>
+cudaError_t launch_norm(long long grid, int warps, int groups, size_t shared, cudaStream_t stream, A... args) {
   if (shared > 32 * 1024) {
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormShared);
-    if (err != cudaSuccess) return err;
+    static std::atomic<unsigned long long> devices;   // that this kernel has been given its shared memory on
+    const DeviceInfo* info = gtk_device_info();
+    if (!info) return cudaErrorInvalidDevice;
+    const unsigned long long bit = 1ull << info->device;
+    if (!(devices.load(std::memory_order_relaxed) & bit)) {
+      const cudaError_t err = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormShared);
+      if (err != cudaSuccess) return err;
+      devices.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
@@ -520,7 +538,7 @@ cudaError_t launch_norm(void (*kernel)(K...), long long grid, int warps, int gro
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(args)...);
+  return cudaLaunchKernelEx(&cfg, Kernel, args...);
 }
 
 template <typename T>
@@ -542,8 +560,8 @@ int norm_forward(const void* x, const void* w, const void* b, void* y, float* me
     const long long all = (s.rows + groups - 1) / groups, grid = all < 148LL * ctas ? all : 148LL * ctas;
     while (s.depth > 1 && ((s.depth - 1) * grid >= all || vec * sizeof(T) < 4)) --s.depth;
     if (!with_plan<T>(p, [&](auto V, auto N) {
-          e = launch_norm(k6_norm_forward<T, decltype(V)::value, decltype(N)::value>, grid, p.warps, groups, slot * s.depth, stream, (const T*)x,
-                          (const T*)w, (const T*)b, (T*)y, mean, rstd, s);
+          e = launch_norm<k6_norm_forward<T, decltype(V)::value, decltype(N)::value>>(grid, p.warps, groups, slot * s.depth, stream, (const T*)x, (const T*)w,
+                          (const T*)b, (T*)y, mean, rstd, s);
         }))
       return GTK_ERR_UNSUPPORTED;
   }
@@ -577,10 +595,13 @@ int norm_backward(const void* dy, const void* x, const float* mean, const float*
   } else {
     const size_t line_bytes = 2 * (size_t)s.cols * 4;
     int groups = shared ? 1 : 16 / p.warps > 8 ? 8 : 16 / p.warps;
-    while (groups > 1 && s.rows < 148LL * groups) --groups;
+    // One CTA takes up to four rows a group: 1.4 us each, of which all but one are more than with a CTA a row, against a
+    // launch less (2.5 us on the device, 2.6 of host time)
+    const bool one = sums && !shared && s.rows <= 4LL * groups;
+    while (!one && groups > 1 && s.rows < 148LL * groups) --groups;
     const size_t slot = (size_t)groups * p.warps * 32 * p.nv * p.vec * sizeof(T) * 2;   // of x and dy
     const long long need = (s.rows + groups - 1) / groups;
-    lines = need < kNormLines ? (int)need : kNormLines;
+    lines = one ? 1 : need < 2 ? 2 : need < kNormLines ? (int)need : kNormLines;
     s.depth = ring_depth(slot, kNormShared);
     while (s.depth > 1 && ((long long)(s.depth - 1) * lines >= need || vec * sizeof(T) < 4)) --s.depth;
     size_t dynamic = shared ? 0 : slot * s.depth;
@@ -588,15 +609,16 @@ int norm_backward(const void* dy, const void* x, const float* mean, const float*
     dynamic = dynamic > join ? dynamic : join;
     if (!with_plan<T>(p, [&](auto V, auto N) {
           constexpr int kV = decltype(V)::value, kN = decltype(N)::value;
-          auto go = [&](auto kernel) {
-            e = launch_norm(kernel, lines, p.warps, groups, dynamic, stream, (const T*)dy, (const T*)x, mean, rstd, (const T*)w, (const T*)add, (T*)dx, sums, s);
+          auto go = [&](auto threads) {
+            e = launch_norm<k6_norm_backward<T, kV, kN, decltype(threads)::value>>(lines, p.warps, groups, dynamic, stream, (const T*)dy, (const T*)x, mean, rstd,
+                                                                                   (const T*)w, (const T*)add, (T*)dx, (T*)dw, (T*)db, sums, s);
           };
-          if (!shared) go(k6_norm_backward<T, kV, kN, 512>);
-          else if constexpr (kV * kN == 16) go(k6_norm_backward<T, kV, kN, 1024>);   // over 8192 elements of 32 warps
+          if (!shared) go(std::integral_constant<int, 512>{});
+          else if constexpr (kV * kN == 16) go(std::integral_constant<int, 1024>{});   // over 8192 elements of 32 warps
           else e = cudaErrorInvalidConfiguration;
         }))
       return GTK_ERR_UNSUPPORTED;
-    if (!sums) {
+    if (!sums || lines == 1) {
       gtk_count_launch(1);
       return e == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;
     }

@@ -350,10 +350,11 @@ __global__ void __launch_bounds__(256) k7_pack(const __grid_constant__ PackList 
   }
 }
 
-// Z: element type of z (signed char: codes).  dz may be null (sums only); partial may be null.
+// Z: element type of z (signed char: codes).  dz may be null (sums only); partial and db may be null.  With one line of
+// partial sums they are the sums, and are stored as such.
 template <typename T, typename Z, int VEC>
-__global__ void __launch_bounds__(256) k7_act_backward(const T* dy, long long dy_ld, Source z, int act, T* dz, long long dz_ld, float* partial, long long rows,
-                                                       int cols) {
+__global__ void __launch_bounds__(256) k7_act_backward(const T* dy, long long dy_ld, Source z, int act, T* dz, long long dz_ld, T* db, float* partial,
+                                                       long long rows, int cols) {
   __shared__ float joined[kRowWarps][32 * VEC];
   pdl_begin(dy, z.p, z.e);
   const int c = (int)((blockIdx.x * 32 + threadIdx.x) * VEC);
@@ -388,7 +389,8 @@ __global__ void __launch_bounds__(256) k7_act_backward(const T* dy, long long dy
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < kRowWarps; ++k) s += joined[k][i];
-    partial[(size_t)blockIdx.y * cols + col] = s;
+    if (gridDim.y == 1) db[col] = from_f32<T>(s);
+    else partial[(size_t)blockIdx.y * cols + col] = s;
   }
 }
 
@@ -462,8 +464,9 @@ int act_backward(const void* dy, long long dy_ld, Source z, int act, void* dz, l
     const long long most = (rows + kRowWarps - 1) / kRowWarps;
     if (y > most) y = most;
     if (y > max_lines) y = max_lines;
+    if (db && rows <= 8 * kRowWarps) y = 1;   // eight rows a warp: less than the launch that adds lines up
     lines = (unsigned)y;
-    return launch_pdl(k7_act_backward<T, Z, VEC>, dim3(strips, lines), dim3(32, kRowWarps), stream, (const T*)dy, dy_ld, z, act, (T*)dz, dz_ld,
+    return launch_pdl(k7_act_backward<T, Z, VEC>, dim3(strips, lines), dim3(32, kRowWarps), stream, (const T*)dy, dy_ld, z, act, (T*)dz, dz_ld, (T*)db,
                       db ? partial : (float*)nullptr, rows, cols);
   };
   auto fits = [&](int vec) {
@@ -477,7 +480,7 @@ int act_backward(const void* dy, long long dy_ld, Source z, int act, void* dz, l
   else err = go(std::integral_constant<int, 1>{});
   gtk_count_launch(1);
   if (err != cudaSuccess) return GTK_ERR_CUDA;
-  if (!db) return GTK_OK;
+  if (!db || lines == 1) return GTK_OK;
   err = launch_col_finish<T>(partial, (int)lines, cols, cols, (T*)db, (T*)nullptr, stream);
   gtk_count_launch(1);
   return err == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;

@@ -84,6 +84,7 @@ struct GemmEpilogue {
   void* h;                // slope: act(z') is stored here
   long long h_ld;
   float* sums;            // slope: [rows / 32, rounded up][n], sums of dz' over 32 rows each
+  void* db;               // with up to 32 rows, a single line, the sums themselves
   const unsigned int* a_most;   // operands of two f16 pieces: the largest magnitudes (bits) of A's m and B's n, from
   const unsigned int* b_most;   // which their scales follow
 };
@@ -501,7 +502,10 @@ __device__ __forceinline__ void finish_slope(float (&v)[32], const GemmEpilogue&
     }
     const float sum = transpose_sum(v);
     const int col = p.col0 + (int)lane_id();
-    if (col < p.n) e.sums[(long long)(p.row0 >> 5) * p.n + col] = sum;
+    if (col < p.n) {
+      if (p.m <= 32) ((T*)e.db)[col] = from_f32<T>(sum);
+      else e.sums[(long long)(p.row0 >> 5) * p.n + col] = sum;
+    }
   }
 }
 
@@ -977,7 +981,7 @@ extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long lo
   s.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)s.a_mn << 15) | ((uint32_t)s.b_mn << 16) | ((uint32_t)(s.bn >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
   CUtensorMap am, bm;
   if (!encode(&am, oa, half, m, k, kRows) || !encode(&bm, ob, half, n, k, s.bn / 2)) return GTK_ERR_CUDA;
-  const GemmEpilogue ep{out, out_ld, bias, add, add_ld, act, z, z_ld, q, q_ld, e8, e_ld, h, h_ld, sums, a_pieces == 2 ? a_most : nullptr, b_most};
+  const GemmEpilogue ep{out, out_ld, bias, add, add_ld, act, z, z_ld, q, q_ld, e8, e_ld, h, h_ld, sums, db, a_pieces == 2 ? a_most : nullptr, b_most};
   const int tiles = s.tiles_m * s.tiles_n, pairs = info->sms / 2;
   const int grid = 2 * (s.splits > 1 ? tiles * s.splits : tiles < pairs ? tiles : pairs);
   const size_t shared = (size_t)stage_bytes * s.stages + fixed;
@@ -991,8 +995,8 @@ extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long lo
   }
   gtk_count_launch(1);
   if (err != cudaSuccess) return GTK_ERR_CUDA;
-  if (!db) return GTK_OK;
   const int lines = (s.m + 31) / 32;
+  if (!db || lines == 1) return GTK_OK;
   switch (type) {
     case kF32: err = launch_col_finish<float>(sums, lines, n, n, (float*)db, (float*)nullptr, stream); break;
     case kF16: err = launch_col_finish<__half>(sums, lines, n, n, (__half*)db, (__half*)nullptr, stream); break;

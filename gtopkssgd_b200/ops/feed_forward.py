@@ -78,11 +78,11 @@ def feed_forward_backward(dy: torch.Tensor, kept: FeedForwardKept, norm_weight: 
     mean, rstd = mean.contiguous(), rstd.contiguous()
     pairs = pairs_for(dy.dtype, True, rows, hidden, dim)
     # dz = (dy W2) act'(z) and h = act(z) again, both in the product's epilogue
-    dz, h, db1 = new((rows, hidden)), new((rows, hidden)), new(hidden)
+    dz, h, db1 = new(rows, hidden), new(rows, hidden), new(hidden)
     go, w2o = operands(pairs, (g, 1), (matrix(w2), 0))
     product(rows, hidden, dim, go, False, w2o, True, dz, stream, activation=code, slope=True, z=z, h=h, db=db1)
     del w2o
-    dw2 = new((dim, hidden))
+    dw2 = new(dim, hidden)
     if pairs:
         go, ho = operands(True, (g, 0), (h, 0))
     else:

@@ -28,19 +28,20 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
         raise ValueError("layer_norm: the last axis is empty")
     weight = parameter(x, "weight", weight, cols)
     bias = parameter(x, "bias", bias, cols)
-    lead = x.shape[:-1]
     if not m.is_cuda:
         y, mean, rstd = oracle.norm_forward(m, weight, bias, eps)
-        return y.view(x.shape), mean.view(lead), rstd.view(lead)
-    y = x.new_empty(x.shape)
-    mean = x.new_empty(lead, dtype=_FLOAT)
+        return y.view(x.shape), mean.view(x.shape[:-1]), rstd.view(x.shape[:-1])
+    y = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+    mean = x.new_empty(rows, dtype=_FLOAT)
     rstd = torch.empty_like(mean)
     if rows:
         err = _lib.calls().gtk_k6_norm_forward(code, m.data_ptr(), ld(m), _ptr(weight), _ptr(bias), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
                                                rows, cols, eps, stream_of(m))
         if err:
             _lib.check(err, "gtk_k6_norm_forward")
-    return y, mean, rstd
+    if x.dim() == 2:
+        return y, mean, rstd
+    return y, mean.view(x.shape[:-1]), rstd.view(x.shape[:-1])
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -67,12 +68,12 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
         return (dx.view(x.shape), dw, db) if want_parameters else (dx.view(x.shape), None, None)
     if mean.dtype is not _FLOAT or rstd.dtype is not _FLOAT:
         raise TypeError("mean and rstd are float32")
-    dx = x.new_empty(x.shape)
+    dx = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
     dw = db = partial = None
     if want_parameters:
         dw = x.new_empty(cols)
         db = torch.empty_like(dw)
-        partial = x.new_empty((min(lines("gtk_k6_norm_lines"), rows), 2 * cols), dtype=_FLOAT)
+        partial = x.new_empty(min(lines("gtk_k6_norm_lines"), rows), 2 * cols, dtype=_FLOAT)
     if rows == 0:
         if want_parameters:
             dw.zero_()

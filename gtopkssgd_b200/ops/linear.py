@@ -114,7 +114,7 @@ def normed(src, mean, rstd, weight, bias, pairs: bool):
     rows, cols = m.shape
     split = src.dtype is _FLOAT and not pairs
     pieces, pitch = (3, (cols + 7) & ~7) if split else (1, cols if pairs else (cols + 7) & ~7)
-    out = m.new_empty((pieces, rows, pitch), dtype=torch.bfloat16 if split else src.dtype)
+    out = m.new_empty(pieces, rows, pitch, dtype=torch.bfloat16 if split else src.dtype)
     err = _lib.calls().gtk_k7_stage(TYPES[src.dtype], m.data_ptr(), ld(m), src.e.data_ptr() if codes else None, ld(src.e) if codes else 0,
                                     mean.data_ptr(), rstd.data_ptr(), _ptr(weight), _ptr(bias), 0, 3 if split else 0, out.data_ptr(), pitch,
                                     rows * pitch, rows, cols, pitch, stream_of(m))
@@ -138,7 +138,7 @@ def product(m: int, n: int, k: int, a: Operand, a_mn: bool, b: Operand, b_mn: bo
         qld = eld = 0
         zp, zld = z.data_ptr(), ld(z)
     if db is not None:
-        sums = out.new_empty((-(-m // 32), n), dtype=_FLOAT)
+        sums = out.new_empty(-(-m // 32), n, dtype=_FLOAT)
     err = _lib.calls().gtk_k8_gemm(TYPES[out.dtype], out.dtype is torch.float16 or a.pieces == 2, m, n, k, a.at, a.ld, a.pieces, a.stride, a_mn,
                                    a.most or None, b.at, b.ld, b.pieces, b.stride, b_mn, b.most or None, out.data_ptr(), n, _ptr(bias), _ptr(add), 0 if add is None else ld(add), activation, slope, zp,
                                    zld, q, qld, e, eld, _ptr(h), n, _ptr(sums), _ptr(db), stream)
@@ -149,7 +149,8 @@ def product(m: int, n: int, k: int, a: Operand, a_mn: bool, b: Operand, b_mn: bo
 def _check(x, weight, what):
     if weight.dim() != 2:
         raise ValueError("%s: weight is a matrix [outer, inner]" % what)
-    if weight.size(1) == 0 or x.shape[-1] != weight.size(1):
+    inner = weight.size(1)
+    if inner == 0 or x.shape[-1] != inner:
         raise ValueError("%s: the input's last axis has %d entries, weight is %s" % (what, x.shape[-1], tuple(weight.shape)))
 
 
@@ -176,14 +177,14 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
         y, z = oracle.linear_forward(m, weight, bias, activation, residual)
         z = None if not keep else Activation8(*oracle.keep8(z), x.dtype) if bits else z.to(x.dtype)
         return y.view(shape), z
-    y = x.new_empty(shape)
+    y = x.new_empty(rows, outer)
     z = None
     if keep:
-        z = Activation8.empty(x, rows, outer, (rows, outer)) if bits else x.new_empty((rows, outer))
+        z = Activation8.empty(x, rows, outer, (rows, outer)) if bits else x.new_empty(rows, outer)
     if rows and outer:
         a, b = operands(pairs_for(x.dtype, False, rows, outer, inner), (m, 1), (matrix(weight), 1))
         product(rows, outer, inner, a, False, b, False, y, stream_of(m), bias, residual, code, z=z)
-    return y, z
+    return y if x.dim() == 2 else y.view(shape), z
 
 
 def _gradients(dz: torch.Tensor, x, weight: torch.Tensor, need_dx: bool, need_dw: bool):
@@ -204,10 +205,10 @@ def _gradients(dz: torch.Tensor, x, weight: torch.Tensor, need_dx: bool, need_dw
         specs.append((x, 0))
     made = operands(pairs, *specs)
     if need_dx:
-        dx = dz.new_empty((rows, inner))
+        dx = dz.new_empty(rows, inner)
         product(rows, inner, outer, made[0], False, made[1], True, dx, stream)
     if need_dw:
-        dw = dz.new_empty((outer, inner))
+        dw = dz.new_empty(outer, inner)
         a, b = (made[-2], made[-1]) if pairs else (made[0], x if type(x) is Operand else made[-1])
         product(outer, inner, rows, a, True, b, True, dw, stream)
     return dx, dw
