@@ -211,6 +211,18 @@ __device__ __forceinline__ int block8_code(float x, uint32_t byte) {
   return byte < kBlock8Last ? q : byte == kBlock8NaN ? 0 : max(-63, min(63, q));
 }
 
+// ---- f32 as three bf16 pieces ---------------------------------------------------------------------------------------
+// Three bf16 pieces whose sum is v to 24 bits: each is the nearest to what the ones before left.  The first is cut
+// instead of rounded where rounding would overflow; a NaN or an infinity is all in the first.
+__device__ __forceinline__ void split3(float v, __nv_bfloat16 (&p)[3]) {
+  p[0] = __float2bfloat16_rn(v);
+  if (isinf(__bfloat162float(p[0])) && !isinf(v)) p[0] = __float2bfloat16_rz(v);
+  float left = v - __bfloat162float(p[0]);
+  if (!(fabsf(v) <= 3.402823466e38f)) left = 0.f;
+  p[1] = __float2bfloat16_rn(left);
+  p[2] = __float2bfloat16_rn(left - __bfloat162float(p[1]));
+}
+
 // ---- f32 as two f16 pieces -----------------------------------------------------------------------------------------
 // The power of two by which values whose largest magnitude has these bits are scaled: it then lies in [2^14, 2^15).
 // Values down to 2^-17 of the largest keep 22 bits, smaller ones are off by 2^-40 of it at most.

@@ -27,23 +27,41 @@ __global__ void __launch_bounds__(256) k7_keep(const T* x, long long x_ld, signe
     const long long row = first + i;
     if (row >= rows) break;   // the whole warp
     float v[VEC];
-    uint32_t most = 0;
     if (c < cols) {
       load_f32<T, VEC>(x + row * x_ld + c, v);
     } else {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) v[j] = 0.f;
     }
+    float largest = fabsf(v[0]);
+    if constexpr (VEC > 1) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+      for (int j = 0; j < VEC; j += 2) largest = max_abs(largest, v[j], v[j + 1]);
+    }
+    uint32_t most = __float_as_uint(largest);
 #pragma unroll
     for (int o = kBlock8 / VEC / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     const uint32_t byte = block8_byte(most);
     if (c < padded) {
-      Vec<signed char, VEC> codes;
+      if constexpr (VEC % 4 == 0) {
+        Vec<uint32_t, VEC / 4> codes;
+        if (byte < kBlock8Last) {
+          const float inverse = block8_inverse(byte);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) codes.v[j] = (signed char)block8_code(v[j], byte);
-      *reinterpret_cast<Vec<signed char, VEC>*>(q + row * q_ld + c) = codes;
+          for (int j = 0; j < VEC / 4; ++j) codes.v[j] = block8_codes(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3], inverse);
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC / 4; ++j) {
+            codes.v[j] = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) codes.v[j] |= ((uint32_t)block8_code(v[4 * j + k], byte) & 255u) << (8 * k);
+          }
+        }
+        *reinterpret_cast<Vec<uint32_t, VEC / 4>*>(q + row * q_ld + c) = codes;
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) q[row * q_ld + c + j] = (signed char)block8_code(v[j], byte);
+      }
       if (c % kBlock8 == 0) e[row * e_ld + c / kBlock8] = (unsigned char)byte;
     }
   }
@@ -85,17 +103,6 @@ struct Apply {
   const G* b;
   int act;
 };
-
-// Three bf16 pieces whose sum is v to 24 bits: each is the nearest to what the ones before left.  The first is cut
-// instead of rounded where rounding would overflow; a NaN or an infinity is all in the first.
-__device__ __forceinline__ void split3(float v, __nv_bfloat16 (&p)[3]) {
-  p[0] = __float2bfloat16_rn(v);
-  if (isinf(__bfloat162float(p[0])) && !isinf(v)) p[0] = __float2bfloat16_rz(v);
-  float left = v - __bfloat162float(p[0]);
-  if (!(fabsf(v) <= 3.402823466e38f)) left = 0.f;
-  p[1] = __float2bfloat16_rn(left);
-  p[2] = __float2bfloat16_rn(left - __bfloat162float(p[1]));
-}
 
 // out: `pieces` matrices of rows x out_ld, piece_stride elements apart; columns cols .. pitch - 1 are written as zeros
 // where the pitch is an operand's (a multiple of VEC).

@@ -73,7 +73,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     if want_parameters:
         dw = x.new_empty(cols)
         db = torch.empty_like(dw)
-        partial = x.new_empty(min(lines("gtk_k6_norm_lines"), rows), 2 * cols, dtype=_FLOAT)
+        partial = x.new_empty(min(lines("gtk_k6_norm_lines"), max(rows, 2)), 2 * cols, dtype=_FLOAT)
     if rows == 0:
         if want_parameters:
             dw.zero_()

@@ -1,4 +1,4 @@
-"""Linear layer with bias, activation and residual in the product's epilogue (K8).
+"""Linear layer with bias, activation and residual in the product's epilogue (K8; K9 for few rows).
 
 ``linear`` is the operator under autograd; ``linear_forward`` and
 ``linear_backward`` are its two directions.  y = act(x W^T + bias) + residual, x
@@ -17,6 +17,10 @@ from . import layers_oracle as oracle
 from . import lib as _lib
 from .activation8 import TYPES, Activation8, act_of, bits_of, colsum, ld, matrix, parameter, same, shaped, stream_of, type_of
 from .select import _FLOAT, _ptr
+
+# Rows up to which K9 takes a forward pass, us on the device by K9 and by K8, whose operands have to be made first: 1500 x 6000
+# in bf16 1, 8, 20 and 32 rows 7, 8, 12 and 14 against 22, in f32 13, 13, 28 and 30 against 48; and a launch less.
+FEW_ROWS = {torch.float32: 32, torch.float16: 32, torch.bfloat16: 32}
 
 Kept = Union[None, torch.Tensor, Activation8]
 
@@ -181,7 +185,22 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
     z = None
     if keep:
         z = Activation8.empty(x, rows, outer, (rows, outer)) if bits else x.new_empty(rows, outer)
-    if rows and outer:
+    if rows == 0 or outer == 0:
+        return y if x.dim() == 2 else y.view(shape), z
+    if rows <= FEW_ROWS[x.dtype]:   # K9 reads x and W where they are
+        w = matrix(weight)
+        zp = q = e = None
+        qld = eld = 0
+        if z is not None:
+            if bits:
+                q, qld, e, eld = z.q.data_ptr(), z.e.size(1) * 32, z.e.data_ptr(), z.e.size(1)
+            else:
+                zp = z.data_ptr()
+        err = _lib.calls().gtk_k9_few_rows(TYPES[x.dtype], m.data_ptr(), ld(m), w.data_ptr(), ld(w), rows, outer, inner, y.data_ptr(), _ptr(bias),
+                                           _ptr(residual), 0 if residual is None else ld(residual), code, zp, q, qld, e, eld, stream_of(m))
+        if err:
+            _lib.check(err, "gtk_k9_few_rows")
+    else:
         a, b = operands(pairs_for(x.dtype, False, rows, outer, inner), (m, 1), (matrix(weight), 1))
         product(rows, outer, inner, a, False, b, False, y, stream_of(m), bias, residual, code, z=z)
     return y if x.dim() == 2 else y.view(shape), z

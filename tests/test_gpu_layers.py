@@ -80,7 +80,7 @@ def _check_norm(x, w, b, dy, add=None, eps=1e-5):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 2), (2, 33), (3, 1000), (20, 1500), (7, 1021), (300, 256), (5, 4096), (700, 1500), (6, 8192), (3, 8200),
-                                       (4, 12000), (2, 16384), (3, 20001)])
+                                       (4, 12000), (2, 16384), (3, 20001), (1, 9000), (1, 16384), (1, 30000), (8, 1500), (33, 64)])
 def test_layer_norm(dtype, rows, cols):
     x = _randn(rows, cols, dtype=dtype) * _randn(cols, dtype=dtype).abs() + _randn(cols, dtype=dtype)
     _check_norm(x, _randn(cols, dtype=dtype, seed=1), _randn(cols, dtype=dtype, seed=2), _randn(rows, cols, dtype=dtype, seed=3),
@@ -269,9 +269,10 @@ def test_linear_not_finite_stays_in_its_row(dtype):
     _, z = linear_forward(x, w, None, "gelu", keep=True, bits=8)
     assert z.restore()[150].isnan().all() and z.restore()[good].isfinite().all()
     # rows past the end are not read as anything but zero: the same product in a larger buffer of NaN
-    room = torch.full((400, 96), math.nan, device=DEV, dtype=dtype)
-    room[:3] = x[:3]
-    assert torch.equal(linear_forward(room[:3], w)[0], y[:3])
+    for rows in (3, 100):
+        room = torch.full((400, 96), math.nan, device=DEV, dtype=dtype)
+        room[:rows] = x[10:10 + rows]
+        assert torch.equal(linear_forward(room[:rows], w)[0], linear_forward(x[10:10 + rows].clone(), w)[0])
     room = torch.full((200, 104), math.nan, device=DEV, dtype=dtype)
     room[:, :96] = torch.nan_to_num(x, 0, 0, 0)
     assert torch.equal(linear_forward(room[:, :96], w)[0][good], y[good])
@@ -478,25 +479,39 @@ def test_refusals_on_the_gpu():
         layer_norm_backward(x, x, mean.double(), rstd)
 
 
-def test_language_model_with_blocks_in_a_sparse_training_step():
-    """The PTB model with a block behind the LSTM, gTop-k: eager, 8 bits and bf16 inside; losses fall."""
+def test_language_model_with_blocks_in_a_sparse_training_step(monkeypatch):
+    """The PTB model with a block behind the LSTM, gTop-k: the losses follow those with the block in library functions
+    (f32: to 1e-3 over ten steps; 8 bits, and bf16 inside: to 2e-2), and fall."""
+    from gtopkssgd_b200.models import feed_forward as module
     from gtopkssgd_b200.models import lstm
     from gtopkssgd_b200.parallel.compression import compressors
     from gtopkssgd_b200.parallel.distributed_optimizer import DistributedOptimizer
-    for bits, dtype in ((0, None), (8, None), (8, torch.bfloat16)):
+
+    def library(x, g, b, w1, b1, w2, b2, activation, eps, bits):
+        return x + F.linear(F.gelu(F.linear(F.layer_norm(x, (x.size(-1),), g, b, eps), w1, b1)), w2, b2)
+
+    def losses(bits, dtype):
         torch.manual_seed(0)
         net = lstm(vocab_size=50, embedding_dim=100, num_steps=5, batch_size=4, ff_layers=1, ff_dim=400, ff_bits=bits, ff_dtype=dtype).to(DEV)
-        opt = DistributedOptimizer(torch.optim.SGD(net.parameters(), lr=0.5), net.named_parameters(), compression=compressors["gtopk"], is_sparse=True,
+        opt = DistributedOptimizer(torch.optim.SGD(net.parameters(), lr=0.05), net.named_parameters(), compression=compressors["gtopk"], is_sparse=True,
                                    density=0.05)
         tokens = torch.randint(0, 50, (6, 4), device=DEV)
-        losses = []
+        got = []
         for _ in range(60):
             opt.zero_grad()
             logits, _ = net(tokens[:-1], net.init_hidden())
             loss = F.cross_entropy(logits.view(-1, 50), tokens[1:].reshape(-1))
             loss.backward()
             opt.step()
-            losses.append(float(loss.detach()))
+            got.append(float(loss.detach()))
         opt.check_status()
         opt.stop()
-        assert losses[-1] < 0.9 * losses[0] and status() == 0
+        return got
+
+    cases = ((0, None, 1e-3), (8, None, 2e-2), (8, torch.bfloat16, 2e-2))
+    got = [losses(bits, dtype) for bits, dtype, _ in cases]
+    assert status() == 0
+    monkeypatch.setattr(module, "feed_forward_block", library)
+    want = losses(0, None)
+    for g, (_, _, off) in zip(got, cases):
+        assert all(abs(a - b) <= off * b for a, b in zip(g[:10], want)) and g[-1] < 0.97 * g[0]
