@@ -99,62 +99,158 @@ __device__ __forceinline__ float rcp_fast(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 1 / (1 + e^-z)
-__device__ __forceinline__ float sigmoid(float z) { return rcp_fast(1.f + exp2_fast(-kLog2E * z)); }
+
+// Two values that are multiplied and added by one instruction; what follows is written for these and for single ones.
+struct Two {
+  unsigned long long u;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.u) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void parts(Two x, float* a, float* b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(x.u)); }
+__device__ __forceinline__ Two vmul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+  return r;
+}
+__device__ __forceinline__ Two vfma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.u) : "l"(a.u), "l"(b.u), "l"(c.u));
+  return r;
+}
+__device__ __forceinline__ float vmul(float a, float b) { return a * b; }
+__device__ __forceinline__ float vfma(float a, float b, float c) { return fmaf(a, b, c); }
+template <typename V>
+__device__ __forceinline__ V vset(float c) {
+  if constexpr (sizeof(V) == 8) return two(c, c);
+  else return c;
+}
+template <typename F>
+__device__ __forceinline__ float each(float x, F&& f) { return f(x); }
+template <typename F>
+__device__ __forceinline__ Two each(Two x, F&& f) {
+  float a, b;
+  parts(x, &a, &b);
+  return two(f(a), f(b));
+}
+template <typename V>
+__device__ __forceinline__ V vexp2(V x) { return each(x, [](float v) { return exp2_fast(v); }); }
+template <typename V>
+__device__ __forceinline__ V vrcp(V x) { return each(x, [](float v) { return rcp_fast(v); }); }
+template <typename V>
+__device__ __forceinline__ V vabs(V x) { return each(x, [](float v) { return fabsf(v); }); }
+__device__ __forceinline__ float vwhere_negative(float z, float a, float b) { return z < 0.f ? a : b; }
+__device__ __forceinline__ Two vwhere_negative(Two z, Two a, Two b) {
+  float z0, z1, a0, a1, b0, b1;
+  parts(z, &z0, &z1);
+  parts(a, &a0, &a1);
+  parts(b, &b0, &b1);
+  return two(z0 < 0.f ? a0 : b0, z1 < 0.f ? a1 : b1);
+}
+
+// 1 / (1 + e^-(c z))
+template <typename V>
+__device__ __forceinline__ V sigmoid(V z, float c) {
+  const V e = vexp2(vmul(z, vset<V>(-kLog2E * c)));
+  return vrcp(vfma(e, vset<V>(1.f), vset<V>(1.f)));
+}
 
 // The normal distribution's Phi(z), and e^(-z^2 / 2), which it contains: Phi(-|z|) = e^(-z^2 / 2) t (b1 + t (b2 + ...)),
 // t = 1 / (1 + p |z| / sqrt 2), Abramowitz and Stegun 7.1.26 for the error function with its coefficients halved; 7.5e-8
 // off at most.
-__device__ __forceinline__ float normal_cdf(float z, float* bell) {
-  const float t = rcp_fast(fmaf(fabsf(z), 0.3275911f * 0.70710678118654752f, 1.f));
-  const float g = exp2_fast(z * z * (-0.5f * kLog2E));
-  float p = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
-  p = fmaf(t, p, 0.5f * 1.421413741f);
-  p = fmaf(t, p, 0.5f * -0.284496736f);
-  p = fmaf(t, p, 0.5f * 0.254829592f);
-  const float tail = p * t * g;
+template <typename V>
+__device__ __forceinline__ V normal_cdf(V z, V* bell) {
+  const V t = vrcp(vfma(vabs(z), vset<V>(0.3275911f * 0.70710678118654752f), vset<V>(1.f)));
+  const V g = vexp2(vmul(vmul(z, z), vset<V>(-0.5f * kLog2E)));
+  V p = vfma(t, vset<V>(0.5f * 1.061405429f), vset<V>(0.5f * -1.453152027f));
+  p = vfma(t, p, vset<V>(0.5f * 1.421413741f));
+  p = vfma(t, p, vset<V>(0.5f * -0.284496736f));
+  p = vfma(t, p, vset<V>(0.5f * 0.254829592f));
+  const V tail = vmul(vmul(p, t), g);
   *bell = g;
-  return z < 0.f ? tail : 1.f - tail;
+  return vwhere_negative(z, tail, vfma(tail, vset<V>(-1.f), vset<V>(1.f)));
 }
 
-template <int ACT>
-__device__ __forceinline__ float act_value(float z) {
-  if constexpr (ACT == kActRelu) return z < 0.f ? 0.f : z;  // a NaN stays one
+// 2 sqrt(2 / pi) (z + c z^3): (1 + tanh u) / 2 = 1 / (1 + e^-2u)
+template <typename V>
+__device__ __forceinline__ V tanh_argument(V z) {
+  return vmul(z, vfma(vmul(z, z), vset<V>(2.f * kSqrt2OverPi * kGeluCubic), vset<V>(2.f * kSqrt2OverPi)));
+}
+
+template <int ACT, typename V>
+__device__ __forceinline__ V act_value(V z) {
+  if constexpr (ACT == kActRelu) return vwhere_negative(z, vset<V>(0.f), z);  // a NaN stays one
   if constexpr (ACT == kActGelu) {
-    float bell;
-    return z * normal_cdf(z, &bell);
+    V bell;
+    return vmul(z, normal_cdf(z, &bell));
   }
-  // (1 + tanh u) / 2 = 1 / (1 + e^-2u)
-  if constexpr (ACT == kActGeluTanh) return z * sigmoid(2.f * kSqrt2OverPi * (z + kGeluCubic * z * z * z));
-  if constexpr (ACT == kActSilu) return z * sigmoid(z);
+  if constexpr (ACT == kActGeluTanh) return vmul(z, sigmoid(tanh_argument(z), 1.f));
+  if constexpr (ACT == kActSilu) return vmul(z, sigmoid(z, 1.f));
   return z;
 }
 
 // d act(z) / dz, and act(z) itself, which shares its work.
-template <int ACT>
-__device__ __forceinline__ float act_slope(float z, float* value) {
+template <int ACT, typename V>
+__device__ __forceinline__ V act_slope(V z, V* value) {
   if constexpr (ACT == kActRelu) {
-    *value = z < 0.f ? 0.f : z;
-    return z > 0.f ? 1.f : 0.f;
+    *value = vwhere_negative(z, vset<V>(0.f), z);
+    return each(z, [](float v) { return v > 0.f ? 1.f : 0.f; });
   }
   if constexpr (ACT == kActGelu) {
-    float bell;
-    const float cdf = normal_cdf(z, &bell);
-    *value = z * cdf;
-    return fmaf(z * 0.39894228040143268f, bell, cdf);   // 1 / sqrt(2 pi)
+    V bell;
+    const V cdf = normal_cdf(z, &bell);
+    *value = vmul(z, cdf);
+    return vfma(vmul(z, vset<V>(0.39894228040143268f)), bell, cdf);   // 1 / sqrt(2 pi)
   }
   if constexpr (ACT == kActGeluTanh) {
-    const float s = sigmoid(2.f * kSqrt2OverPi * (z + kGeluCubic * z * z * z));
-    *value = z * s;
-    return s + z * s * (1.f - s) * (2.f * kSqrt2OverPi) * (1.f + 3.f * kGeluCubic * z * z);
+    const V s = sigmoid(tanh_argument(z), 1.f);
+    const V h = vmul(z, s);
+    *value = h;
+    // s + h (1 - s) du, du = 2 sqrt(2 / pi) (1 + 3 c z^2)
+    const V du = vfma(vmul(z, z), vset<V>(6.f * kSqrt2OverPi * kGeluCubic), vset<V>(2.f * kSqrt2OverPi));
+    return vfma(vmul(h, vfma(s, vset<V>(-1.f), vset<V>(1.f))), du, s);
   }
   if constexpr (ACT == kActSilu) {
-    const float s = sigmoid(z);
-    *value = z * s;
-    return s * (1.f + z * (1.f - s));
+    const V s = sigmoid(z, 1.f);
+    const V h = vmul(z, s);
+    *value = h;
+    return vfma(h, vfma(s, vset<V>(-1.f), vset<V>(1.f)), s);   // s (1 + z (1 - s))
   }
   *value = z;
-  return 1.f;
+  return vset<V>(1.f);
+}
+
+// N values in place; and slopes times what is in g, z becoming the values.
+template <int ACT, int N>
+__device__ __forceinline__ void act_values(float (&z)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) parts(act_value<ACT>(two(z[i], z[i + 1])), &z[i], &z[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = act_value<ACT>(z[i]);
+  }
+}
+template <int ACT, int N>
+__device__ __forceinline__ void act_slopes(float (&g)[N], float (&z)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      Two value;
+      const Two slope = act_slope<ACT>(two(z[i], z[i + 1]), &value);
+      parts(vmul(two(g[i], g[i + 1]), slope), &g[i], &g[i + 1]);
+      parts(value, &z[i], &z[i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float value;
+      g[i] *= act_slope<ACT>(z[i], &value);
+      z[i] = value;
+    }
+  }
 }
 
 // Calls f with the activation's number as a type.
@@ -205,6 +301,14 @@ __device__ __forceinline__ uint32_t block8_codes(float a, float b, float c, floa
   const uint32_t ia = __float_as_uint(fmaf(a, inverse, kMagic)), ib = __float_as_uint(fmaf(b, inverse, kMagic));
   const uint32_t ic = __float_as_uint(fmaf(c, inverse, kMagic)), id = __float_as_uint(fmaf(d, inverse, kMagic));
   return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
+}
+// What the four codes of a word stand for: byte + 128 becomes the low byte of 2^23, from which one exact multiply-add
+// takes 2^23 + 128 and scales.
+__device__ __forceinline__ void block8_values(uint32_t codes, float scale, float* v) {
+  const uint32_t u = codes ^ 0x80808080u;
+  const float back = -8388736.f * scale;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = fmaf(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + i)), scale, back);
 }
 __device__ __forceinline__ int block8_code(float x, uint32_t byte) {
   const int q = __float2int_rn(x * block8_inverse(byte));

@@ -77,10 +77,16 @@ struct Source {
 template <typename S, int VEC>
 __device__ __forceinline__ void load_source(const Source& s, long long row, int c, float (&v)[VEC]) {
   if constexpr (sizeof(S) == 1) {
-    const Vec<signed char, VEC> q = *reinterpret_cast<const Vec<signed char, VEC>*>((const signed char*)s.p + row * s.ld + c);
     const float scale = block8_scale(s.e[row * s.e_ld + c / kBlock8]);
+    const signed char* p = (const signed char*)s.p + row * s.ld + c;
+    if constexpr (VEC % 4 == 0) {
+      const Vec<uint32_t, VEC / 4> w = *reinterpret_cast<const Vec<uint32_t, VEC / 4>*>(p);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = (float)q.v[j] * scale;
+      for (int j = 0; j < VEC / 4; ++j) block8_values(w.v[j], scale, v + 4 * j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = (float)p[j] * scale;
+    }
   } else {
     load_f32<S, VEC>((const S*)s.p + row * s.ld + c, v);
   }
@@ -131,8 +137,7 @@ __global__ void __launch_bounds__(256) k7_stage(Source src, Apply<G> f, O* out, 
       }
       if (f.act != kActNone)
         with_act(f.act, [&](auto A) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) v[j] = act_value<decltype(A)::value>(v[j]);
+          act_values<decltype(A)::value, VEC>(v);
         });
     } else {
 #pragma unroll
@@ -357,10 +362,22 @@ __global__ void __launch_bounds__(256) k7_pack(const __grid_constant__ PackList 
   }
 }
 
+template <int BYTES>
+__device__ __forceinline__ void async_copy(void* to, const void* from) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (BYTES >= 16) {
+#pragma unroll
+    for (int i = 0; i < BYTES; i += 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + i), "l"(reinterpret_cast<const uint8_t*>(from) + i) : "memory");
+  } else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
+}
+
 // Z: element type of z (signed char: codes).  dz may be null (sums only); partial and db may be null.  With one line of
 // partial sums they are the sums, and are stored as such.
+// One wave of CTAs, four an SM, whose threads each have four rows under way: with a row at a time, loaded to registers,
+// 24 KB an SM were under way and a pass over 16384 x 8192 took 152 us instead of 140.
 template <typename T, typename Z, int VEC>
-__global__ void __launch_bounds__(256) k7_act_backward(const T* dy, long long dy_ld, Source z, int act, T* dz, long long dz_ld, T* db, float* partial,
+__global__ void __launch_bounds__(256, 4) k7_act_backward(const T* dy, long long dy_ld, Source z, int act, T* dz, long long dz_ld, T* db, float* partial,
                                                        long long rows, int cols) {
   __shared__ float joined[kRowWarps][32 * VEC];
   pdl_begin(dy, z.p, z.e);
@@ -368,28 +385,62 @@ __global__ void __launch_bounds__(256) k7_act_backward(const T* dy, long long dy
   float sum[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
-  if (c < cols)
-    for (long long row = (long long)blockIdx.y * kRowWarps + threadIdx.y; row < rows; row += (long long)gridDim.y * kRowWarps) {
+  const long long step = (long long)gridDim.y * kRowWarps, row0 = (long long)blockIdx.y * kRowWarps + threadIdx.y;
+  // Rows to come: each thread's own part in shared memory (vectors of less than 4 bytes, of which there are no
+  // asynchronous copies, are loaded when they are used)
+  constexpr int kBytes = VEC * (int)sizeof(T), kBytesZ = VEC * (int)sizeof(Z);
+  constexpr bool kAsync = kBytes >= 4 && kBytesZ >= 4;
+  constexpr int kActDepth = VEC == 16 ? 2 : 4;   // rows of a thread under way
+  __shared__ alignas(16) uint8_t ring[kAsync ? kActDepth : 1][256][kBytes], ring_z[kAsync ? kActDepth : 1][256][kBytesZ];
+  const int t = (int)(threadIdx.y * 32 + threadIdx.x);
+  auto copy = [&](int slot, long long row) {
+    if constexpr (kAsync) {
+      if (c < cols && row < rows) {
+        async_copy<kBytes>(ring[slot][t], dy + row * dy_ld + c);
+        if (act != kActNone) {
+          async_copy<kBytesZ>(ring_z[slot][t], (const Z*)z.p + row * z.ld + c);
+          if (sizeof(Z) == 1) asm volatile("prefetch.global.L2 [%0];" ::"l"(z.e + row * z.e_ld + c / kBlock8) : "memory");
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  if constexpr (kAsync) {
+#pragma unroll
+    for (int i = 0; i < kActDepth; ++i) copy(i, row0 + i * step);
+  }
+  int slot = 0;
+  for (long long row = row0; row < rows; row += step) {
+    if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(kActDepth - 1) : "memory");
+    if (c < cols) {
       float g[VEC];
-      load_f32<T, VEC>(dy + row * dy_ld + c, g);
+      if constexpr (kAsync) to_f32<T, VEC>(*reinterpret_cast<const Vec<T, VEC>*>(ring[slot][t]), g);
+      else load_f32<T, VEC>(dy + row * dy_ld + c, g);
       if (act != kActNone) {
         float zv[VEC];
-        load_source<Z, VEC>(z, row, c, zv);
-        with_act(act, [&](auto A) {
-          float value;
+        if constexpr (!kAsync) {
+          load_source<Z, VEC>(z, row, c, zv);
+        } else if constexpr (sizeof(Z) == 1) {
+          const float scale = block8_scale(z.e[row * z.e_ld + c / kBlock8]);
+          const Vec<uint32_t, VEC / 4> q = *reinterpret_cast<const Vec<uint32_t, VEC / 4>*>(ring_z[slot][t]);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) g[j] *= act_slope<decltype(A)::value>(zv[j], &value);
-        });
+          for (int j = 0; j < VEC / 4; ++j) block8_values(q.v[j], scale, zv + 4 * j);
+        } else {
+          to_f32<Z, VEC>(*reinterpret_cast<const Vec<Z, VEC>*>(ring_z[slot][t]), zv);
+        }
+        with_act(act, [&](auto A) { act_slopes<decltype(A)::value, VEC>(g, zv); });
       }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) sum[j] += g[j];
       if (dz) store_f32<T, VEC>(dz + row * dz_ld + c, g);
     }
+    copy(slot, row + kActDepth * step);   // what was there has been used
+    slot = slot + 1 == kActDepth ? 0 : slot + 1;
+  }
   if (!partial) return;
 #pragma unroll
   for (int j = 0; j < VEC; ++j) joined[threadIdx.y][threadIdx.x * VEC + j] = sum[j];
   __syncthreads();
-  const int t = (int)(threadIdx.y * 32 + threadIdx.x);
   for (int i = t; i < 32 * VEC; i += 256) {
     const int col = (int)(blockIdx.x * 32 * VEC) + i;
     if (col >= cols) break;
@@ -451,12 +502,17 @@ int stage(Source src, Apply<G> f, void* out, long long out_ld, long long piece_s
     return err == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;
   };
   // a block's scale is read once per vector, so vectors do not cross blocks (they start at multiples of their length)
-  constexpr int wide = sizeof(S) == 4 || sizeof(O) == 4 ? 4 : 8;
+  constexpr int wide = sizeof(S) == 4 || sizeof(O) == 4 ? 4 : sizeof(S) == 1 ? 16 : 8;   // more elements a thread: fewer addresses
   auto fits = [&](int vec) {
-    return cols % vec == 0 && pitch % vec == 0 && piece_stride % vec == 0 && aligned(src.p, src.ld, sizeof(S), vec) && aligned(out, out_ld, sizeof(O), vec);
+    return cols % vec == 0 && pitch % vec == 0 && piece_stride % vec == 0 && aligned(src.p, src.ld, sizeof(S), vec) && aligned(out, out_ld, sizeof(O), vec < 8 ? vec : 16 / (int)sizeof(O));
   };
   if (fits(wide)) return go(std::integral_constant<int, wide>{});
-  if (wide == 8 && fits(4)) return go(std::integral_constant<int, 4>{});
+  if constexpr (wide == 16) {
+    if (fits(8)) return go(std::integral_constant<int, 8>{});
+  }
+  if constexpr (wide > 4) {
+    if (fits(4)) return go(std::integral_constant<int, 4>{});
+  }
   return go(std::integral_constant<int, 1>{});
 }
 
@@ -467,7 +523,8 @@ int act_backward(const void* dy, long long dy_ld, Source z, int act, void* dz, l
   auto go = [&](auto V) {
     constexpr int VEC = decltype(V)::value;
     const unsigned strips = (unsigned)((cols + 32 * VEC - 1) / (32 * VEC));
-    long long y = (148LL * 8 + strips - 1) / strips;
+    long long y = 148LL * 4 / strips;
+    if (y < 1) y = 1;
     const long long most = (rows + kRowWarps - 1) / kRowWarps;
     if (y > most) y = most;
     if (y > max_lines) y = max_lines;
@@ -477,14 +534,21 @@ int act_backward(const void* dy, long long dy_ld, Source z, int act, void* dz, l
                       db ? partial : (float*)nullptr, rows, cols);
   };
   auto fits = [&](int vec) {
-    return cols % vec == 0 && aligned(dy, dy_ld, sizeof(T), vec) && (act == kActNone || aligned(z.p, z.ld, sizeof(Z), vec)) &&
-           (!dz || aligned(dz, dz_ld, sizeof(T), vec));
+    const int most = vec < 16 / (int)sizeof(T) ? vec : 16 / (int)sizeof(T);   // 16 bytes at a time
+    return cols % vec == 0 && aligned(dy, dy_ld, sizeof(T), most) && (act == kActNone || aligned(z.p, z.ld, sizeof(Z), vec)) &&
+           (!dz || aligned(dz, dz_ld, sizeof(T), most));
   };
-  constexpr int wide = 16 / sizeof(T);
+  constexpr int wide = sizeof(T) == 2 && sizeof(Z) == 1 ? 16 : 16 / sizeof(T);
   cudaError_t err;
-  if (fits(wide)) err = go(std::integral_constant<int, wide>{});
-  else if (wide == 8 && fits(4)) err = go(std::integral_constant<int, 4>{});
-  else err = go(std::integral_constant<int, 1>{});
+  if (fits(wide)) {
+    err = go(std::integral_constant<int, wide>{});
+  } else if (wide > 8 && fits(8)) {
+    err = go(std::integral_constant<int, (wide == 16 ? 8 : 1)>{});
+  } else if (wide > 4 && fits(4)) {
+    err = go(std::integral_constant<int, (wide > 4 ? 4 : 1)>{});
+  } else {
+    err = go(std::integral_constant<int, 1>{});
+  }
   gtk_count_launch(1);
   if (err != cudaSuccess) return GTK_ERR_CUDA;
   if (!db || lines == 1) return GTK_OK;

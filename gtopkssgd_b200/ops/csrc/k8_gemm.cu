@@ -468,8 +468,7 @@ __device__ __forceinline__ void finish_forward(float (&v)[32], float* bias, cons
   if (e.z) write32<T>(e.z, e.z_ld, p, v);
   if (e.act != kActNone)
     with_act(e.act, [&](auto A) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = act_value<decltype(A)::value>(v[i]);
+      act_values<decltype(A)::value, 32>(v);
     });
   if (e.add) {
 #pragma unroll
@@ -486,12 +485,7 @@ __device__ __forceinline__ void finish_slope(float (&v)[32], const GemmEpilogue&
   if (e.q) read_codes(e, p, h);
   else read32<T>(e.z, e.z_ld, p, h);
   with_act(e.act, [&](auto A) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      float value;
-      v[i] *= act_slope<decltype(A)::value>(h[i], &value);
-      h[i] = value;
-    }
+    act_slopes<decltype(A)::value, 32>(v, h);
   });
   write32<T>(e.out, e.out_ld, p, v);
   if (e.h) write32<T>(e.h, e.h_ld, p, h);
