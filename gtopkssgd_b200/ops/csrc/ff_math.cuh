@@ -120,6 +120,12 @@ __device__ __forceinline__ Two vfma(Two a, Two b, Two c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.u) : "l"(a.u), "l"(b.u), "l"(c.u));
   return r;
 }
+__device__ __forceinline__ Two vadd(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+  return r;
+}
+__device__ __forceinline__ float vadd(float a, float b) { return a + b; }
 __device__ __forceinline__ float vmul(float a, float b) { return a * b; }
 __device__ __forceinline__ float vfma(float a, float b, float c) { return fmaf(a, b, c); }
 template <typename V>
@@ -127,6 +133,23 @@ __device__ __forceinline__ V vset(float c) {
   if constexpr (sizeof(V) == 8) return two(c, c);
   else return c;
 }
+__device__ __forceinline__ float vtotal(float x) { return x; }
+__device__ __forceinline__ float vtotal(Two x) {
+  float a, b;
+  parts(x, &a, &b);
+  return a + b;
+}
+// Element, or pair of elements, i of an array, and back.
+template <typename V>
+__device__ __forceinline__ V vget(const float* v, int i) {
+  if constexpr (sizeof(V) == 8) return two(v[2 * i], v[2 * i + 1]);
+  else return v[i];
+}
+__device__ __forceinline__ void vput(float* v, int i, float x) { v[i] = x; }
+__device__ __forceinline__ void vput(float* v, int i, Two x) { parts(x, v + 2 * i, v + 2 * i + 1); }
+template <int N>
+using Wide = std::conditional_t<N % 2 == 0, Two, float>;   // what N elements are computed in
+
 template <typename F>
 __device__ __forceinline__ float each(float x, F&& f) { return f(x); }
 template <typename F>

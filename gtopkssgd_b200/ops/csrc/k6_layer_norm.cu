@@ -116,6 +116,8 @@ constexpr int kRingDepth = 4;   // at most; ring_wait knows these
 // blockDim = (32 * warps, groups).  Dynamic shared memory: `depth` rows of every group.
 template <typename T, int VEC, int NV>
 __global__ void __launch_bounds__(1024) k6_norm_forward(const T* x, const T* w, const T* b, T* y, float* mean, float* rstd, NormShape s) {
+  using V = Wide<VEC>;
+  constexpr int kV = VEC * 4 / (int)sizeof(V);   // of V in a vector
   extern __shared__ uint4 dynamic[];
   __shared__ alignas(16) float scratch[8][2][kNormMaxWarps];
   pdl_begin(x, w, b);
@@ -142,14 +144,15 @@ __global__ void __launch_bounds__(1024) k6_norm_forward(const T* x, const T* w, 
     ring_wait(s.depth - 1);
     if (mine) ring.take(slot, at, threads, s.cols, &raw);
     float v[NV][VEC];
-    float sum[1] = {0.f};
+    V total = vset<V>(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((at + i * threads) * VEC < s.cols) {
         to_f32<T, VEC>(raw.v[i], v[i]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) sum[0] += v[i][j];
+        for (int j = 0; j < kV; ++j) total = vadd(total, vget<V>(v[i], j));
       }
+    float sum[1] = {vtotal(total)};
     group_sum<1>(sum, s.warps, at >> 5, scratch[group][0]);
     if (coming_row < s.rows) ring.copy(slot, coming, at, threads, s.cols);
     ring_commit();
@@ -157,16 +160,19 @@ __global__ void __launch_bounds__(1024) k6_norm_forward(const T* x, const T* w, 
     coming_row += step;
     slot = slot + 1 == s.depth ? 0 : slot + 1;
     const float m = sum[0] * inv;
-    float sq[1] = {0.f};
+    const V minus = vset<V>(-m);
+    total = vset<V>(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((at + i * threads) * VEC < s.cols) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          v[i][j] -= m;
-          sq[0] = fmaf(v[i][j], v[i][j], sq[0]);
+        for (int j = 0; j < kV; ++j) {
+          const V d = vadd(vget<V>(v[i], j), minus);
+          vput(v[i], j, d);
+          total = vfma(d, d, total);
         }
       }
+    float sq[1] = {vtotal(total)};
     group_sum<1>(sq, s.warps, at >> 5, scratch[group][1]);
     const float r = rsqrtf(fmaf(sq[0], inv, s.eps));
     if (mine) {
@@ -187,7 +193,7 @@ __global__ void __launch_bounds__(1024) k6_norm_forward(const T* x, const T* w, 
           if (w) load_f32<T, VEC>(w + c, wv);
           if (b) load_f32<T, VEC>(b + c, bv);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) v[i][j] = fmaf(v[i][j] * r, wv[j], bv[j]);
+          for (int j = 0; j < kV; ++j) vput(v[i], j, vfma(vmul(vget<V>(v[i], j), vset<V>(r)), vget<V>(wv, j), vget<V>(bv, j)));
           store_f32<T, VEC>(yr + c, v[i]);
         }
       }
@@ -237,6 +243,8 @@ __global__ void __launch_bounds__(THREADS)
 k6_norm_backward(const T* dy, const T* x, const float* mean, const float* rstd, const T* w, const T* add, T* dx, T* dw_out, T* db_out, float* partial,
                  NormShape s) {
   constexpr bool kShared = THREADS > 512;
+  using V = Wide<VEC>;
+  constexpr int kV = VEC * 4 / (int)sizeof(V);   // of V in a vector
   extern __shared__ uint4 dynamic[];   // then [groups - 1][2 * cols], or [2 * cols], of floats
   __shared__ alignas(16) float scratch[8][2][2 * kNormMaxWarps];
   pdl_begin(dy, x, mean, rstd, w, add);
@@ -275,7 +283,7 @@ k6_norm_backward(const T* dy, const T* x, const float* mean, const float* rstd, 
     const bool mine = row < s.rows;
     const float r = nr, mr = -nm * nr;
     float xh[NV][VEC], t[NV][VEC];
-    float sums[2] = {0.f, 0.f};
+    V sum_t = vset<V>(0.f), sum_th = vset<V>(0.f);
     {
       RowRaw<T, VEC, NV> rx, rg;
       if constexpr (kShared) {
@@ -306,26 +314,29 @@ k6_norm_backward(const T* dy, const T* x, const float* mean, const float* rstd, 
             to_f32<T, VEC>(rx.v[i], xh[i]);
             to_f32<T, VEC>(rg.v[i], t[i]);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              const float h = fmaf(xh[i][j], r, mr), g = t[i][j];
+            for (int j = 0; j < kV; ++j) {
+              const V h = vfma(vget<V>(xh[i], j), vset<V>(r), vset<V>(mr)), g = vget<V>(t[i], j);
               if constexpr (kShared) {
                 if (partial) {   // this thread's own columns
-                  joined[c + j] += g * h;
-                  joined[s.cols + c + j] += g;
+                  float* own = joined + c;
+                  vput(own, j, vfma(g, h, vget<V>(own, j)));
+                  vput(own + s.cols, j, vadd(vget<V>(own + s.cols, j), g));
                 }
               } else {
-                dw[i][j] = fmaf(g, h, dw[i][j]);
-                db[i][j] += g;
+                vput(dw[i], j, vfma(g, h, vget<V>(dw[i], j)));
+                vput(db[i], j, vadd(vget<V>(db[i], j), g));
               }
-              xh[i][j] = h;
-              t[i][j] = w ? g * wv[j] : g;
-              sums[0] += t[i][j];
-              sums[1] = fmaf(t[i][j], h, sums[1]);
+              const V gw = w ? vmul(g, vget<V>(wv, j)) : g;
+              vput(xh[i], j, h);
+              vput(t[i], j, gw);
+              sum_t = vadd(sum_t, gw);
+              sum_th = vfma(gw, h, sum_th);
             }
           }
         }
       }
     }
+    float sums[2] = {vtotal(sum_t), vtotal(sum_th)};
     row += step;
     if (row < s.rows) {
       nm = mean[row];
@@ -353,9 +364,9 @@ k6_norm_backward(const T* dy, const T* x, const float* mean, const float* rstd, 
           float o[VEC];
           if (add) load_f32<T, VEC>(ar + c, o);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float g = fmaf(t[i][j], r, fmaf(xh[i][j], c2, c1));
-            o[j] = add ? g + o[j] : g;
+          for (int j = 0; j < kV; ++j) {
+            const V g = vfma(vget<V>(t[i], j), vset<V>(r), vfma(vget<V>(xh[i], j), vset<V>(c2), vset<V>(c1)));
+            vput(o, j, add ? vadd(g, vget<V>(o, j)) : g);
           }
           store_f32<T, VEC>(out + c, o);
         }
@@ -455,8 +466,10 @@ __global__ void __launch_bounds__(256) k6_norm_columns_long(const T* dy, const T
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------
-// How a row is spread over a group: `nv` vectors of `vec` elements per thread.  16 elements where there are rows for two
-// groups of every SM and the rows to come can be copied to shared memory, else 8; at most `most` warps; longer rows take another form (nv 0).
+// How a row is spread over a group of `most` warps at most: `nv` vectors of `vec` elements per thread, 8 elements or, where
+// there are rows for two groups of every SM and those to come can be copied to shared memory, 16, so that the work per
+// thread and row is shared by more elements (32 do not fit the registers: 82 us for 72).  Longer rows take another form
+// (nv 0).
 struct NormPlan {
   int vec, nv, warps;
 };
