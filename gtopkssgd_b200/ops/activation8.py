@@ -91,6 +91,13 @@ def ld(m: torch.Tensor) -> int:
     return m.stride(0) if m.size(0) > 1 else m.size(1)
 
 
+def padded_rows(like: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """An uninitialised matrix whose rows lie on 16-byte boundaries, so that a product's kernel reads it where it is."""
+    if like.dtype is _FLOAT or cols % 8 == 0:   # (f32 operands are made anew in any case)
+        return like.new_empty(rows, cols)
+    return like.new_empty(rows, (cols + 7) & ~7)[:, :cols]
+
+
 def stream_of(t: torch.Tensor) -> int:
     """The current stream of the tensor's device, which has to be the current one: launches go there."""
     index = t.get_device()
@@ -99,11 +106,11 @@ def stream_of(t: torch.Tensor) -> int:
     return _raw_stream(index)
 
 
-def colsum(dy: torch.Tensor, activation: int = 0, z=None, want_dz: bool = False, want_sum: bool = True):
+def colsum(dy: torch.Tensor, activation: int = 0, z=None, want_dz: bool = False, want_sum: bool = True, padded: bool = False):
     """(dz, sum of dz over the rows) with dz = dy * act'(z), over CUDA matrices; each None where not wanted.
-    ``activation``: its number."""
+    ``activation``: its number; ``padded``: dz's rows lie on 16-byte boundaries."""
     rows, cols = dy.shape
-    dz = dy.new_empty(rows, cols) if want_dz else None   # (numbers, not a tuple: half the host time)
+    dz = padded_rows(dy, rows, cols) if padded else dy.new_empty(rows, cols) if want_dz else None   # (numbers, not a tuple: half the host time)
     db = dy.new_empty(cols) if want_sum else None
     if rows == 0 or cols == 0:
         if db is not None:
@@ -116,7 +123,8 @@ def colsum(dy: torch.Tensor, activation: int = 0, z=None, want_dz: bool = False,
     else:
         zp, zld, e, eld = z.data_ptr(), ld(z), None, 0
     partial = dy.new_empty(min(lines("gtk_k7_act_lines"), rows), cols, dtype=_FLOAT) if want_sum else None
-    err = _lib.calls().gtk_k7_act_backward(TYPES[dy.dtype], dy.data_ptr(), ld(dy), zp, zld, e, eld, activation, _ptr(dz), cols, _ptr(db),
+    err = _lib.calls().gtk_k7_act_backward(TYPES[dy.dtype], dy.data_ptr(), ld(dy), zp, zld, e, eld, activation, _ptr(dz),
+                                           0 if dz is None else ld(dz), _ptr(db),
                                            _ptr(partial), rows, cols, stream_of(dy))
     if err:
         _lib.check(err, "gtk_k7_act_backward")
@@ -192,10 +200,10 @@ class Activation8:
             return oracle.restore8(self.q, self.e, self.dtype).view(self.shape)
         out = self.q.new_empty(rows, cols, dtype=self.dtype)
         if rows and cols:
-            err = _lib.calls().gtk_k7_stage(TYPES[self.dtype], self.q.data_ptr(), ld(self.q), self.e.data_ptr(), ld(self.e), None, None, None, None, 0,
-                                            0, out.data_ptr(), cols, 0, rows, cols, cols, stream_of(self.q))
+            err = _lib.calls().gtk_k7_restore(TYPES[self.dtype], self.q.data_ptr(), ld(self.q), self.e.data_ptr(), ld(self.e), None, None, None, None,
+                                              out.data_ptr(), cols, rows, cols, stream_of(self.q))
             if err:
-                _lib.check(err, "gtk_k7_stage")
+                _lib.check(err, "gtk_k7_restore")
         return out if len(self.shape) == 2 else out.view(self.shape)
 
     def backward(self, dy: torch.Tensor, activation: str) -> Tuple[torch.Tensor, torch.Tensor]:

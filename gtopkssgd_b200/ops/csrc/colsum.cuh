@@ -6,10 +6,10 @@
 
 namespace gtk {
 
-// partial[lines][cols] -> out0[0 .. split) and out1[0 .. cols - split), of type T.  A CTA of 32 x 8 threads takes 32
-// columns; 8 threads share a column's lines.
+// partial[lines][cols] -> up to three vectors of `each` sums, one after the other in a line (a null one is left out).  A CTA
+// of 32 x 8 threads takes 32 columns; 8 threads share a column's lines.
 template <typename T>
-__global__ void __launch_bounds__(256) col_finish(const float* partial, int lines, long long cols, long long split, T* out0, T* out1) {
+__global__ void __launch_bounds__(256) col_finish(const float* partial, int lines, long long cols, long long each, T* out0, T* out1, T* out2) {
   __shared__ float s[8][33];
   pdl_begin(partial);
   const long long c = (long long)blockIdx.x * 32 + threadIdx.x;
@@ -30,17 +30,14 @@ __global__ void __launch_bounds__(256) col_finish(const float* partial, int line
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += s[i][threadIdx.x];
-    if (c < split) {
-      if (out0) out0[c] = from_f32<T>(sum);
-    } else if (out1) {
-      out1[c - split] = from_f32<T>(sum);
-    }
+    T* out = c < each ? out0 : c < 2 * each ? out1 : out2;
+    if (out) out[c % each] = from_f32<T>(sum);
   }
 }
 
 template <typename T>
-inline cudaError_t launch_col_finish(const float* partial, int lines, long long cols, long long split, T* out0, T* out1, cudaStream_t stream) {
-  return launch_pdl(col_finish<T>, dim3((unsigned)((cols + 31) / 32)), dim3(32, 8), stream, partial, lines, cols, split, out0, out1);
+inline cudaError_t launch_col_finish(const float* partial, int lines, long long cols, long long each, T* out0, T* out1, T* out2, cudaStream_t stream) {
+  return launch_pdl(col_finish<T>, dim3((unsigned)((cols + 31) / 32)), dim3(32, 8), stream, partial, lines, cols, each, out0, out1, out2);
 }
 
 }  // namespace gtk

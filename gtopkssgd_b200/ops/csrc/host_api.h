@@ -90,17 +90,17 @@ int gtk_k4_finalize(void* state, float scale, float max_norm, float* coef_out, v
 int gtk_k5_top1(const float* logits, const long long* target, int rows, int classes, float scale, float* out,
                 void* stream);
 int gtk_k6_norm_lines(void);
-int gtk_k6_norm_forward(int type, const void* x, long long x_ld, const void* w, const void* b, void* y, float* mean,
-                        float* rstd, long long rows, long long cols, float eps, void* stream);
-int gtk_k6_norm_backward(int type, const void* dy, long long dy_ld, const void* x, long long x_ld, const float* mean,
-                         const float* rstd, const void* w, const void* add, long long add_ld, void* dx, void* dw,
-                         void* db, float* partial, long long rows, long long cols, void* stream);
+int gtk_k6_norm_forward(int type, const void* x, long long x_ld, const void* w, const void* b, void* y, long long y_ld,
+                        float* mean, float* rstd, long long rows, long long cols, float eps, void* stream);
+int gtk_k6_norm_backward(int type, const void* dy, long long dy_ld, const void* x, long long x_ld,
+                         const unsigned char* e, long long e_ld, const float* mean, const float* rstd, const void* w,
+                         const void* b, const void* add, long long add_ld, void* dx, void* dw, void* db, void* y,
+                         long long y_ld, void* dadd, float* partial, long long rows, long long cols, void* stream);
 int gtk_k7_keep(int type, const void* x, long long x_ld, signed char* q, long long q_ld, unsigned char* e,
                 long long e_ld, long long rows, long long cols, void* stream);
-int gtk_k7_stage(int type, const void* src, long long src_ld, const unsigned char* e, long long e_ld,
-                 const float* mean, const float* rstd, const void* g, const void* b, int act, int out_kind, void* out,
-                 long long out_ld, long long piece_stride, long long rows, long long cols, long long pitch,
-                 void* stream);
+int gtk_k7_restore(int type, const void* src, long long src_ld, const unsigned char* e, long long e_ld,
+                   const float* mean, const float* rstd, const void* g, const void* b, void* out, long long out_ld,
+                   long long rows, long long cols, void* stream);
 int gtk_k7_pack(gtk_addresses list, void* stream);
 int gtk_k7_act_lines(void);
 int gtk_k7_act_backward(int type, const void* dy, long long dy_ld, const void* z, long long z_ld,
@@ -114,8 +114,8 @@ int gtk_k8_gemm(int type, int half, long long m, long long n, long long k, const
                 void* z, long long z_ld, signed char* q, long long q_ld, unsigned char* e8, long long e_ld, void* h,
                 long long h_ld, float* sums, void* db, void* stream);
 int gtk_k9_few_rows(int type, const void* x, long long x_ld, const void* w, long long w_ld, long long m, long long n,
-                    long long k, void* y, const void* bias, const void* add, long long add_ld, int act, void* z,
-                    signed char* q, long long q_ld, unsigned char* e, long long e_ld, void* stream);
+                    long long k, void* y, long long y_ld, const void* bias, const void* add, long long add_ld, int act,
+                    void* z, signed char* q, long long q_ld, unsigned char* e, long long e_ld, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,8 +1,8 @@
 // K7: element-wise passes over a matrix of activations.
 //
 //   k7_keep          x -> 8-bit codes and one exponent byte per 32 columns of a row (the format is in ff_math.cuh)
-//   k7_stage         a matrix, in its own type or in 8 bits, -> operand or result: restored, with the norm or the
-//                    activation applied again, or split into bf16 pieces for the f32 matrix product
+//   k7_restore       a matrix, in 8 bits or in its own type, restored, or with the norm applied again
+//   k7_pack          matrices -> operands of a matrix product
 //   k7_act_backward  dz = dy act'(z) and the sums of dz over the rows (the bias's gradient)
 //
 // Bound by memory.  A warp takes 32 * VEC neighbouring columns of a row, so that a block of 32 lies in 32 / VEC
@@ -100,64 +100,37 @@ __device__ __forceinline__ void hold_f16(float (&v)[VEC]) {
     if (fabsf(v[j]) > 65504.f) v[j] = copysignf(65504.f, v[j]);
 }
 
-// What is done to it: (v - mean) rstd g + b where mean is given, then the activation.
-template <typename G>
+// What is done to it: (v - mean) rstd g + b where mean is given.
+template <typename T>
 struct Apply {
   const float* mean;
   const float* rstd;
-  const G* g;
-  const G* b;
-  int act;
+  const T* g;
+  const T* b;
 };
 
-// out: `pieces` matrices of rows x out_ld, piece_stride elements apart; columns cols .. pitch - 1 are written as zeros
-// where the pitch is an operand's (a multiple of VEC).
-template <typename S, typename O, typename G, int PIECES, int VEC>
-__global__ void __launch_bounds__(256) k7_stage(Source src, Apply<G> f, O* out, long long out_ld, long long piece_stride, long long rows, int cols, int pitch,
-                                                int rows_per_warp) {
+template <typename S, typename T, int VEC>
+__global__ void __launch_bounds__(256) k7_restore(Source src, Apply<T> f, T* out, long long out_ld, long long rows, int cols, int rows_per_warp) {
   pdl_begin(src.p, src.e, f.mean, f.rstd, f.g, f.b);
   const int c = (int)((blockIdx.x * 32 + threadIdx.x) * VEC);
-  if (c >= pitch) return;
+  if (c >= cols) return;
   const long long first = ((long long)blockIdx.y * kRowWarps + threadIdx.y) * rows_per_warp;
   for (int i = 0; i < rows_per_warp; ++i) {
     const long long row = first + i;
     if (row >= rows) return;
     float v[VEC];
-    if (c < cols) {
-      load_source<S, VEC>(src, row, c, v);
-      if constexpr (sizeof(S) == 1 && std::is_same_v<O, __half>) hold_f16<VEC>(v);
-      if (f.mean) {
-        const float m = f.mean[row], r = f.rstd[row];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          v[j] = (v[j] - m) * r;
-          if (f.g) v[j] *= to_f32(f.g[c + j]);
-          if (f.b) v[j] += to_f32(f.b[c + j]);
-        }
-      }
-      if (f.act != kActNone)
-        with_act(f.act, [&](auto A) {
-          act_values<decltype(A)::value, VEC>(v);
-        });
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[j] = 0.f;
-    }
-    O* at = out + row * out_ld + c;
-    if constexpr (PIECES == 3) {
-      Vec<__nv_bfloat16, VEC> o[3];
+    load_source<S, VEC>(src, row, c, v);
+    if constexpr (sizeof(S) == 1 && std::is_same_v<T, __half>) hold_f16<VEC>(v);
+    if (f.mean) {
+      const float m = f.mean[row], r = f.rstd[row];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        __nv_bfloat16 p[3];
-        split3(v[j], p);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) o[k].v[j] = p[k];
+        v[j] = (v[j] - m) * r;
+        if (f.g) v[j] *= to_f32(f.g[c + j]);
+        if (f.b) v[j] += to_f32(f.b[c + j]);
       }
-#pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<Vec<__nv_bfloat16, VEC>*>(at + k * piece_stride) = o[k];
-    } else {
-      store_f32<O, VEC>(at, v);
     }
+    store_f32<T, VEC>(out + row * out_ld + c, v);
   }
 }
 
@@ -488,23 +461,23 @@ int keep(const void* x, long long x_ld, signed char* q, long long q_ld, unsigned
   return go(std::integral_constant<int, 1>{});
 }
 
-template <typename S, typename O, typename G, int PIECES>
-int stage(Source src, Apply<G> f, void* out, long long out_ld, long long piece_stride, long long rows, int cols, int pitch, cudaStream_t stream) {
+template <typename S, typename T>
+int restore(Source src, Apply<T> f, void* out, long long out_ld, long long rows, int cols, cudaStream_t stream) {
   auto go = [&](auto V) -> int {
     constexpr int VEC = decltype(V)::value;
-    const unsigned strips = (unsigned)((pitch + 32 * VEC - 1) / (32 * VEC));
+    const unsigned strips = (unsigned)((cols + 32 * VEC - 1) / (32 * VEC));
     int per;
     unsigned y;
     if (!row_grid(rows, strips, &per, &y)) return GTK_ERR_UNSUPPORTED;
-    const cudaError_t err = launch_pdl(k7_stage<S, O, G, PIECES, VEC>, dim3(strips, y), dim3(32, kRowWarps), stream, src, f, (O*)out, out_ld, piece_stride,
-                                       rows, cols, pitch, per);
+    const cudaError_t err = launch_pdl(k7_restore<S, T, VEC>, dim3(strips, y), dim3(32, kRowWarps), stream, src, f, (T*)out, out_ld, rows, cols, per);
     gtk_count_launch(1);
     return err == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;
   };
   // a block's scale is read once per vector, so vectors do not cross blocks (they start at multiples of their length)
-  constexpr int wide = sizeof(S) == 4 || sizeof(O) == 4 ? 4 : sizeof(S) == 1 ? 16 : 8;   // more elements a thread: fewer addresses
+  constexpr int wide = sizeof(T) == 4 ? 4 : sizeof(S) == 1 ? 16 : 8;   // more elements a thread: fewer addresses
   auto fits = [&](int vec) {
-    return cols % vec == 0 && pitch % vec == 0 && piece_stride % vec == 0 && aligned(src.p, src.ld, sizeof(S), vec) && aligned(out, out_ld, sizeof(O), vec < 8 ? vec : 16 / (int)sizeof(O));
+    const int most = vec < 16 / (int)sizeof(T) ? vec : 16 / (int)sizeof(T);   // 16 bytes at a time
+    return cols % vec == 0 && aligned(src.p, src.ld, sizeof(S), vec < 16 / (int)sizeof(S) ? vec : 16 / (int)sizeof(S)) && aligned(out, out_ld, sizeof(T), most);
   };
   if (fits(wide)) return go(std::integral_constant<int, wide>{});
   if constexpr (wide == 16) {
@@ -552,7 +525,7 @@ int act_backward(const void* dy, long long dy_ld, Source z, int act, void* dz, l
   gtk_count_launch(1);
   if (err != cudaSuccess) return GTK_ERR_CUDA;
   if (!db || lines == 1) return GTK_OK;
-  err = launch_col_finish<T>(partial, (int)lines, cols, cols, (T*)db, (T*)nullptr, stream);
+  err = launch_col_finish<T>(partial, (int)lines, cols, cols, (T*)db, (T*)nullptr, (T*)nullptr, stream);
   gtk_count_launch(1);
   return err == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;
 }
@@ -576,30 +549,16 @@ extern "C" int gtk_k7_keep(int type, const void* x, long long x_ld, signed char*
   return GTK_ERR_ARG;
 }
 
-// The matrix src (of `type`, or 8-bit codes where e is given), normalised again where mean is given, through the
-// activation, -> out.  out_kind 0: a matrix of `type`; 1: one bf16 piece (f32 codes without a transform, which are
-// exact in it); 3: three bf16 pieces (f32).  Columns up to `pitch` are written, those past `cols` as zeros.
-extern "C" int gtk_k7_stage(int type, const void* src, long long src_ld, const unsigned char* e, long long e_ld, const float* mean, const float* rstd,
-                            const void* g, const void* b, int act, int out_kind, void* out, long long out_ld, long long piece_stride, long long rows,
-                            long long cols, long long pitch, void* stream_) {
-  if (rows <= 0 || cols <= 0 || pitch < cols || out_ld < pitch || pitch > 0x3fffffff || src_ld < 0 || act < 0 || act >= kActCount) return GTK_ERR_ARG;
+// The matrix src (of `type`, or 8-bit codes where e is given), normalised again where mean is given, -> out, of `type`.
+extern "C" int gtk_k7_restore(int type, const void* src, long long src_ld, const unsigned char* e, long long e_ld, const float* mean, const float* rstd,
+                              const void* g, const void* b, void* out, long long out_ld, long long rows, long long cols, void* stream_) {
+  if (rows <= 0 || cols <= 0 || out_ld < cols || cols > 0x3fffffff || src_ld < 0) return GTK_ERR_ARG;
   const cudaStream_t stream = (cudaStream_t)stream_;
   const Source s{src, src_ld, e, e_ld};
-  const int n = (int)cols, p = (int)pitch;
   auto of = [&](auto t) -> int {
     using T = decltype(t);
-    const Apply<T> f{mean, rstd, (const T*)g, (const T*)b, act};
-    if (out_kind == 0)
-      return e ? stage<signed char, T, T, 1>(s, f, out, out_ld, piece_stride, rows, n, p, stream)
-               : stage<T, T, T, 1>(s, f, out, out_ld, piece_stride, rows, n, p, stream);
-    if constexpr (sizeof(T) == 4) {
-      if (out_kind == 1 && e && !mean && act == kActNone)
-        return stage<signed char, __nv_bfloat16, T, 1>(s, f, out, out_ld, piece_stride, rows, n, p, stream);
-      if (out_kind == 3)
-        return e ? stage<signed char, __nv_bfloat16, T, 3>(s, f, out, out_ld, piece_stride, rows, n, p, stream)
-                 : stage<T, __nv_bfloat16, T, 3>(s, f, out, out_ld, piece_stride, rows, n, p, stream);
-    }
-    return GTK_ERR_ARG;
+    const Apply<T> f{mean, rstd, (const T*)g, (const T*)b};
+    return e ? restore<signed char, T>(s, f, out, out_ld, rows, (int)cols, stream) : restore<T, T>(s, f, out, out_ld, rows, (int)cols, stream);
   };
   switch (type) {
     case kF32: return of(float{});

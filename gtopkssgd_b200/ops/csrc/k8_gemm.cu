@@ -992,9 +992,9 @@ extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long lo
   const int lines = (s.m + 31) / 32;
   if (!db || lines == 1) return GTK_OK;
   switch (type) {
-    case kF32: err = launch_col_finish<float>(sums, lines, n, n, (float*)db, (float*)nullptr, stream); break;
-    case kF16: err = launch_col_finish<__half>(sums, lines, n, n, (__half*)db, (__half*)nullptr, stream); break;
-    default: err = launch_col_finish<__nv_bfloat16>(sums, lines, n, n, (__nv_bfloat16*)db, (__nv_bfloat16*)nullptr, stream); break;
+    case kF32: err = launch_col_finish<float>(sums, lines, n, n, (float*)db, (float*)nullptr, (float*)nullptr, stream); break;
+    case kF16: err = launch_col_finish<__half>(sums, lines, n, n, (__half*)db, (__half*)nullptr, (__half*)nullptr, stream); break;
+    default: err = launch_col_finish<__nv_bfloat16>(sums, lines, n, n, (__nv_bfloat16*)db, (__nv_bfloat16*)nullptr, (__nv_bfloat16*)nullptr, stream); break;
   }
   gtk_count_launch(1);
   return err == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;

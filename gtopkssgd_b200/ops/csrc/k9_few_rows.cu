@@ -10,8 +10,8 @@
 //
 // A CTA takes 32 rows of W (a block of the 8-bit form): two halves of 8 warps, which take 64 of k in turn and join
 // their sums through shared memory, in order.  The next 64 of W and x are on their way meanwhile (x, too, comes from L2:
-// no two warps of a half read the same part of it).  f32: three bf16 pieces a value, the six products that count, the
-// large one summed apart from the small ones, as in K8.
+// no two warps of a half read the same part of it).  f32: three bf16 pieces a value and the six products that count; the
+// large one is summed apart from the small ones, and both go to an f32 sum after every 64 of k, as in K8.
 #include "colsum.cuh"
 #include "common.cuh"
 #include "host_api.h"
@@ -29,6 +29,7 @@ struct FewArgs {
   long long x_ld, w_ld;
   int m, n, k;
   void* y;
+  long long y_ld;
   const void* bias;
   const void* add;
   long long add_ld;
@@ -109,11 +110,11 @@ __global__ void __launch_bounds__(kFewThreads) k9_few_rows(FewArgs g) {
   const T* xr[TOK];
 #pragma unroll
   for (int t = 0; t < TOK; ++t) xr[t] = (const T*)g.x + (long long)(r0 + min(t * 8 + row, rows - 1)) * g.x_ld;
-  float large[TOK][4], small[TOK][4];
+  float large[TOK][4], small[TOK][4], total[TOK][4];
 #pragma unroll
   for (int t = 0; t < TOK; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) large[t][i] = small[t][i] = 0.f;
+    for (int i = 0; i < 4; ++i) large[t][i] = small[t][i] = total[t][i] = 0.f;
   // Loads of single 16-bit elements are put together at once and cannot be ahead; f32 has registers for x's only with
   // up to 8 rows.
   constexpr bool kAhead = VEC * sizeof(T) >= 4, kXAhead = kAhead && (sizeof(T) == 2 || TOK == 1);
@@ -166,12 +167,21 @@ __global__ void __launch_bounds__(kFewThreads) k9_few_rows(FewArgs g) {
         }
       }
     }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int t = 0; t < TOK; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          total[t][i] += large[t][i] + small[t][i];
+          large[t][i] = small[t][i] = 0.f;
+        }
+    }
   }
 #pragma unroll
   for (int t = 0; t < TOK; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      sums[split][half * 16 + row + (i >> 1) * 8][t * 8 + quad * 2 + (i & 1)] = sizeof(T) == 2 ? large[t][i] : large[t][i] + small[t][i];
+      sums[split][half * 16 + row + (i >> 1) * 8][t * 8 + quad * 2 + (i & 1)] = sizeof(T) == 2 ? large[t][i] : total[t][i];
   __syncthreads();
   // a lane is a column of y, a warp takes rows in turn
   const int col = (int)blockIdx.x * 32 + lane;
@@ -192,7 +202,7 @@ __global__ void __launch_bounds__(kFewThreads) k9_few_rows(FewArgs g) {
       if (g.z) ((T*)g.z)[r * g.n + col] = from_f32<T>(v);
       with_act(g.act, [&](auto A) { v = act_value<decltype(A)::value>(v); });
       if (g.add) v += to_f32(((const T*)g.add)[r * g.add_ld + col]);
-      ((T*)g.y)[r * g.n + col] = from_f32<T>(v);
+      ((T*)g.y)[r * g.y_ld + col] = from_f32<T>(v);
     }
   }
 }
@@ -221,15 +231,15 @@ cudaError_t launch_few(const FewArgs& g, cudaStream_t stream) {
 
 using namespace gtk;
 
-// y[m][n] = act(x W^T + bias) + add; y and z dense, everything of `type`.  q has q_ld >= n rounded up to 32.
+// y[m][n] = act(x W^T + bias) + add; z dense, everything of `type`.  q has q_ld >= n rounded up to 32.
 extern "C" int gtk_k9_few_rows(int type, const void* x, long long x_ld, const void* w, long long w_ld, long long m, long long n, long long k, void* y,
-                               const void* bias, const void* add, long long add_ld, int act, void* z, signed char* q, long long q_ld, unsigned char* e,
+                               long long y_ld, const void* bias, const void* add, long long add_ld, int act, void* z, signed char* q, long long q_ld, unsigned char* e,
                                long long e_ld, void* stream) {
-  if (m <= 0 || m > kFewMost || n <= 0 || k <= 0 || !x || !w || !y || x_ld < 0 || w_ld < 0 || act < 0 || act >= kActCount ||
+  if (m <= 0 || m > kFewMost || n <= 0 || k <= 0 || !x || !w || !y || x_ld < 0 || w_ld < 0 || y_ld < n || act < 0 || act >= kActCount ||
       (q && (!e || q_ld < (n + kBlock8 - 1) / kBlock8 * kBlock8)))
     return GTK_ERR_ARG;
   if (n > 0x3fffffff || k > 0x3fffffff) return GTK_ERR_UNSUPPORTED;
-  const FewArgs g{x, w, x_ld, w_ld, (int)m, (int)n, (int)k, y, bias, add, add_ld, act, z, q, q_ld, e, e_ld};
+  const FewArgs g{x, w, x_ld, w_ld, (int)m, (int)n, (int)k, y, y_ld, bias, add, add_ld, act, z, q, q_ld, e, e_ld};
   cudaError_t err;
   switch (type) {
     case kF32: err = launch_few<float>(g, (cudaStream_t)stream); break;

@@ -131,7 +131,7 @@ PyMethodDef kMethods[] = {
     GTK_METHOD(gtk_k3_momentum_correct), GTK_METHOD(gtk_k4_sumsq_dense), GTK_METHOD(gtk_k4_sumsq_pairs),
     GTK_METHOD(gtk_k4_finalize),      GTK_METHOD(gtk_k5_top1),
     GTK_METHOD(gtk_k6_norm_forward),  GTK_METHOD(gtk_k6_norm_backward), GTK_METHOD(gtk_k7_keep),
-    GTK_METHOD(gtk_k7_stage),         GTK_METHOD(gtk_k7_pack),          GTK_METHOD(gtk_k7_act_backward),
+    GTK_METHOD(gtk_k7_restore),       GTK_METHOD(gtk_k7_pack),          GTK_METHOD(gtk_k7_act_backward),
     GTK_METHOD(gtk_k8_gemm),          GTK_METHOD(gtk_k9_few_rows),
     {"clear_grads", clear_grads, METH_O, nullptr},
     {"grad_addresses", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&grad_addresses)), METH_FASTCALL, nullptr},

@@ -16,9 +16,10 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 
 from . import layers_oracle as oracle
-from .activation8 import Activation8, act_of, bits_of, colsum, matrix, parameter, same, shaped, stream_of, type_of
-from .layer_norm import layer_norm_backward, layer_norm_forward
-from .linear import _check, _gradients, linear_forward, normed, operands, pairs_for, product
+from .activation8 import Activation8, act_of, bits_of, colsum, matrix, padded_rows, parameter, same, shaped, stream_of, type_of
+from .layer_norm import MOST_IN_BLOCK, layer_norm_backward, norm_backward_in_block
+from .layer_norm import _forward as _norm_forward
+from .linear import _check, _forward, normed, operands, pairs_for, product
 
 
 class FeedForwardKept(NamedTuple):
@@ -38,9 +39,12 @@ def feed_forward(x: torch.Tensor, norm_weight: torch.Tensor, norm_bias: torch.Te
         raise ValueError("feed_forward: without an activation the two products are one")
     _check(x, w1, "feed_forward")
     shaped("w2", w2, w1.size(1), w1.size(0))
-    a, mean, rstd = layer_norm_forward(x, norm_weight, norm_bias, eps)
-    h, z = linear_forward(a, w1, b1, activation, keep=keep, bits=bits)
-    y, _ = linear_forward(h, w2, b2, residual=x)
+    m = matrix(x)
+    a, mean, rstd = _norm_forward(m, norm_weight, norm_bias, eps, True)   # operands of the next product, where they lie
+    h, z = _forward(a, w1, b1, activation, None, keep, bits, True)
+    y, _ = _forward(h, w2, b2, "none", m, False, 0, False)
+    if x.dim() != 2:
+        y, mean, rstd = y.view(x.shape), mean.view(x.shape[:-1]), rstd.view(x.shape[:-1])
     if not keep:
         return y, None
     return y, FeedForwardKept(Activation8.keep(x) if bits else x, mean, rstd, z)
@@ -78,7 +82,7 @@ def feed_forward_backward(dy: torch.Tensor, kept: FeedForwardKept, norm_weight: 
     mean, rstd = mean.contiguous(), rstd.contiguous()
     pairs = pairs_for(dy.dtype, True, rows, hidden, dim)
     # dz = (dy W2) act'(z) and h = act(z) again, both in the product's epilogue
-    dz, h, db1 = new(rows, hidden), new(rows, hidden), new(hidden)
+    dz, h, db1 = padded_rows(g, rows, hidden), padded_rows(g, rows, hidden), new(hidden)
     go, w2o = operands(pairs, (g, 1), (matrix(w2), 0))
     product(rows, hidden, dim, go, False, w2o, True, dz, stream, activation=code, slope=True, z=z, h=h, db=db1)
     del w2o
@@ -89,10 +93,22 @@ def feed_forward_backward(dy: torch.Tensor, kept: FeedForwardKept, norm_weight: 
         ho, = operands(False, (h, 0))
     product(dim, hidden, rows, go, True, ho, True, dw2, stream)
     del h, go, ho
-    _, db2 = colsum(g)
-    a = normed(x if isinstance(x, Activation8) else matrix(x), mean, rstd, norm_weight, norm_bias, pairs)   # the norm's output again
-    da, dw1 = _gradients(dz, a, w1, True, True)
-    dx, dg, db = layer_norm_backward(da.view(shape), x.restore() if isinstance(x, Activation8) else x, mean, rstd, norm_weight, add=dy)
+    zo, w1o, *zt = operands(pairs, (dz, 1), (matrix(w1), 0), *(((dz, 0),) if pairs else ()))
+    da = new(rows, dim)
+    product(rows, dim, hidden, zo, False, w1o, True, da, stream)
+    del w1o
+    xm = x if isinstance(x, Activation8) else matrix(x)
+    if dim <= MOST_IN_BLOCK:   # the norm's output again and dy's sums on the way
+        dx, dg, db, a, db2 = norm_backward_in_block(da, xm, mean, rstd, norm_weight, norm_bias, g)
+    else:
+        a = normed(xm, mean, rstd, norm_weight, norm_bias)
+        dx, dg, db = layer_norm_backward(da, x.restore().view(rows, dim) if isinstance(x, Activation8) else xm, mean, rstd, norm_weight, add=g)
+        _, db2 = colsum(g)
+    dw1 = new(hidden, dim)
+    ao, = operands(pairs, (a, 0))
+    product(hidden, dim, rows, zt[0] if pairs else zo, True, ao, True, dw1, stream)
+    if len(shape) != 2:
+        dx = dx.view(shape)
     return dx, dg, db, dw1, db1, dw2, db2
 
 

@@ -13,7 +13,7 @@ import torch
 
 from . import layers_oracle as oracle
 from . import lib as _lib
-from .activation8 import ld, lines, matrix, parameter, same, shaped, stream_of, type_of
+from .activation8 import TYPES, Activation8, ld, lines, matrix, padded_rows, parameter, same, shaped, stream_of, type_of
 from .select import _FLOAT, _ptr
 
 
@@ -21,6 +21,11 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
                        eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(y, mean, rstd): y = (x - mean) * rstd * weight + bias, rstd = (variance + eps)^-1/2; mean and rstd are f32, of
     x's shape without its last axis."""
+    return _forward(x, weight, bias, eps, False)
+
+
+def _forward(x, weight, bias, eps, padded: bool):
+    """``padded``: y of two axes, its rows on 16-byte boundaries."""
     code = type_of(x, "layer_norm")
     m = matrix(x)
     rows, cols = m.shape
@@ -31,12 +36,12 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
     if not m.is_cuda:
         y, mean, rstd = oracle.norm_forward(m, weight, bias, eps)
         return y.view(x.shape), mean.view(x.shape[:-1]), rstd.view(x.shape[:-1])
-    y = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+    y = padded_rows(x, rows, cols) if padded else torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
     mean = x.new_empty(rows, dtype=_FLOAT)
     rstd = torch.empty_like(mean)
     if rows:
-        err = _lib.calls().gtk_k6_norm_forward(code, m.data_ptr(), ld(m), _ptr(weight), _ptr(bias), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
-                                               rows, cols, eps, stream_of(m))
+        err = _lib.calls().gtk_k6_norm_forward(code, m.data_ptr(), ld(m), _ptr(weight), _ptr(bias), y.data_ptr(), ld(y) if padded else cols,
+                                               mean.data_ptr(), rstd.data_ptr(), rows, cols, eps, stream_of(m))
         if err:
             _lib.check(err, "gtk_k6_norm_forward")
     if x.dim() == 2:
@@ -80,12 +85,36 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
             db.zero_()
         return dx, dw, db
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    err = _lib.calls().gtk_k6_norm_backward(code, g.data_ptr(), ld(g), m.data_ptr(), ld(m), mean.data_ptr(), rstd.data_ptr(), _ptr(weight), _ptr(add),
-                                            0 if add is None else ld(add), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(partial), rows, cols,
-                                            stream_of(m))
+    err = _lib.calls().gtk_k6_norm_backward(code, g.data_ptr(), ld(g), m.data_ptr(), ld(m), None, 0, mean.data_ptr(), rstd.data_ptr(), _ptr(weight), None,
+                                            _ptr(add), 0 if add is None else ld(add), dx.data_ptr(), _ptr(dw), _ptr(db), None, 0, None,
+                                            _ptr(partial), rows, cols, stream_of(m))
     if err:
         _lib.check(err, "gtk_k6_norm_backward")
     return dx, dw, db
+
+
+MOST_IN_BLOCK = 16384   # columns
+
+
+def norm_backward_in_block(da: torch.Tensor, x, mean: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, dy: torch.Tensor):
+    """(dx, dweight, dbias, a, dysum) over CUDA matrices of up to ``MOST_IN_BLOCK`` columns, for a block's backward pass: x
+    may be codes; dx is with dy, the gradient that goes past the norm, of which dysum is the sum over the rows; a, the
+    norm's output, is made again, its rows on 16-byte boundaries."""
+    codes = type(x) is Activation8
+    m = x.q if codes else x
+    rows, cols = da.shape
+    dx = da.new_empty(rows, cols)
+    a = padded_rows(da, rows, cols)
+    dw = da.new_empty(cols)
+    db, dysum = torch.empty_like(dw), torch.empty_like(dw)
+    partial = da.new_empty(min(lines("gtk_k6_norm_lines"), max(rows, 2)), 3 * cols, dtype=_FLOAT)
+    err = _lib.calls().gtk_k6_norm_backward(TYPES[da.dtype], da.data_ptr(), ld(da), m.data_ptr(), ld(m), x.e.data_ptr() if codes else None,
+                                            ld(x.e) if codes else 0, mean.data_ptr(), rstd.data_ptr(), weight.data_ptr(), bias.data_ptr(),
+                                            dy.data_ptr(), ld(dy), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), a.data_ptr(), ld(a),
+                                            dysum.data_ptr(), partial.data_ptr(), rows, cols, stream_of(da))
+    if err:
+        _lib.check(err, "gtk_k6_norm_backward")
+    return dx, dw, db, a, dysum
 
 
 class _LayerNorm(torch.autograd.Function):

@@ -15,7 +15,7 @@ import torch
 
 from . import layers_oracle as oracle
 from . import lib as _lib
-from .activation8 import TYPES, Activation8, act_of, bits_of, colsum, ld, matrix, parameter, same, shaped, stream_of, type_of
+from .activation8 import TYPES, Activation8, act_of, bits_of, colsum, ld, matrix, padded_rows, parameter, same, shaped, stream_of, type_of
 from .select import _FLOAT, _ptr
 
 # Rows up to which K9 takes a forward pass, us on the device by K9 and by K8, whose operands have to be made first: 1500 x 6000
@@ -110,27 +110,22 @@ def operands(pairs: bool, *specs) -> list:
     return made
 
 
-def normed(src, mean, rstd, weight, bias, pairs: bool):
-    """The matrix (v - mean) * rstd * weight + bias of a matrix or of codes, as an operand (f32 with ``pairs``: as a
-    matrix, for ``operands``)."""
+def normed(src, mean, rstd, weight, bias) -> torch.Tensor:
+    """The matrix (v - mean) * rstd * weight + bias of a matrix or of codes."""
     codes = type(src) is Activation8
     m = src.q if codes else src
     rows, cols = m.shape
-    split = src.dtype is _FLOAT and not pairs
-    pieces, pitch = (3, (cols + 7) & ~7) if split else (1, cols if pairs else (cols + 7) & ~7)
-    out = m.new_empty(pieces, rows, pitch, dtype=torch.bfloat16 if split else src.dtype)
-    err = _lib.calls().gtk_k7_stage(TYPES[src.dtype], m.data_ptr(), ld(m), src.e.data_ptr() if codes else None, ld(src.e) if codes else 0,
-                                    mean.data_ptr(), rstd.data_ptr(), _ptr(weight), _ptr(bias), 0, 3 if split else 0, out.data_ptr(), pitch,
-                                    rows * pitch, rows, cols, pitch, stream_of(m))
+    out = m.new_empty(rows, cols, dtype=src.dtype)
+    err = _lib.calls().gtk_k7_restore(TYPES[src.dtype], m.data_ptr(), ld(m), src.e.data_ptr() if codes else None, ld(src.e) if codes else 0,
+                                      mean.data_ptr(), rstd.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), cols, rows, cols, stream_of(m))
     if err:
-        _lib.check(err, "gtk_k7_stage")
-    return out[0] if pairs else Operand(out.data_ptr(), pitch, pieces, rows * pitch, 0, out)
+        _lib.check(err, "gtk_k7_restore")
+    return out
 
 
 def product(m: int, n: int, k: int, a: Operand, a_mn: bool, b: Operand, b_mn: bool, out: torch.Tensor, stream: int, bias=None, add=None,
             activation: int = 0, slope: bool = False, z: Kept = None, h: Optional[torch.Tensor] = None, db: Optional[torch.Tensor] = None) -> None:
-    """out[m, n] = epilogue(sum_k a[m, k] b[n, k]); ``a_mn``, ``b_mn``: the operand's matrix is [k, m] or [k, n].  out and
-    h are dense."""
+    """out[m, n] = epilogue(sum_k a[m, k] b[n, k]); ``a_mn``, ``b_mn``: the operand's matrix is [k, m] or [k, n]."""
     sums = None
     zp = zld = q = qld = e = eld = None
     if z is None:
@@ -144,8 +139,8 @@ def product(m: int, n: int, k: int, a: Operand, a_mn: bool, b: Operand, b_mn: bo
     if db is not None:
         sums = out.new_empty(-(-m // 32), n, dtype=_FLOAT)
     err = _lib.calls().gtk_k8_gemm(TYPES[out.dtype], out.dtype is torch.float16 or a.pieces == 2, m, n, k, a.at, a.ld, a.pieces, a.stride, a_mn,
-                                   a.most or None, b.at, b.ld, b.pieces, b.stride, b_mn, b.most or None, out.data_ptr(), n, _ptr(bias), _ptr(add), 0 if add is None else ld(add), activation, slope, zp,
-                                   zld, q, qld, e, eld, _ptr(h), n, _ptr(sums), _ptr(db), stream)
+                                   a.most or None, b.at, b.ld, b.pieces, b.stride, b_mn, b.most or None, out.data_ptr(), ld(out), _ptr(bias), _ptr(add), 0 if add is None else ld(add), activation, slope, zp,
+                                   zld, q, qld, e, eld, _ptr(h), 0 if h is None else ld(h), _ptr(sums), _ptr(db), stream)
     if err:
         _lib.check(err, "gtk_k8_gemm")
 
@@ -162,6 +157,11 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
                    residual: Optional[torch.Tensor] = None, keep: bool = False, bits: int = 0) -> Tuple[torch.Tensor, Kept]:
     """(y, z): y = act(x W^T + bias) + residual.  With ``keep`` z is the activation's input for ``linear_backward``, in
     x's type or, with ``bits=8``, as ``Activation8``; None where there is no activation."""
+    return _forward(x, weight, bias, activation, residual, keep, bits, False)
+
+
+def _forward(x, weight, bias, activation, residual, keep, bits, padded: bool):
+    """``padded``: y of two axes, its rows on 16-byte boundaries."""
     type_of(x, "linear")
     code = act_of(activation)
     if bits:
@@ -181,7 +181,7 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
         y, z = oracle.linear_forward(m, weight, bias, activation, residual)
         z = None if not keep else Activation8(*oracle.keep8(z), x.dtype) if bits else z.to(x.dtype)
         return y.view(shape), z
-    y = x.new_empty(rows, outer)
+    y = padded_rows(x, rows, outer) if padded else x.new_empty(rows, outer)
     z = None
     if keep:
         z = Activation8.empty(x, rows, outer, (rows, outer)) if bits else x.new_empty(rows, outer)
@@ -196,7 +196,7 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
                 q, qld, e, eld = z.q.data_ptr(), z.e.size(1) * 32, z.e.data_ptr(), z.e.size(1)
             else:
                 zp = z.data_ptr()
-        err = _lib.calls().gtk_k9_few_rows(TYPES[x.dtype], m.data_ptr(), ld(m), w.data_ptr(), ld(w), rows, outer, inner, y.data_ptr(), _ptr(bias),
+        err = _lib.calls().gtk_k9_few_rows(TYPES[x.dtype], m.data_ptr(), ld(m), w.data_ptr(), ld(w), rows, outer, inner, y.data_ptr(), ld(y), _ptr(bias),
                                            _ptr(residual), 0 if residual is None else ld(residual), code, zp, q, qld, e, eld, stream_of(m))
         if err:
             _lib.check(err, "gtk_k9_few_rows")
@@ -207,7 +207,7 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
 
 
 def _gradients(dz: torch.Tensor, x, weight: torch.Tensor, need_dx: bool, need_dw: bool):
-    """(dz W, dz^T x) over CUDA matrices; x may be codes, or (not for ``pairs_for``) an operand already."""
+    """(dz W, dz^T x) over CUDA matrices; x may be codes."""
     rows, outer = dz.shape
     inner = weight.size(1)
     dx = dw = None
@@ -220,7 +220,7 @@ def _gradients(dz: torch.Tensor, x, weight: torch.Tensor, need_dx: bool, need_dw
         specs.append((matrix(weight), 0))
     if need_dw and pairs:
         specs.append((dz, 0))
-    if need_dw and type(x) is not Operand:
+    if need_dw:
         specs.append((x, 0))
     made = operands(pairs, *specs)
     if need_dx:
@@ -228,7 +228,7 @@ def _gradients(dz: torch.Tensor, x, weight: torch.Tensor, need_dx: bool, need_dw
         product(rows, inner, outer, made[0], False, made[1], True, dx, stream)
     if need_dw:
         dw = dz.new_empty(outer, inner)
-        a, b = (made[-2], made[-1]) if pairs else (made[0], x if type(x) is Operand else made[-1])
+        a, b = made[-2] if pairs else made[0], made[-1]
         product(outer, inner, rows, a, True, b, True, dw, stream)
     return dx, dw
 
@@ -266,7 +266,7 @@ def linear_backward(dy: torch.Tensor, x: Union[torch.Tensor, Activation8], weigh
     products = need[0] or need[1]
     db = None
     if (code and products) or need[2]:
-        dz, db = colsum(g, code, z, want_dz=bool(code and products), want_sum=need[2])
+        dz, db = colsum(g, code, z, want_dz=bool(code and products), want_sum=need[2], padded=bool(code and products))
         g = dz if code and products else g
     dx, dw = _gradients(g, x if isinstance(x, Activation8) or not need[1] else matrix(x), weight, need[0], need[1])
     return dx if dx is None or len(shape) == 2 else dx.view(shape), dw, db

@@ -346,7 +346,7 @@ def test_linear_needs_and_8_bit_input():
 # -- block ------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bits", [0, 8])
-@pytest.mark.parametrize("rows,dim,hidden", [(1, 40, 33), (35, 300, 1200), (70, 101, 203), (300, 64, 256)])
+@pytest.mark.parametrize("rows,dim,hidden", [(1, 40, 33), (35, 300, 1200), (70, 101, 203), (300, 64, 256), (400, 1500, 40), (5, 9000, 24), (3, 16400, 16)])
 def test_feed_forward_block(dtype, bits, rows, dim, hidden):
     """Against the formulas in 64 bits at the kept values.  Five roundings to the type lie between dy and a gradient
     (dz, the hidden layer or the norm's output, da, and the result's own), each of relative size u; in the 2-norm of
