@@ -141,7 +141,7 @@ struct PackItem {
   Source src;
   void* out;
   long long rows;
-  int cols, pitch, kind, vec, per;
+  int cols, pitch, kind, step, per;   // step: elements of a load (8, 4 or 1)
   unsigned strips, first;      // strips of columns; the matrix's first CTA
   unsigned int* most;          // pairs: the largest magnitudes (bits) of the rows (written) or of the columns (read)
 };
@@ -151,7 +151,21 @@ struct PackList {
   int count;
 };
 
-template <int KIND, int VEC>
+// VEC elements of a row from column c on, zeros past its end, by loads of STEP: the row's columns are whole STEPs on their
+// boundaries.  An odd row costs narrow loads, but its stores stay wide (515 x 1001 and 2047 x 1001 of f16: 6.4 us, 13.4
+// with both element by element).
+template <int STEP, typename T, int VEC>
+__device__ __forceinline__ void load_row(const T* row, int c, int cols, Vec<T, VEC>* v) {
+#pragma unroll
+  for (int j = 0; j < VEC; j += STEP) {
+    Vec<T, STEP> part = {};
+    if (c + j < cols) part = *reinterpret_cast<const Vec<T, STEP>*>(row + c + j);
+#pragma unroll
+    for (int k = 0; k < STEP; ++k) v->v[j + k] = part.v[k];
+  }
+}
+
+template <int KIND, int VEC, int STEP>
 __device__ __forceinline__ void pack_rows(const PackItem& p, unsigned block) {
   const int c = (int)((block % p.strips * 32 + threadIdx.x) * VEC);
   if (c >= p.pitch) return;
@@ -161,33 +175,34 @@ __device__ __forceinline__ void pack_rows(const PackItem& p, unsigned block) {
     if (row >= p.rows) return;
     const long long to = row * p.pitch + c;
     if constexpr (KIND == kPackCopy) {
-      Vec<uint16_t, VEC> v = {};
-      if (c < p.cols) v = *reinterpret_cast<const Vec<uint16_t, VEC>*>((const uint16_t*)p.src.p + row * p.src.ld + c);
+      Vec<uint16_t, VEC> v;
+      load_row<STEP>((const uint16_t*)p.src.p + row * p.src.ld, c, p.cols, &v);
       *reinterpret_cast<Vec<uint16_t, VEC>*>((uint16_t*)p.out + to) = v;
+    } else if constexpr (KIND == kPackPieces) {
+      Vec<float, VEC> v;
+      load_row<STEP>((const float*)p.src.p + row * p.src.ld, c, p.cols, &v);
+      float piece[3][VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        __nv_bfloat16 b[3];
+        split3(v.v[j], b);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) piece[k][j] = __bfloat162float(b[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) store_f32<__nv_bfloat16, VEC>((__nv_bfloat16*)p.out + k * stride + to, piece[k]);
     } else {
+      Vec<signed char, VEC> q;
+      load_row<STEP>((const signed char*)p.src.p + row * p.src.ld, c, p.cols, &q);
+      const float scale = c < p.cols ? block8_scale(p.src.e[row * p.src.e_ld + c / kBlock8]) : 0.f;
       float v[VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[j] = 0.f;
-      if constexpr (KIND == kPackPieces) {
-        if (c < p.cols) load_source<float, VEC>(p.src, row, c, v);
-        float left[3][VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          __nv_bfloat16 b[3];
-          split3(v[j], b);
-#pragma unroll
-          for (int k = 0; k < 3; ++k) left[k][j] = __bfloat162float(b[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < 3; ++k) store_f32<__nv_bfloat16, VEC>((__nv_bfloat16*)p.out + k * stride + to, left[k]);
+      for (int j = 0; j < VEC; ++j) v[j] = c + j < p.cols ? (float)q.v[j] * scale : 0.f;   // (a NaN's scale stays inside)
+      if constexpr (KIND == kPackCodesF16) {
+        hold_f16<VEC>(v);
+        store_f32<__half, VEC>((__half*)p.out + to, v);
       } else {
-        if (c < p.cols) load_source<signed char, VEC>(p.src, row, c, v);
-        if constexpr (KIND == kPackCodesF16) {
-          hold_f16<VEC>(v);
-          store_f32<__half, VEC>((__half*)p.out + to, v);
-        } else {
-          store_f32<__nv_bfloat16, VEC>((__nv_bfloat16*)p.out + to, v);
-        }
+        store_f32<__nv_bfloat16, VEC>((__nv_bfloat16*)p.out + to, v);
       }
     }
   }
@@ -195,11 +210,11 @@ __device__ __forceinline__ void pack_rows(const PackItem& p, unsigned block) {
 
 // Two f16 pieces of scaled f32 values.
 template <int VEC>
-__device__ __forceinline__ void store_pairs(__half* out, long long stride, const float (&v)[VEC], const float (&scale)[VEC]) {
+__device__ __forceinline__ void store_pairs(__half* out, long long stride, const Vec<float, VEC>& v, const float (&scale)[VEC]) {
   float high[VEC], low[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) {
-    const float x = v[j] * scale[j];
+    const float x = v.v[j] * scale[j];
     high[j] = __half2float(__float2half_rn(x));
     low[j] = isinf(high[j]) || isnan(high[j]) ? 0.f : x - high[j];
   }
@@ -207,21 +222,30 @@ __device__ __forceinline__ void store_pairs(__half* out, long long stride, const
   store_f32<__half, VEC>(out + stride, low);
 }
 
-// Rows scaled by their own largest magnitude: a warp takes a row of up to 1024 columns (strips 1: eight rows a CTA),
-// the CTA's eight warps one of more.
-template <int VEC>
+// Loads of a thread in flight: one of 16 bytes does not cover the memory's latency.
+constexpr int kLoads = 4;
+constexpr int kWarpRow = 2048;
+
+// Rows scaled by their own largest magnitude: a warp takes a row of up to kWarpRow columns (strips 1: eight rows a CTA),
+// the CTA's eight warps one of more; the row's second reading comes from the caches.  10000 + 700 rows of 1500: 23 us
+// (64 MB read and as many written, 5.5 TB/s); with a load at a time and a CTA to each row 38 us.
+template <int STEP>
 __device__ __forceinline__ void pack_pairs_of_rows(const PackItem& p, unsigned block, unsigned int* room) {
+  constexpr int VEC = 4;
   const bool shared = p.strips != 1;
   const long long row = shared ? block : (long long)block * kRowWarps + threadIdx.y, stride = p.rows * p.pitch;
   const int first = (int)((shared ? threadIdx.y * 32 + threadIdx.x : threadIdx.x) * VEC), step = (shared ? 256 : 32) * VEC;
   if (row >= p.rows) return;   // the whole warp, or the whole CTA
   const float* x = (const float*)p.src.p + row * p.src.ld;
   unsigned int most = 0;
-  for (int c = first; c < p.cols; c += step) {
-    float v[VEC];
-    load_f32<float, VEC>(x + c, v);
+  for (int c = first; c < p.cols; c += step * kLoads) {
+    Vec<float, VEC> v[kLoads];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+    for (int k = 0; k < kLoads; ++k) load_row<STEP>(x, c + k * step, p.cols, &v[k]);
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) most = max(most, __float_as_uint(v[k].v[j]) & 0x7fffffffu);
   }
   most = __reduce_max_sync(0xffffffffu, most);
   if (shared) {
@@ -234,52 +258,73 @@ __device__ __forceinline__ void pack_pairs_of_rows(const PackItem& p, unsigned b
   float scale[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) scale[j] = __uint_as_float((uint32_t)(pair_shift(most) + 127) << 23);
-  for (int c = first; c < p.pitch; c += step) {
-    float v[VEC];
+  __half* out = (__half*)p.out + row * p.pitch;
+  for (int c = first; c < p.pitch; c += step * kLoads) {
+    Vec<float, VEC> v[kLoads];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = 0.f;
-    if (c < p.cols) load_f32<float, VEC>(x + c, v);
-    store_pairs<VEC>((__half*)p.out + row * p.pitch + c, stride, v, scale);
+    for (int k = 0; k < kLoads; ++k) load_row<STEP>(x, c + k * step, p.cols, &v[k]);
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k)
+      if (c + k * step < p.pitch) store_pairs<VEC>(out + c + k * step, stride, v[k], scale);
   }
 }
 
-template <int VEC>
+template <int STEP>
 __device__ __forceinline__ void pack_pairs_of_columns(const PackItem& p, unsigned block) {
+  constexpr int VEC = 4;
   const int c = (int)((block % p.strips * 32 + threadIdx.x) * VEC);
   if (c >= p.pitch) return;
   const long long first = ((long long)(block / p.strips) * kRowWarps + threadIdx.y) * p.per, stride = p.rows * p.pitch;
   float scale[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) scale[j] = c + j < p.cols ? __uint_as_float((uint32_t)(pair_shift(p.most[c + j]) + 127) << 23) : 0.f;
-  for (int i = 0; i < p.per; ++i) {
-    const long long row = first + i;
-    if (row >= p.rows) return;
-    float v[VEC];
+  const int rows = (int)max(min(p.rows - first, (long long)p.per), 0ll);
+  const float* x = (const float*)p.src.p + first * p.src.ld;
+  __half* out = (__half*)p.out + first * p.pitch + c;
+  int i = 0;
+  for (; i + kLoads <= rows; i += kLoads) {
+    Vec<float, VEC> v[kLoads];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = 0.f;
-    if (c < p.cols) load_f32<float, VEC>((const float*)p.src.p + row * p.src.ld + c, v);
-    store_pairs<VEC>((__half*)p.out + row * p.pitch + c, stride, v, scale);
+    for (int k = 0; k < kLoads; ++k) load_row<STEP>(x + (i + k) * p.src.ld, c, p.cols, &v[k]);
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) store_pairs<VEC>(out + (i + k) * (long long)p.pitch, stride, v[k], scale);
+  }
+  for (; i < rows; ++i) {
+    Vec<float, VEC> v;
+    load_row<STEP>(x + i * p.src.ld, c, p.cols, &v);
+    store_pairs<VEC>(out + i * (long long)p.pitch, stride, v, scale);
   }
 }
 
 // The largest magnitudes of the columns of the list's kPackPairsOfColumns matrices, by atomic maxima over zeros: whatever
 // their order, the result is the same.
-template <int VEC>
+template <int STEP>
 __device__ __forceinline__ void column_most(const PackItem& p, unsigned block, unsigned int (*room)[32 * 4]) {
+  constexpr int VEC = 4;
   const int c = (int)((block % p.strips * 32 + threadIdx.x) * VEC);
   const long long first = ((long long)(block / p.strips) * kRowWarps + threadIdx.y) * p.per;
   unsigned int most[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) most[j] = 0;
-  if (c < p.cols)
-    for (int i = 0; i < p.per; ++i) {
-      const long long row = first + i;
-      if (row >= p.rows) break;
-      float v[VEC];
-      load_f32<float, VEC>((const float*)p.src.p + row * p.src.ld + c, v);
+  const int rows = c < p.cols ? (int)max(min(p.rows - first, (long long)p.per), 0ll) : 0;
+  const float* x = (const float*)p.src.p + first * p.src.ld;
+  auto look = [&](const Vec<float, VEC>& v) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) most[j] = max(most[j], __float_as_uint(v[j]) & 0x7fffffffu);
-    }
+    for (int j = 0; j < VEC; ++j) most[j] = max(most[j], __float_as_uint(v.v[j]) & 0x7fffffffu);
+  };
+  int i = 0;
+  for (; i + kLoads <= rows; i += kLoads) {
+    Vec<float, VEC> v[kLoads];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) load_row<STEP>(x + (i + k) * p.src.ld, c, p.cols, &v[k]);
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) look(v[k]);
+  }
+  for (; i < rows; ++i) {
+    Vec<float, VEC> v;
+    load_row<STEP>(x + i * p.src.ld, c, p.cols, &v);
+    look(v);
+  }
 #pragma unroll
   for (int j = 0; j < VEC; ++j) room[threadIdx.y][threadIdx.x * VEC + j] = most[j];
   __syncthreads();
@@ -299,16 +344,16 @@ __global__ void __launch_bounds__(256) k7_column_most(const __grid_constant__ Pa
   int k = 0;
   while (k + 1 < list.count && blockIdx.x >= list.item[k + 1].first) ++k;
   const PackItem& p = list.item[k];
-  if (p.vec == 4) column_most<4>(p, blockIdx.x - p.first, room);
+  if (p.step == 4) column_most<4>(p, blockIdx.x - p.first, room);
   else column_most<1>(p, blockIdx.x - p.first, room);
 }
 
 template <int KIND>
 __device__ __forceinline__ void pack_of(const PackItem& p, unsigned block) {
-  constexpr int wide = KIND == kPackPieces ? 4 : 8;
-  if (p.vec == wide) pack_rows<KIND, wide>(p, block);
-  else if (p.vec == 4) pack_rows<KIND, 4>(p, block);
-  else pack_rows<KIND, 1>(p, block);
+  constexpr int VEC = KIND == kPackPieces ? 4 : 8;   // of the pitch, a multiple of 8
+  if (p.step == VEC) pack_rows<KIND, VEC, VEC>(p, block);
+  else if (p.step == 4) pack_rows<KIND, VEC, 4>(p, block);
+  else pack_rows<KIND, VEC, 1>(p, block);
 }
 
 __global__ void __launch_bounds__(256) k7_pack(const __grid_constant__ PackList list) {
@@ -324,11 +369,11 @@ __global__ void __launch_bounds__(256) k7_pack(const __grid_constant__ PackList 
     case kPackCopy: pack_of<kPackCopy>(p, block); break;
     case kPackCodesF16: pack_of<kPackCodesF16>(p, block); break;
     case kPackPairsOfRows:
-      if (p.vec == 4) pack_pairs_of_rows<4>(p, block, room);
+      if (p.step == 4) pack_pairs_of_rows<4>(p, block, room);
       else pack_pairs_of_rows<1>(p, block, room);
       break;
     case kPackPairsOfColumns:
-      if (p.vec == 4) pack_pairs_of_columns<4>(p, block);
+      if (p.step == 4) pack_pairs_of_columns<4>(p, block);
       else pack_pairs_of_columns<1>(p, block);
       break;
     default: pack_of<kPackCodesBF16>(p, block); break;
@@ -591,16 +636,16 @@ extern "C" int gtk_k7_pack(gtk_addresses list, void* stream) {
     p.cols = (int)cols;
     p.pitch = (p.cols + 7) / 8 * 8;
     const bool f32 = p.kind == kPackPieces || p.kind >= kPackPairsOfRows;
-    const int elem = f32 ? 4 : p.kind == kPackCopy ? 2 : 1, wide = f32 ? 4 : 8;
-    p.vec = 1;
-    for (int vec : {wide, 4})
-      if (p.vec == 1 && p.cols % vec == 0 && aligned(p.src.p, p.src.ld, elem, vec)) p.vec = vec;
+    const int elem = f32 ? 4 : p.kind == kPackCopy ? 2 : 1, vec = f32 ? 4 : 8;
+    p.step = 1;
+    for (int step : {vec, 4})
+      if (p.step == 1 && p.cols % step == 0 && aligned(p.src.p, p.src.ld, elem, step)) p.step = step;
     p.first = (unsigned)blocks;
     if (p.kind == kPackPairsOfRows) {
-      p.strips = p.cols <= 1024 ? 1u : 2u;
+      p.strips = p.cols <= kWarpRow ? 1u : 2u;
       blocks += (unsigned long long)(p.strips == 1 ? (p.rows + kRowWarps - 1) / kRowWarps : p.rows);
     } else {
-      p.strips = (unsigned)((p.pitch + 32 * p.vec - 1) / (32 * p.vec));
+      p.strips = (unsigned)((p.pitch + 32 * vec - 1) / (32 * vec));
       unsigned y;
       if (!row_grid(p.rows, p.strips, &p.per, &y)) return GTK_ERR_UNSUPPORTED;
       blocks += (unsigned long long)p.strips * y;
