@@ -20,6 +20,12 @@ from .activation8 import Activation8, act_of, bits_of, colsum, matrix, padded_ro
 from .layer_norm import MOST_IN_BLOCK, layer_norm_backward, norm_backward_in_block
 from .layer_norm import _forward as _norm_forward
 from .linear import _check, _forward, normed, operands, pairs_for, product
+from .select import _FLOAT
+
+
+def _norm_given(weight, bias) -> None:
+    if weight is None or bias is None:
+        raise ValueError("feed_forward: the norm has a weight and a bias")
 
 
 class FeedForwardKept(NamedTuple):
@@ -39,6 +45,7 @@ def feed_forward(x: torch.Tensor, norm_weight: torch.Tensor, norm_bias: torch.Te
         raise ValueError("feed_forward: without an activation the two products are one")
     _check(x, w1, "feed_forward")
     shaped("w2", w2, w1.size(1), w1.size(0))
+    _norm_given(norm_weight, norm_bias)
     m = matrix(x)
     a, mean, rstd = _norm_forward(m, norm_weight, norm_bias, eps, True)   # operands of the next product, where they lie
     h, z = _forward(a, w1, b1, activation, None, keep, bits, True)
@@ -61,6 +68,7 @@ def feed_forward_backward(dy: torch.Tensor, kept: FeedForwardKept, norm_weight: 
     hidden, dim = w1.shape
     shape = tuple(dy.shape)
     shaped("w2", w2, dim, hidden)
+    _norm_given(norm_weight, norm_bias)
     norm_weight = parameter(dy, "norm_weight", norm_weight, dim)
     norm_bias = parameter(dy, "norm_bias", norm_bias, dim)
     if tuple(x.shape) != shape or shape[-1] != dim:
@@ -71,10 +79,12 @@ def feed_forward_backward(dy: torch.Tensor, kept: FeedForwardKept, norm_weight: 
     z = z if isinstance(z, Activation8) else matrix(z)
     if (tuple(z.q.shape) if isinstance(z, Activation8) else tuple(z.shape)) != (rows, hidden):
         raise ValueError("z has shape %s instead of %s" % (tuple(z.shape), (rows, hidden)))
-    if mean.numel() != rows or rstd.numel() != rows:
+    if mean.numel() != rows or rstd.numel() != rows or mean.device != dy.device or rstd.device != dy.device:
         raise ValueError("mean and rstd are the forward pass's, one value for each of %d rows" % rows)
     if not g.is_cuda:
         return _backward_plain(g, FeedForwardKept(x, mean.reshape(-1), rstd.reshape(-1), z), norm_weight, norm_bias, w1, w2, activation, shape)
+    if mean.dtype is not _FLOAT or rstd.dtype is not _FLOAT:
+        raise TypeError("mean and rstd are float32")
     new = dy.new_empty
     if rows == 0:
         return (new(shape), *(new(n).zero_() for n in (dim, dim, (hidden, dim), hidden, (dim, hidden), dim)))

@@ -149,6 +149,8 @@ def _check(x, weight, what):
     if weight.dim() != 2:
         raise ValueError("%s: weight is a matrix [outer, inner]" % what)
     inner = weight.size(1)
+    if not x.shape:
+        raise ValueError("%s: a scalar has no last axis" % what)
     if inner == 0 or x.shape[-1] != inner:
         raise ValueError("%s: the input's last axis has %d entries, weight is %s" % (what, x.shape[-1], tuple(weight.shape)))
 

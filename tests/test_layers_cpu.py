@@ -175,6 +175,26 @@ def test_refusals():
         FeedForward(8, 16, activation="none")
 
 
+def test_refusals_of_a_block_s_statistics_and_of_scalars():
+    x = torch.randn(4, 6)
+    p = [torch.ones(6), torch.zeros(6), torch.randn(8, 6), torch.zeros(8), torch.randn(6, 8), torch.zeros(6)]
+    with pytest.raises(ValueError):
+        linear(torch.tensor(1.0), torch.randn(5, 6))
+    for gone in (0, 1):
+        with pytest.raises(ValueError):
+            feed_forward(x, *(None if i == gone else t for i, t in enumerate(p)))
+    y, kept = feed_forward(x, *p)
+    with pytest.raises(ValueError):
+        feed_forward_backward(y, kept, None, p[1], p[2], p[4])
+    elsewhere = torch.empty(4, device="meta")
+    with pytest.raises(ValueError):
+        feed_forward_backward(y, kept._replace(mean=elsewhere), p[0], p[1], p[2], p[4])
+    with pytest.raises(ValueError):
+        feed_forward_backward(y, kept._replace(rstd=elsewhere), p[0], p[1], p[2], p[4])
+    with pytest.raises(ValueError):
+        layer_norm_backward(y, x, elsewhere, kept.rstd)
+
+
 def test_block_forward_and_backward_parts_agree_with_autograd():
     torch.manual_seed(3)
     x = torch.randn(2, 5, 40, dtype=torch.float64)
