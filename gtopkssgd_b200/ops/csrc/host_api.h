@@ -106,12 +106,11 @@ int gtk_k7_act_lines(void);
 int gtk_k7_act_backward(int type, const void* dy, long long dy_ld, const void* z, long long z_ld,
                         const unsigned char* e, long long e_ld, int act, void* dz, long long dz_ld, void* db,
                         float* partial, long long rows, long long cols, void* stream);
-long long gtk_k8_sum_lines(long long m);
 unsigned int gtk_k8_status(void);
 int gtk_k8_gemm(int type, int half, long long m, long long n, long long k, const void* a, long long a_ld, int a_pieces,
                 long long a_stride, int a_mn, const unsigned int* a_most, const void* b, long long b_ld, int b_pieces,
-                long long b_stride, int b_mn, const unsigned int* b_most, void* out, long long out_ld, const void* bias, const void* add, long long add_ld, int act, int slope,
-                void* z, long long z_ld, signed char* q, long long q_ld, unsigned char* e8, long long e_ld, void* h,
+                long long b_stride, int b_mn, const unsigned int* b_most, void* out, long long out_ld, const void* bias,
+                const void* add, long long add_ld, int act, int slope, void* z, long long z_ld, signed char* q, long long q_ld, unsigned char* e8, long long e_ld, void* h,
                 long long h_ld, float* sums, void* db, void* stream);
 int gtk_k9_few_rows(int type, const void* x, long long x_ld, const void* w, long long w_ld, long long m, long long n,
                     long long k, void* y, long long y_ld, const void* bias, const void* add, long long add_ld, int act,

@@ -59,7 +59,7 @@ constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 __device__ unsigned int g_gemm_status;   // not 0: a wait ran out (its place in the code)
 
 struct GemmShape {
-  int m, n, k;
+  int m, n;
   int tiles_m, tiles_n, blocks_k;
   int bn, stages, splits;
   int wide;                            // the epilogue's matrices have rows on boundaries of 32 bytes (2), of 16 (1) or of neither (0)
@@ -219,10 +219,6 @@ __device__ __forceinline__ int piece_products(int a_pieces, int b_pieces, uint32
   }
   if (a_pieces == 3) {
     *list = 0x012u;      // (2,0), (1,0), (0,0)
-    return 3;
-  }
-  if (b_pieces == 3) {
-    *list = 0x048u;      // (0,2), (0,1), (0,0)
     return 3;
   }
   if (a_pieces == 2) {
@@ -828,7 +824,8 @@ inline bool encode(CUtensorMap* map, const Operand& o, int half, long long rows,
 }
 
 inline bool operand_ok(const Operand& o) {
-  return o.p && (uintptr_t)o.p % 16 == 0 && o.ld > 0 && o.ld % 8 == 0 && (o.pieces == 1 || ((o.pieces == 3 || (o.pieces == 2 && o.most)) && o.piece_stride > 0 && o.piece_stride % 8 == 0));
+  return o.p && (uintptr_t)o.p % 16 == 0 && o.ld > 0 && o.ld % 8 == 0 &&
+         (o.pieces == 1 || ((o.pieces == 3 || (o.pieces == 2 && o.most)) && o.piece_stride > 0 && o.piece_stride % 8 == 0));
 }
 
 // Pairs that run side by side in clusters of `splits` of them (74, 66 and 56 of 1, 2 and 4 on B200: a cluster lies within
@@ -922,9 +919,6 @@ cudaError_t launch_gemm(int device, bool slope, int grid, size_t shared, cudaStr
 
 using namespace gtk;
 
-// Lines of n floats that `sums` has to hold for m rows.
-extern "C" long long gtk_k8_sum_lines(long long m) { return (m + 31) / 32; }
-
 // Status word of the current device's products: 0, or where a wait ran out.  Synchronises.
 extern "C" unsigned int gtk_k8_status(void) {
   unsigned int v = 0;
@@ -933,16 +927,17 @@ extern "C" unsigned int gtk_k8_status(void) {
 }
 
 // out[m][n] = epilogue(sum_k a[m][k] b[n][k]).  type: of what the epilogue reads and writes.  half: the operands are
-// f16, else bf16.  Leading dimensions and piece strides of operands are multiples of 8 elements, their addresses of
-// 16 bytes.  slope: see the top of this file.  sums with db: the sums over all rows of what the slope form stores.
+// f16, else bf16; their pieces 1 and 1, 2 and 2, 3 and 3 or 3 and 1.  Leading dimensions and piece strides of operands are multiples of 8 elements, their addresses of
+// 16 bytes.  slope: see the top of this file.  sums, room for (m + 31) / 32 lines of n, with db: the sums over all rows of what the slope form stores.
 extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long long k, const void* a, long long a_ld, int a_pieces, long long a_stride, int a_mn,
                            const unsigned int* a_most, const void* b, long long b_ld, int b_pieces, long long b_stride, int b_mn, const unsigned int* b_most,
                            void* out, long long out_ld, const void* bias,
                            const void* add, long long add_ld, int act, int slope, void* z, long long z_ld, signed char* q, long long q_ld, unsigned char* e8,
                            long long e_ld, void* h, long long h_ld, float* sums, void* db, void* stream_) {
   const Operand oa{a, a_ld, a_pieces, a_stride, a_mn != 0, a_most}, ob{b, b_ld, b_pieces, b_stride, b_mn != 0, b_most};
-  if (m <= 0 || n <= 0 || k <= 0 || !out || act < 0 || act >= kActCount || !operand_ok(oa) || !operand_ok(ob) || (q && !e8) || (q && !slope && (q_ld < (n + kBlock8 - 1) / kBlock8 * kBlock8 || q_ld % 32 || (uintptr_t)q % 32)) || (sums == nullptr) != (db == nullptr) ||
-      ((a_pieces == 2) != (b_pieces == 2)) || (a_pieces == 2 && (!half || type != kF32)) || ((a_pieces == 3 || b_pieces == 3) && (half || type != kF32)))
+  if (m <= 0 || n <= 0 || k <= 0 || !out || act < 0 || act >= kActCount || !operand_ok(oa) || !operand_ok(ob) || (q && !e8) ||
+      (q && !slope && (q_ld < (n + kBlock8 - 1) / kBlock8 * kBlock8 || q_ld % 32 || (uintptr_t)q % 32)) || (sums == nullptr) != (db == nullptr) ||
+      ((a_pieces == 2) != (b_pieces == 2)) || (a_pieces == 2 && (!half || type != kF32)) || ((a_pieces == 3 || b_pieces == 3) && (a_pieces != 3 || half || type != kF32)))
     return GTK_ERR_ARG;
   if (m > 0x7fffff00LL || n > 0x7fffff00LL || k > 0x7fffff00LL) return GTK_ERR_UNSUPPORTED;
   const DeviceInfo* info = gtk_device_info();
@@ -950,7 +945,6 @@ extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long lo
   GemmShape s{};
   s.m = (int)m;
   s.n = (int)n;
-  s.k = (int)k;
   s.a_pieces = a_pieces;
   s.b_pieces = b_pieces;
   s.a_mn = oa.mn_major;

@@ -20,7 +20,7 @@ from .select import _FLOAT, _ptr
 
 # Rows up to which K9 takes a forward pass, us on the device by K9 and by K8, whose operands have to be made first: 1500 x 6000
 # in bf16 1, 8, 20 and 32 rows 7, 8, 12 and 14 against 22, in f32 13, 13, 28 and 30 against 48; and a launch less.
-FEW_ROWS = {torch.float32: 32, torch.float16: 32, torch.bfloat16: 32}
+FEW_ROWS = 32
 
 Kept = Union[None, torch.Tensor, Activation8]
 
@@ -139,8 +139,9 @@ def product(m: int, n: int, k: int, a: Operand, a_mn: bool, b: Operand, b_mn: bo
     if db is not None:
         sums = out.new_empty(-(-m // 32), n, dtype=_FLOAT)
     err = _lib.calls().gtk_k8_gemm(TYPES[out.dtype], out.dtype is torch.float16 or a.pieces == 2, m, n, k, a.at, a.ld, a.pieces, a.stride, a_mn,
-                                   a.most or None, b.at, b.ld, b.pieces, b.stride, b_mn, b.most or None, out.data_ptr(), ld(out), _ptr(bias), _ptr(add), 0 if add is None else ld(add), activation, slope, zp,
-                                   zld, q, qld, e, eld, _ptr(h), 0 if h is None else ld(h), _ptr(sums), _ptr(db), stream)
+                                   a.most or None, b.at, b.ld, b.pieces, b.stride, b_mn, b.most or None, out.data_ptr(), ld(out), _ptr(bias), _ptr(add),
+                                   0 if add is None else ld(add), activation, slope, zp, zld, q, qld, e, eld, _ptr(h), 0 if h is None else ld(h),
+                                   _ptr(sums), _ptr(db), stream)
     if err:
         _lib.check(err, "gtk_k8_gemm")
 
@@ -189,7 +190,7 @@ def _forward(x, weight, bias, activation, residual, keep, bits, padded: bool):
         z = Activation8.empty(x, rows, outer, (rows, outer)) if bits else x.new_empty(rows, outer)
     if rows == 0 or outer == 0:
         return y if x.dim() == 2 else y.view(shape), z
-    if rows <= FEW_ROWS[x.dtype]:   # K9 reads x and W where they are
+    if rows <= FEW_ROWS:   # K9 reads x and W where they are
         w = matrix(weight)
         zp = q = e = None
         qld = eld = 0
