@@ -699,11 +699,13 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
           for (int j = 0; j < 2; ++j) {
             const int c = side * 32 + j * 64;
             if (c < s.bn) {
-              float large[32], small[32];
-              tmem_load32(lanes + (uint32_t)acc * acc_columns + (uint32_t)c, large);
-              tmem_load32(lanes + (uint32_t)acc * acc_columns + (uint32_t)(s.bn + c), small);
+              float v[32];   // (one after the other: both at once spill)
+              tmem_load32(lanes + (uint32_t)acc * acc_columns + (uint32_t)(s.bn + c), v);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) sum[j][i] += large[i] + small[i];
+              for (int i = 0; i < 32; ++i) sum[j][i] += v[i];
+              tmem_load32(lanes + (uint32_t)acc * acc_columns + (uint32_t)c, v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) sum[j][i] += v[i];
             }
           }
           tc_fence_before();
