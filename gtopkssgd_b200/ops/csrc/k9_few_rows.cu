@@ -11,7 +11,8 @@
 // A CTA takes 32 rows of W (a block of the 8-bit form): two halves of 8 warps, which take 64 of k in turn and join
 // their sums through shared memory, in order.  The next 64 of W and x are on their way meanwhile (x, too, comes from L2:
 // no two warps of a half read the same part of it).  f32: three bf16 pieces a value and the six products that count; the
-// large one is summed apart from the small ones, and both go to an f32 sum after every 64 of k, as in K8.
+// large one is summed apart from the small ones, and both go to an f32 sum after every 64 of k, as in K8.  1500 x 6000 bf16
+// (18 MB, 2.8 us at a copy's rate): 1, 8, 20 and 32 rows 7, 8, 12 and 14 us; f32 13, 13, 28 and 30.
 #include "colsum.cuh"
 #include "common.cuh"
 #include "host_api.h"

@@ -43,8 +43,8 @@ class Operand:
 # f32 operands as two scaled f16 pieces (three products) from this many multiplications a product on, as three bf16 pieces
 # (six products) below.  Forward the scales are found where the pieces are made; a backward pass's operands, scaled by
 # columns, take two launches more and are read once more.  Both ways, us a pass forward and backward: 512 x 1024 x 1024
-# 18 and 42 against 20 and 38; 2048 x 1024 x 1024 25 and 66 against 31 and 66; 700 x 1500 x 10000 111 and 246 against 132
-# and 292.
+# 18 and 42 against 21 and 39; 2048 x 1024 x 1024 24 and 70 against 32 and 67; 700 x 1500 x 10000 107 and 247 against 138
+# and 286.
 PAIRS_FROM_FORWARD = 500_000_000
 PAIRS_FROM_BACKWARD = 2_200_000_000
 
