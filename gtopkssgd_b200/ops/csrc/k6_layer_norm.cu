@@ -6,7 +6,8 @@ namespace gtk {
 template <typename T>
 int norm_forward(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, NormShape s, cudaStream_t stream) {
   const int vec = pick_vec<T>(s.cols, {{x, s.x_ld}, {w, 0}, {b, 0}, {y, s.y_ld}});
-  const NormPlan p = norm_plan(s.rows, s.cols, vec, vec * (int)sizeof(T), 32);
+  const bool async = ring_async(vec, (int)sizeof(T));
+  const NormPlan p = norm_plan(s.rows, s.cols, vec, async, 32);
   s.warps = p.warps;
   cudaError_t e = cudaSuccess;
   if (p.nv == 0) {
@@ -20,7 +21,7 @@ int norm_forward(const void* x, const void* w, const void* b, void* y, float* me
     const size_t slot = (size_t)groups * p.warps * 32 * p.nv * p.vec * sizeof(T);
     s.depth = ring_depth(slot, (size_t)kNormShared / ctas);
     const long long all = (s.rows + groups - 1) / groups, grid = all < 148LL * ctas ? all : 148LL * ctas;
-    while (s.depth > 1 && ((s.depth - 1) * grid >= all || vec * sizeof(T) < 4)) --s.depth;
+    while (s.depth > 1 && ((s.depth - 1) * grid >= all || !async)) --s.depth;
     if (!with_plan<T>(p, [&](auto V, auto N) {
           e = launch_norm<k6_norm_forward<T, decltype(V)::value, decltype(N)::value>>(grid, p.warps, groups, slot * s.depth, stream, (const T*)x, (const T*)w,
                           (const T*)b, (T*)y, mean, rstd, s);

@@ -62,12 +62,13 @@ struct RowRaw {
   Vec<T, VEC> v[NV];
 };
 
-// The rows to come.  Vectors of less than 4 bytes have no asynchronous copy: of those rows the next one waits in
-// registers (depth 1).
+// The rows to come.  Vectors of less than 4 elements or 8 bytes are not copied asynchronously, an instruction to each: of
+// those rows the next one waits in registers (depth 1).
+constexpr bool ring_async(int vec, int elem) { return vec >= 4 || vec * elem >= 8; }
 template <typename T, int VEC, int NV>
 struct RowRing {
   static constexpr int kBytes = VEC * (int)sizeof(T);
-  static constexpr bool kAsync = kBytes >= 4;
+  static constexpr bool kAsync = ring_async(VEC, (int)sizeof(T));
   uint8_t* mine;      // [depth][NV][threads of the CTA] vectors
   uint32_t stride;    // bytes between the vectors of a thread
   uint32_t slot;      // bytes of a row of all groups
@@ -529,9 +530,9 @@ inline bool divides(long long bytes, const void* p, long long ld_bytes) {
   return p == nullptr || ((uintptr_t)p % bytes == 0 && ld_bytes % bytes == 0);
 }
 
-inline NormPlan norm_plan(long long rows, int cols, int vec, int vec_bytes, int most) {
+inline NormPlan norm_plan(long long rows, int cols, int vec, bool async, int most) {
   const int vectors = (cols + vec - 1) / vec;
-  for (int each = rows >= 296 && vec_bytes >= 4 ? 16 : 8; each <= 16; each *= 2) {
+  for (int each = rows >= 296 && async ? 16 : 8; each <= 16; each *= 2) {
     const int warps = (vectors + 32 * (each / vec) - 1) / (32 * (each / vec));
     if (warps <= most) {
       int nv = 1;
@@ -564,12 +565,13 @@ bool with_plan(const NormPlan& p, F&& f) {
   };
   if (p.vec == wide) return nv(std::integral_constant<int, wide>{});
   if (sizeof(T) == 2 && p.vec == 4) return nv(std::integral_constant<int, 4>{});
+  if (p.vec == 2) return nv(std::integral_constant<int, 2>{});
   return nv(std::integral_constant<int, 1>{});
 }
 
 template <typename T>
 int pick_vec(long long cols, std::initializer_list<std::pair<const void*, long long>> bases) {
-  for (int vec : {(int)(16 / sizeof(T)), 4, 1}) {
+  for (int vec : {(int)(16 / sizeof(T)), 4, 2, 1}) {
     bool ok = cols % vec == 0;
     for (const auto& b : bases) ok = ok && divides((long long)vec * (long long)sizeof(T), b.first, b.second * (long long)sizeof(T));
     if (ok) return vec;
@@ -612,11 +614,11 @@ template <typename T, typename S, bool MORE>
 int norm_backward(const void* dy, const void* x, const float* mean, const float* rstd, const void* w, const void* add, void* dx, void* dw, void* db,
                   float* partial, NormShape s, NormMore<T> more, cudaStream_t stream) {
   int vec = pick_vec<T>(s.cols, {{w, 0}, {dy, s.dy_ld}, {add, s.add_ld}, {dx, s.cols}, {more.b, 0}, {more.y, s.y_ld}});
-  while (vec > 1 && !divides((long long)vec * (long long)sizeof(S), x, s.x_ld * (long long)sizeof(S))) vec = vec == 8 ? 4 : 1;
-  const int vec_bytes = vec * (int)(sizeof(S) < sizeof(T) ? sizeof(S) : sizeof(T));
-  NormPlan p = norm_plan(s.rows, s.cols, vec, vec_bytes, 16);   // 512 threads of 128 registers
+  while (vec > 1 && !divides((long long)vec * (long long)sizeof(S), x, s.x_ld * (long long)sizeof(S))) vec /= 2;
+  const bool async = ring_async(vec, (int)(sizeof(S) < sizeof(T) ? sizeof(S) : sizeof(T)));
+  NormPlan p = norm_plan(s.rows, s.cols, vec, async, 16);   // 512 threads of 128 registers
   const bool shared = p.nv == 0;
-  if (shared) p = norm_plan(296, s.cols, vec, 4, 32);
+  if (shared) p = norm_plan(296, s.cols, vec, true, 32);
   s.warps = p.warps;
   cudaError_t e = cudaSuccess;
   constexpr int kSums = MORE ? 3 : 2;
@@ -647,7 +649,7 @@ int norm_backward(const void* dy, const void* x, const float* mean, const float*
     const long long need = (s.rows + groups - 1) / groups;
     lines = one ? 1 : need < 2 ? 2 : need < kNormLines ? (int)need : kNormLines;
     s.depth = ring_depth(slot, kNormShared);
-    while (s.depth > 1 && ((long long)(s.depth - 1) * lines >= need || vec_bytes < 4)) --s.depth;
+    while (s.depth > 1 && ((long long)(s.depth - 1) * lines >= need || !async)) --s.depth;
     size_t dynamic = shared ? 0 : slot * s.depth;
     const size_t join = !sums ? 0 : shared ? line_bytes : (groups - 1) * line_bytes;
     dynamic = dynamic > join ? dynamic : join;
