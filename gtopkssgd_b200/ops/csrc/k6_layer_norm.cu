@@ -6,7 +6,7 @@ namespace gtk {
 template <typename T>
 int norm_forward(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, NormShape s, cudaStream_t stream) {
   const int vec = pick_vec<T>(s.cols, {{x, s.x_ld}, {w, 0}, {b, 0}, {y, s.y_ld}});
-  const bool async = ring_async(vec, (int)sizeof(T));
+  const bool async = ring_async(vec);
   const NormPlan p = norm_plan(s.rows, s.cols, vec, async, 32);
   s.warps = p.warps;
   cudaError_t e = cudaSuccess;

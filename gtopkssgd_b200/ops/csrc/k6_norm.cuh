@@ -62,13 +62,15 @@ struct RowRaw {
   Vec<T, VEC> v[NV];
 };
 
-// The rows to come.  Vectors of less than 4 elements or 8 bytes are not copied asynchronously, an instruction to each: of
-// those rows the next one waits in registers (depth 1).
-constexpr bool ring_async(int vec, int elem) { return vec >= 4 || vec * elem >= 8; }
+// The rows to come.  Vectors of less than 4 elements are not copied asynchronously, which costs an instruction each: of
+// those rows the next one waits in registers (depth 1).  7553 rows of 893 and 894 f32, forward and backward: 20 and 43, 16
+// and 30 us; with asynchronous copies 36 and 99, 20 and 47.
+constexpr bool ring_async(int vec) { return vec >= 4; }
+
 template <typename T, int VEC, int NV>
 struct RowRing {
   static constexpr int kBytes = VEC * (int)sizeof(T);
-  static constexpr bool kAsync = ring_async(VEC, (int)sizeof(T));
+  static constexpr bool kAsync = ring_async(VEC);
   uint8_t* mine;      // [depth][NV][threads of the CTA] vectors
   uint32_t stride;    // bytes between the vectors of a thread
   uint32_t slot;      // bytes of a row of all groups
@@ -615,7 +617,7 @@ int norm_backward(const void* dy, const void* x, const float* mean, const float*
                   float* partial, NormShape s, NormMore<T> more, cudaStream_t stream) {
   int vec = pick_vec<T>(s.cols, {{w, 0}, {dy, s.dy_ld}, {add, s.add_ld}, {dx, s.cols}, {more.b, 0}, {more.y, s.y_ld}});
   while (vec > 1 && !divides((long long)vec * (long long)sizeof(S), x, s.x_ld * (long long)sizeof(S))) vec /= 2;
-  const bool async = ring_async(vec, (int)(sizeof(S) < sizeof(T) ? sizeof(S) : sizeof(T)));
+  const bool async = ring_async(vec);
   NormPlan p = norm_plan(s.rows, s.cols, vec, async, 16);   // 512 threads of 128 registers
   const bool shared = p.nv == 0;
   if (shared) p = norm_plan(296, s.cols, vec, true, 32);
