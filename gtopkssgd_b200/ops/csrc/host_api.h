@@ -107,6 +107,8 @@ int gtk_k7_act_backward(int type, const void* dy, long long dy_ld, const void* z
                         const unsigned char* e, long long e_ld, int act, void* dz, long long dz_ld, void* db,
                         float* partial, long long rows, long long cols, void* stream);
 unsigned int gtk_k8_status(void);
+int gtk_k8_clear_status(void);
+int gtk_k8_rehearse_wait(unsigned long long limit_ns, unsigned int* answers, void* stream);
 int gtk_k8_gemm(int type, int half, long long m, long long n, long long k, const void* a, long long a_ld, int a_pieces,
                 long long a_stride, int a_mn, const unsigned int* a_most, const void* b, long long b_ld, int b_pieces,
                 long long b_stride, int b_mn, const unsigned int* b_most, void* out, long long out_ld, const void* bias,

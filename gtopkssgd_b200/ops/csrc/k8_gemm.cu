@@ -137,7 +137,7 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // False where the CTA has given up; then nothing may be assumed about what was waited for.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t where) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t where, uint64_t limit_ns = kWaitLimitNs) {
   uint64_t t0 = 0;
   for (uint32_t spins = 1;; ++spins) {
     if (mbar_try(bar, parity)) return true;
@@ -145,13 +145,18 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
       if (*abort) return false;
       const uint64_t t = globaltimer_ns();
       if (t0 == 0) t0 = t;
-      if (t - t0 > kWaitLimitNs) {
+      if (t - t0 > limit_ns) {
         *abort = 1;
         atomicCAS(&g_gemm_status, 0u, where);
         return false;
       }
     }
   }
+}
+// The same by a whole warp, with one answer for all its lanes: one may see the barrier complete where another gives up, and
+// a part of a warp must not go on to instructions that all of it has to execute.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t where, uint64_t limit_ns = kWaitLimitNs) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, where, limit_ns));
 }
 // Into this CTA's shared memory; `bar` may be the pair's other CTA's.
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int piece, uint32_t bar) {
@@ -717,9 +722,8 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
           for (int i = 0; i < 32; ++i) sum[j][i] = 0.f;
         for (int kb = kb_begin; kb < kb_end; kb += run, ++turn) {
           const int acc = turn & 1;
-          ok = mbar_wait(acc_full + 8u * acc, (uint32_t)(turn >> 1) & 1u, &abort, 4);
+          ok = warp_wait(acc_full + 8u * acc, (uint32_t)(turn >> 1) & 1u, &abort, 4);
           if (!ok) break;
-          __syncwarp();
           tc_fence_after();
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
@@ -749,9 +753,8 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
         }
       } else {
         const int acc = turn & 1;
-        ok = mbar_wait(acc_full + 8u * acc, (uint32_t)(turn >> 1) & 1u, &abort, 4);
+        ok = warp_wait(acc_full + 8u * acc, (uint32_t)(turn >> 1) & 1u, &abort, 4);
         if (!ok) break;
-        __syncwarp();
         tc_fence_after();
         for (int c = side * 32; c < s.bn; c += 64) {
           float v[32];
@@ -813,6 +816,23 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
   }
   tc_fence_after();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+}
+
+// A wait that runs out, by itself: the first lane of a warp waits for a barrier that is complete, the others for one on
+// which nothing arrives.  answers: what each lane is told.
+__global__ void __launch_bounds__(32) k8_rehearse_wait(unsigned long long limit_ns, unsigned int* answers) {
+  __shared__ uint64_t bars[2];
+  __shared__ volatile int abort;
+  pdl_begin(answers);
+  const uint32_t complete = smem_addr(bars), never = complete + 8u;
+  if (threadIdx.x == 0) {
+    abort = 0;
+    mbar_init(complete, 1);
+    mbar_init(never, 1);
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(complete) : "memory");
+  }
+  __syncwarp();
+  answers[threadIdx.x] = warp_wait(threadIdx.x == 0 ? complete : never, 0u, &abort, 6, limit_ns) ? 1u : 0u;
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------
@@ -952,6 +972,20 @@ extern "C" unsigned int gtk_k8_status(void) {
   unsigned int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_gemm_status, sizeof(v)) != cudaSuccess) return ~0u;
   return v;
+}
+
+// Sets the status word to 0.  Synchronises.
+extern "C" int gtk_k8_clear_status(void) {
+  const unsigned int v = 0;
+  return cudaMemcpyToSymbol(g_gemm_status, &v, sizeof(v)) == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;
+}
+
+// answers: 32 words, 1 for each lane that takes the wait for complete (see k8_rehearse_wait).
+extern "C" int gtk_k8_rehearse_wait(unsigned long long limit_ns, unsigned int* answers, void* stream) {
+  if (!answers) return GTK_ERR_ARG;
+  const cudaError_t err = launch_pdl(k8_rehearse_wait, dim3(1), dim3(32), (cudaStream_t)stream, limit_ns, answers);
+  gtk_count_launch(1);
+  return err == cudaSuccess ? GTK_OK : GTK_ERR_CUDA;
 }
 
 // out[m][n] = epilogue(sum_k a[m][k] b[n][k]).  type: of what the epilogue reads and writes.  half: the operands are

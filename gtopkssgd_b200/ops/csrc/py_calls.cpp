@@ -132,7 +132,7 @@ PyMethodDef kMethods[] = {
     GTK_METHOD(gtk_k4_finalize),      GTK_METHOD(gtk_k5_top1),
     GTK_METHOD(gtk_k6_norm_forward),  GTK_METHOD(gtk_k6_norm_backward), GTK_METHOD(gtk_k7_keep),
     GTK_METHOD(gtk_k7_restore),       GTK_METHOD(gtk_k7_pack),          GTK_METHOD(gtk_k7_act_backward),
-    GTK_METHOD(gtk_k8_gemm),          GTK_METHOD(gtk_k9_few_rows),
+    GTK_METHOD(gtk_k8_gemm),          GTK_METHOD(gtk_k8_rehearse_wait), GTK_METHOD(gtk_k9_few_rows),
     {"clear_grads", clear_grads, METH_O, nullptr},
     {"grad_addresses", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&grad_addresses)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -30,6 +30,20 @@ def status() -> int:
     return int(_lib.lib().gtk_k8_status())
 
 
+def clear_status() -> None:
+    """Sets the status to 0, after its results have been thrown away.  Synchronises."""
+    _lib.check(_lib.lib().gtk_k8_clear_status(), "gtk_k8_clear_status")
+
+
+def rehearse_timeout(device: torch.device, limit_ms: float = 50.0) -> torch.Tensor:
+    """Lets one wait run out on the device, as a product's would behind work that never ends, so that what a program does
+    about it can be tried: afterwards ``status()`` is not 0.  Returns what each of 32 lanes of the waiting warp was told, of
+    which the first waits for something that is there: 0 for all of them, as they have to go on together."""
+    answers = torch.empty(32, dtype=torch.int32, device=device)
+    _lib.check(_lib.calls().gtk_k8_rehearse_wait(int(limit_ms * 1e6), answers.data_ptr(), stream_of(answers)), "gtk_k8_rehearse_wait")
+    return answers
+
+
 class Operand:
     """A matrix as the tensor cores read it: 16-bit pieces with rows on 16-byte boundaries.  ``most``: the largest
     magnitudes that two f16 pieces were scaled by, else 0."""

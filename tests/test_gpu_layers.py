@@ -515,3 +515,17 @@ def test_language_model_with_blocks_in_a_sparse_training_step(monkeypatch):
     want = losses(0, None)
     for g, (_, _, off) in zip(got, cases):
         assert all(abs(a - b) <= off * b for a, b in zip(g[:10], want)) and g[-1] < 0.97 * g[0]
+
+
+# -- what runs out ------------------------------------------------------------------------
+def test_a_wait_that_runs_out_is_told_to_the_whole_warp():
+    """Lanes of an epilogue's warp that go on while others give up would wait for them without end: one answer for all."""
+    from gtopkssgd_b200.ops.linear import clear_status, rehearse_timeout
+    assert status() == 0
+    answers = rehearse_timeout(DEV, limit_ms=5)
+    assert answers.tolist() == [0] * 32 and status() == 6
+    clear_status()
+    x, w = _randn(70, 64), _randn(40, 64, seed=1)
+    y = linear_forward(x, w)[0]
+    _within(y, x.double() @ w.double().t(), _c(64, x.dtype) * (x.double().abs() @ w.double().abs().t()), "y")
+    assert status() == 0
