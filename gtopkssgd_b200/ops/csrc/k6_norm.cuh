@@ -27,7 +27,8 @@ constexpr int kNormMaxWarps = 32;
 
 // Sums of N values over the threads of a group of warps.  All groups of the CTA take part at the same time: a barrier
 // whose number is known only at run time makes the compiler reserve all 16, and four such CTAs fill an SM.  Scratch:
-// N floats a warp, zeros past the last warp up to a multiple of 4; used in turn, so that one barrier a sum is enough.
+// N floats a warp on a boundary of 16 bytes, zeros past the last warp up to a multiple of 4; used in turn, so that one
+// barrier a sum is enough.
 template <int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], int warps, int warp, float* scratch) {
 #pragma unroll
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(1024) k6_norm_forward(const T* x, const T* w, 
 // Rows longer than the registers hold: three passes over the row, the later two from the caches.
 template <typename T>
 __global__ void __launch_bounds__(1024) k6_norm_forward_long(const T* x, const T* w, const T* b, T* y, float* mean, float* rstd, NormShape s) {
-  __shared__ float scratch[2][kNormMaxWarps];
+  __shared__ alignas(16) float scratch[2][kNormMaxWarps];
   pdl_begin(x, w, b);
   for (long long row = blockIdx.x; row < s.rows; row += gridDim.x) {
     const T* xr = x + row * s.x_ld;
@@ -480,7 +481,7 @@ k6_norm_backward(const T* dy, const S* x, const float* mean, const float* rstd, 
 template <typename T>
 __global__ void __launch_bounds__(1024) k6_norm_backward_long(const T* dy, const T* x, const float* mean, const float* rstd, const T* w,
                                                               const T* add, T* dx, NormShape s) {
-  __shared__ float scratch[2][2][kNormMaxWarps];
+  __shared__ alignas(16) float scratch[2][2][kNormMaxWarps];
   pdl_begin(dy, x, mean, rstd, w, add);
   int turn = 0;
   for (long long row = blockIdx.x; row < s.rows; row += gridDim.x) {
