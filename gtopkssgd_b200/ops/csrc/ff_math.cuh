@@ -325,13 +325,16 @@ __device__ __forceinline__ uint32_t block8_codes(float a, float b, float c, floa
   const uint32_t ic = __float_as_uint(fmaf(c, inverse, kMagic)), id = __float_as_uint(fmaf(d, inverse, kMagic));
   return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
 }
-// What the four codes of a word stand for: byte + 128 becomes the low byte of 2^23, from which one exact multiply-add
-// takes 2^23 + 128 and scales.
+// What the four codes of a word stand for: byte + 128 becomes the low byte of 2^23, from which 2^23 + 128 is taken and the
+// rest scaled, both exactly.  (One multiply-add of what is scaled already would take it past f32's range from 2^105 on.)
 __device__ __forceinline__ void block8_values(uint32_t codes, float scale, float* v) {
   const uint32_t u = codes ^ 0x80808080u;
-  const float back = -8388736.f * scale;
+  const Two back = vset<Two>(-8388736.f), by = vset<Two>(scale);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = fmaf(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + i)), scale, back);
+  for (int i = 0; i < 4; i += 2) {
+    const Two q = two(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540 + i)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7541 + i)));
+    parts(vmul(vadd(q, back), by), v + i, v + i + 1);
+  }
 }
 __device__ __forceinline__ int block8_code(float x, uint32_t byte) {
   const int q = __float2int_rn(x * block8_inverse(byte));

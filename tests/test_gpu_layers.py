@@ -169,6 +169,46 @@ def test_gradient_through_a_kept_activation(dtype, name, rows, cols):
     _within(db, want.sum(0), 64 * EPS32 * want.abs().sum(0) + off.sum(0), "db")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [64, 70, 72, 96])
+def test_codes_of_large_values(dtype, cols):
+    """Every step up to the last, 2^122, whatever the width of a thread's loads: restored values are the codes' exactly, and
+    what is finite stays finite on the way back too (a slope of a large positive value is 1, of a negative one 0)."""
+    steps = [90, 103, 104, 105, 106, 110, 116, 121, 122]
+    x = _randn(len(steps), cols).to(dtype)
+    for i, e in enumerate(steps):
+        x[i] = (x[i] / x[i].abs().max() * 2.0 ** 6 * 0.96).double().mul(2.0 ** e).to(dtype)   # 61.4 * 2^e is the largest
+        x[i, 1], x[i, cols - 1] = 0.0, 2.0 ** e
+    kept = Activation8.keep(x)
+    q, e = oracle.keep8(x.cpu())
+    assert torch.equal(kept.q.cpu(), q) and torch.equal(kept.e.cpu(), e) and int(kept.e.max()) >= 121 + 127
+    back = kept.restore()
+    assert torch.equal(back.cpu(), oracle.restore8(q, e, dtype)) and back.isfinite().all()
+    dy = _randn(len(steps), cols, dtype=dtype, seed=2)
+    z = oracle.values8(kept.q, kept.e, torch.float64)
+    for name in ("none", "relu", "gelu", "silu"):
+        dz, db = kept.backward(dy, name)
+        want = dy.double() * oracle.act_slope(name, z)
+        _within(dz, want, 16 * EPS32 * dy.double().abs(), name)
+        _within(db, want.sum(0), 80 * EPS32 * dy.double().abs().sum(0), name)
+    # x from codes under the norm of a block's backward pass, at steps whose squares f32 does not hold
+    rows, hidden = len(steps), 40
+    mean = z.mean(1).float()
+    rstd = (1 / (z - mean.double()[:, None]).square().mean(1).sqrt()).clamp(min=2.0 ** -126).float()
+    small = _randn(rows, hidden, dtype=dtype, seed=3)
+    p = [_randn(cols, dtype=dtype, seed=4), _randn(cols, dtype=dtype, seed=5), _randn(hidden, cols, dtype=dtype, seed=6), _randn(cols, hidden, dtype=dtype, seed=7)]
+    got = feed_forward_backward(dy, FeedForwardKept(kept, mean, rstd, Activation8.keep(small)), *p, "silu")
+    g, b, w1, w2 = (t.double() for t in p)
+    h = oracle.values8(*oracle.keep8(small), torch.float64)
+    dz = (dy.double() @ w2) * oracle.act_slope("silu", h)
+    xh = (z - mean.double()[:, None]) * rstd.double()[:, None]
+    da = dz @ w1
+    limit = max(1e-5, 8 * U[dtype])
+    for have, want, what in zip(got[1:4], ((da * xh).sum(0), da.sum(0), dz.t() @ (xh * g + b)), ("dg", "db", "dw1")):
+        assert float((have.double() - want).norm()) <= limit * float(want.norm()), what
+    assert got[0].isfinite().all()
+
+
 # -- linear ---------------------------------------------------------------------------
 SHAPES = [(1, 1, 1), (1, 40, 33), (3, 7, 5), (20, 1500, 600), (64, 64, 128), (129, 65, 257), (128, 1000, 64), (515, 1001, 130), (300, 2000, 96),
           (1, 4096, 1000), (1000, 8, 1000), (257, 200, 1030)]
