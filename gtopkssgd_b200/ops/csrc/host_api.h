@@ -113,7 +113,7 @@ int gtk_k8_gemm(int type, int half, long long m, long long n, long long k, const
                 long long a_stride, int a_mn, const unsigned int* a_most, const void* b, long long b_ld, int b_pieces,
                 long long b_stride, int b_mn, const unsigned int* b_most, void* out, long long out_ld, const void* bias,
                 const void* add, long long add_ld, int act, int slope, void* z, long long z_ld, signed char* q, long long q_ld, unsigned char* e8, long long e_ld, void* h,
-                long long h_ld, float* sums, void* db, void* stream);
+                long long h_ld, float* sums, void* db, unsigned long long limit_ns, void* stream);
 int gtk_k9_few_rows(int type, const void* x, long long x_ld, const void* w, long long w_ld, long long m, long long n,
                     long long k, void* y, long long y_ld, const void* bias, const void* add, long long add_ld, int act,
                     void* z, signed char* q, long long q_ld, unsigned char* e, long long e_ld, void* stream);

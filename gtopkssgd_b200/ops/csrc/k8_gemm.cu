@@ -58,7 +58,6 @@ constexpr int kF32Blocks = 4;         // f32: blocks of k that are summed in TME
 constexpr int kMaxSplits = 4;         // pairs of a cluster: 8 CTAs are portable
 constexpr int kMaxShared = 227 * 1024;
 constexpr int kStaticShared = 2048;   // room for the kernel's static part
-constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 
 __device__ unsigned int g_gemm_status;   // not 0: a wait ran out (its place in the code)
 
@@ -70,6 +69,7 @@ struct GemmShape {
   int a_pieces, b_pieces;
   int a_mn, b_mn;                      // 1: mn-major
   uint32_t idesc;
+  unsigned long long limit_ns;         // of a wait
 };
 
 struct GemmEpilogue {
@@ -137,7 +137,7 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // False where the CTA has given up; then nothing may be assumed about what was waited for.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t where, uint64_t limit_ns = kWaitLimitNs) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t where, uint64_t limit_ns) {
   uint64_t t0 = 0;
   for (uint32_t spins = 1;; ++spins) {
     if (mbar_try(bar, parity)) return true;
@@ -155,7 +155,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 }
 // The same by a whole warp, with one answer for all its lanes: one may see the barrier complete where another gives up, and
 // a part of a warp must not go on to instructions that all of it has to execute.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t where, uint64_t limit_ns = kWaitLimitNs) {
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t where, uint64_t limit_ns) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, where, limit_ns));
 }
 // Into this CTA's shared memory; `bar` may be the pair's other CTA's.
@@ -607,7 +607,7 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
         int tm, tn;
         tile_at(s, tile, &tm, &tn);
         for (int kb = kb_begin; kb < kb_end; ++kb) {
-          ok = mbar_wait(empty + 8u * stage, phase ^ 1u, &abort, 1);
+          ok = mbar_wait(empty + 8u * stage, phase ^ 1u, &abort, 1, s.limit_ns);
           if (!ok) break;
           if (is_a && half == 0) mbar_expect(full + 8u * stage, 2u * stage_bytes);   // the pair's
           const uint32_t dst = tiles + (uint32_t)stage * stage_bytes, bar = pair_full + 8u * stage;
@@ -621,7 +621,7 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
       }
       // No copy and no arrival is left under way: the consumer has freed every stage.
       for (int i = 0; ok && i < s.stages; ++i) {
-        ok = mbar_wait(empty + 8u * stage, phase ^ 1u, &abort, 5);
+        ok = mbar_wait(empty + 8u * stage, phase ^ 1u, &abort, 5, s.limit_ns);
         if (++stage == s.stages) {
           stage = 0;
           phase ^= 1u;
@@ -648,13 +648,13 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
       for (int tile = first_tile; ok && tile < n_tiles; tile += step)
         for (int kb = kb_begin; ok && kb < kb_end; ++turn) {
           const int acc = turn & 1, stop = min(kb + run, kb_end);
-          ok = mbar_wait(acc_empty + 8u * acc, ((uint32_t)(turn >> 1) & 1u) ^ 1u, &abort, 2);
+          ok = mbar_wait(acc_empty + 8u * acc, ((uint32_t)(turn >> 1) & 1u) ^ 1u, &abort, 2, s.limit_ns);
           if (!ok) break;
           tc_fence_after();
           const uint32_t large = tmem + (uint32_t)acc * acc_columns, small = kSplit ? large + (uint32_t)s.bn : large;
           uint32_t on_large = 0, on_small = 0;   // whether the accumulator holds something already
           for (; kb < stop; ++kb) {
-            ok = mbar_wait(full + 8u * stage, phase, &abort, 3);
+            ok = mbar_wait(full + 8u * stage, phase, &abort, 3, s.limit_ns);
             if (!ok) break;
             tc_fence_after();
             const uint32_t a0 = a_desc + (uint32_t)stage * stage_step, b0 = b_desc + (uint32_t)stage * stage_step;
@@ -722,7 +722,7 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
           for (int i = 0; i < 32; ++i) sum[j][i] = 0.f;
         for (int kb = kb_begin; kb < kb_end; kb += run, ++turn) {
           const int acc = turn & 1;
-          ok = warp_wait(acc_full + 8u * acc, (uint32_t)(turn >> 1) & 1u, &abort, 4);
+          ok = warp_wait(acc_full + 8u * acc, (uint32_t)(turn >> 1) & 1u, &abort, 4, s.limit_ns);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
@@ -753,7 +753,7 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
         }
       } else {
         const int acc = turn & 1;
-        ok = warp_wait(acc_full + 8u * acc, (uint32_t)(turn >> 1) & 1u, &abort, 4);
+        ok = warp_wait(acc_full + 8u * acc, (uint32_t)(turn >> 1) & 1u, &abort, 4, s.limit_ns);
         if (!ok) break;
         tc_fence_after();
         for (int c = side * 32; c < s.bn; c += 64) {
@@ -991,11 +991,12 @@ extern "C" int gtk_k8_rehearse_wait(unsigned long long limit_ns, unsigned int* a
 // out[m][n] = epilogue(sum_k a[m][k] b[n][k]).  type: of what the epilogue reads and writes.  half: the operands are
 // f16, else bf16; their pieces 1 and 1, 2 and 2, 3 and 3 or 3 and 1.  Leading dimensions and piece strides of operands are multiples of 8 elements, their addresses of
 // 16 bytes.  slope: see the top of this file.  sums, room for (m + 31) / 32 lines of n, with db: the sums over all rows of what the slope form stores.
+// limit_ns: how long a wait lasts at most.
 extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long long k, const void* a, long long a_ld, int a_pieces, long long a_stride, int a_mn,
                            const unsigned int* a_most, const void* b, long long b_ld, int b_pieces, long long b_stride, int b_mn, const unsigned int* b_most,
                            void* out, long long out_ld, const void* bias,
                            const void* add, long long add_ld, int act, int slope, void* z, long long z_ld, signed char* q, long long q_ld, unsigned char* e8,
-                           long long e_ld, void* h, long long h_ld, float* sums, void* db, void* stream_) {
+                           long long e_ld, void* h, long long h_ld, float* sums, void* db, unsigned long long limit_ns, void* stream_) {
   const Operand oa{a, a_ld, a_pieces, a_stride, a_mn != 0, a_most}, ob{b, b_ld, b_pieces, b_stride, b_mn != 0, b_most};
   if (m <= 0 || n <= 0 || k <= 0 || !out || act < 0 || act >= kActCount || !operand_ok(oa) || !operand_ok(ob) || (q && !e8) ||
       (q && !slope && (q_ld < (n + kBlock8 - 1) / kBlock8 * kBlock8 || q_ld % 32 || (uintptr_t)q % 32)) || (sums == nullptr) != (db == nullptr) ||
@@ -1007,6 +1008,7 @@ extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long lo
   GemmShape s{};
   s.m = (int)m;
   s.n = (int)n;
+  s.limit_ns = limit_ns;
   s.a_pieces = a_pieces;
   s.b_pieces = b_pieces;
   s.a_mn = oa.mn_major;

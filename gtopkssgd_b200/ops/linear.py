@@ -13,6 +13,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 
+from .. import settings
 from . import layers_oracle as oracle
 from . import lib as _lib
 from .activation8 import TYPES, Activation8, act_of, bits_of, colsum, ld, matrix, padded_rows, parameter, same, shaped, stream_of, type_of
@@ -25,9 +26,21 @@ FEW_ROWS = 32
 Kept = Union[None, torch.Tensor, Activation8]
 
 
+_launched = False   # whether this process has launched a product
+
+
 def status() -> int:
-    """0, or where in the product's kernel a wait ran out (its results are void).  Synchronises."""
+    """0, or where in the product's kernel a wait ran out since the status was last cleared (the results of that product,
+    and what was computed from them, are void).  Of the current device.  Synchronises."""
     return int(_lib.lib().gtk_k8_status())
+
+
+def check_status() -> None:
+    """Raises GtopkNativeError where a wait of a product ran out.  ``DistributedOptimizer.check_status`` and the training
+    loops, every so many steps, do this; synchronises, and does nothing where no product was launched."""
+    where = status() if _launched else 0
+    if where:
+        raise _lib.GtopkNativeError("a linear layer's product: a wait ran out (code location %d); results since the last check are void" % where)
 
 
 def clear_status() -> None:
@@ -37,8 +50,10 @@ def clear_status() -> None:
 
 def rehearse_timeout(device: torch.device, limit_ms: float = 50.0) -> torch.Tensor:
     """Lets one wait run out on the device, as a product's would behind work that never ends, so that what a program does
-    about it can be tried: afterwards ``status()`` is not 0.  Returns what each of 32 lanes of the waiting warp was told, of
+    about it can be tried: afterwards ``status()`` is not 0 and ``check_status`` raises.  Returns what each of 32 lanes of the waiting warp was told, of
     which the first waits for something that is there: 0 for all of them, as they have to go on together."""
+    global _launched
+    _launched = True
     answers = torch.empty(32, dtype=torch.int32, device=device)
     _lib.check(_lib.calls().gtk_k8_rehearse_wait(int(limit_ms * 1e6), answers.data_ptr(), stream_of(answers)), "gtk_k8_rehearse_wait")
     return answers
@@ -140,6 +155,8 @@ def normed(src, mean, rstd, weight, bias) -> torch.Tensor:
 def product(m: int, n: int, k: int, a: Operand, a_mn: bool, b: Operand, b_mn: bool, out: torch.Tensor, stream: int, bias=None, add=None,
             activation: int = 0, slope: bool = False, z: Kept = None, h: Optional[torch.Tensor] = None, db: Optional[torch.Tensor] = None) -> None:
     """out[m, n] = epilogue(sum_k a[m, k] b[n, k]); ``a_mn``, ``b_mn``: the operand's matrix is [k, m] or [k, n]."""
+    global _launched
+    _launched = True
     sums = None
     zp = zld = q = qld = e = eld = None
     if z is None:
@@ -155,7 +172,7 @@ def product(m: int, n: int, k: int, a: Operand, a_mn: bool, b: Operand, b_mn: bo
     err = _lib.calls().gtk_k8_gemm(TYPES[out.dtype], out.dtype is torch.float16 or a.pieces == 2, m, n, k, a.at, a.ld, a.pieces, a.stride, a_mn,
                                    a.most or None, b.at, b.ld, b.pieces, b.stride, b_mn, b.most or None, out.data_ptr(), ld(out), _ptr(bias), _ptr(add),
                                    0 if add is None else ld(add), activation, slope, zp, zld, q, qld, e, eld, _ptr(h), 0 if h is None else ld(h),
-                                   _ptr(sums), _ptr(db), stream)
+                                   _ptr(sums), _ptr(db), int(settings.WAIT_LIMIT_MS * 1e6), stream)
     if err:
         _lib.check(err, "gtk_k8_gemm")
 

@@ -34,6 +34,7 @@ from typing import Optional
 import torch
 
 from .. import settings
+from ..ops import linear
 from ..ops.clip import ClipNorm
 from ..ops.sgd import SgdHyper, momentum_correct, scatter_dense, sgd_dense, sgd_sparse
 from ..settings import logger
@@ -449,8 +450,10 @@ class _DistributedOptimizer(torch.optim.Optimizer):
 
     def check_status(self):
         """Raise GTopkTimeout if a device-side wait of the last exchange ran
-        out (synchronises).  Cheap enough for every N-th iteration."""
+        out, GtopkNativeError if one of a linear layer's product did
+        (synchronises).  Cheap enough for every N-th iteration."""
         self._allreducer.check_status()
+        linear.check_status()
 
     def stop(self):
         if self._watchdog is not None:

@@ -72,6 +72,7 @@ def ssgd_dense(dnn, dataset, data_dir, nworkers, lr, batch_size, nsteps_update, 
                     trainer.update_model()
                 if i % display == 0 and use_cuda:
                     torch.cuda.synchronize()
+                    optimizer.check_status()
                 times.append(time.time() - s)
                 if i % display == 0 and i > 0:
                     t = float(np.mean(times))

@@ -28,7 +28,7 @@ from ..data import ptb_reader
 from ..data.synthetic import SyntheticAN4, SyntheticImages, SyntheticPTB
 from ..models import direct
 from ..models.lstm import repackage_hidden
-from ..ops import accuracy
+from ..ops import accuracy, linear
 from ..settings import logger
 from ..utils import create_path
 
@@ -756,6 +756,8 @@ def train_with_single(dnn, dataset, data_dir, nworkers, lr, batch_size, nsteps_u
             trainer.update_model()
             if trainer.is_cuda:
                 torch.cuda.synchronize()
+                if i % display == 0:
+                    linear.check_status()
             times.append(time.time() - s)
             if i % display == 0 and i > 0:
                 t = float(np.mean(times))

@@ -569,3 +569,21 @@ def test_a_wait_that_runs_out_is_told_to_the_whole_warp():
     y = linear_forward(x, w)[0]
     _within(y, x.double() @ w.double().t(), _c(64, x.dtype) * (x.double().abs() @ w.double().abs().t()), "y")
     assert status() == 0
+
+
+def test_a_wait_that_runs_out_reaches_the_optimizer():
+    from gtopkssgd_b200.ops.lib import GtopkNativeError
+    from gtopkssgd_b200.ops.linear import check_status, clear_status, rehearse_timeout
+    from gtopkssgd_b200.parallel.compression import compressors
+    from gtopkssgd_b200.parallel.distributed_optimizer import DistributedOptimizer
+    net = torch.nn.Linear(8, 4).to(DEV)
+    opt = DistributedOptimizer(torch.optim.SGD(net.parameters(), lr=0.1), net.named_parameters(), compression=compressors["gtopk"], is_sparse=True,
+                               density=0.1)
+    opt.check_status()
+    rehearse_timeout(DEV, limit_ms=5)
+    for check in (opt.check_status, check_status):
+        with pytest.raises(GtopkNativeError):
+            check()
+    clear_status()
+    opt.check_status()
+    opt.stop()

@@ -234,3 +234,36 @@ def test_language_model_with_feed_forward_blocks_trains_sparsely(bits):
         losses.append(float(loss.detach()))
     opt.stop()
     assert all(math.isfinite(v) for v in losses) and losses[-1] < 0.99 * losses[0]
+
+
+# -- failures -----------------------------------------------------------------------
+def test_a_product_whose_wait_ran_out_stops_the_training(monkeypatch):
+    from gtopkssgd_b200 import settings
+    from gtopkssgd_b200.ops import lib
+    from gtopkssgd_b200.ops import linear as module
+    from gtopkssgd_b200.parallel.compression import compressors
+    from gtopkssgd_b200.parallel.distributed_optimizer import DistributedOptimizer
+    net = torch.nn.Linear(8, 4)
+    opt = DistributedOptimizer(torch.optim.SGD(net.parameters(), lr=0.1), net.named_parameters(), compression=compressors["gtopk"], is_sparse=True,
+                               density=0.1)
+    word = []
+    monkeypatch.setattr(module, "status", lambda: word[0])
+    opt.check_status()                                    # no product launched: the device is not asked
+    monkeypatch.setattr(module, "_launched", True)
+    word[:] = [0]
+    opt.check_status()
+    word[:] = [4]
+    with pytest.raises(lib.GtopkNativeError, match="code location 4"):
+        opt.check_status()
+    with pytest.raises(lib.GtopkNativeError):
+        module.check_status()
+    word[:] = [0]
+    opt.stop()
+    # the limit is the framework's own, and launching says that there is something to ask for
+    calls = []
+    monkeypatch.setattr(lib, "calls", lambda: type("Calls", (), {"gtk_k8_gemm": staticmethod(lambda *a: calls.append(a) or 0)}))
+    monkeypatch.setattr(settings, "WAIT_LIMIT_MS", 125.0)
+    monkeypatch.setattr(module, "_launched", False)
+    operand = module.Operand(16, 64, 1, 0, 0, None)
+    module.product(64, 64, 64, operand, False, operand, False, torch.empty(64, 64), 0)
+    assert module._launched and calls[0][-2] == 125_000_000
