@@ -343,12 +343,20 @@ __device__ __forceinline__ int block8_code(float x, uint32_t byte) {
 
 // ---- f32 as three bf16 pieces ---------------------------------------------------------------------------------------
 // Three bf16 pieces whose sum is v to 24 bits: each is the nearest to what the ones before left.  The first is cut
-// instead of rounded where rounding would overflow; a NaN or an infinity is all in the first.
+// instead of rounded where rounding would overflow; a NaN is all in the first.  An infinity is 1, 0 and itself with its
+// sign: the last piece meets the other operand's first one only, which is zero where the operand is and has its sign
+// elsewhere, so that no infinity is multiplied by a lower piece that is zero or of the other sign.
 __device__ __forceinline__ void split3(float v, __nv_bfloat16 (&p)[3]) {
+  if (isinf(v)) {
+    p[0] = __float2bfloat16_rn(copysignf(1.f, v));
+    p[1] = __float2bfloat16_rn(0.f);
+    p[2] = __float2bfloat16_rn(v);
+    return;
+  }
   p[0] = __float2bfloat16_rn(v);
-  if (isinf(__bfloat162float(p[0])) && !isinf(v)) p[0] = __float2bfloat16_rz(v);
+  if (isinf(__bfloat162float(p[0]))) p[0] = __float2bfloat16_rz(v);
   float left = v - __bfloat162float(p[0]);
-  if (!(fabsf(v) <= 3.402823466e38f)) left = 0.f;
+  if (isnan(v)) left = 0.f;
   p[1] = __float2bfloat16_rn(left);
   p[2] = __float2bfloat16_rn(left - __bfloat162float(p[1]));
 }

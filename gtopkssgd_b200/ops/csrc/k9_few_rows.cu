@@ -86,8 +86,19 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 
 // Three bf16 pieces of two neighbours, a word each: the significand cut after 8, 16 and 24 bits, which takes a third of the
 // instructions of rounding the pieces.  What the products of pieces then leave out is 2^-22 of a product at most, 2^-24
-// on average.
+// on average.  FINITE: infinities come out as NaN; else as 1, 0 and the infinity (see split3).
+template <bool FINITE>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[3]) {
+  if constexpr (!FINITE) {
+    const bool ai = isinf(a), bi = isinf(b);
+    const float ax = a, bx = b;
+    if (ai) a = copysignf(1.f, a);
+    if (bi) b = copysignf(1.f, b);
+    split_pair<true>(a, b, w);
+    if (ai) w[2] = (w[2] & 0xffff0000u) | (__float_as_uint(ax) >> 16);
+    if (bi) w[2] = (w[2] & 0xffffu) | (__float_as_uint(bx) & 0xffff0000u);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
     w[i] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
@@ -129,19 +140,8 @@ __global__ void __launch_bounds__(kFewThreads) k9_few_rows(FewArgs g) {
     for (int t = 0; t < TOK; ++t) ax[t].load(xr[t], from, quad, g.k, t * 8 + row < rows);
   };
   const int end = n0 < g.n ? g.k : 0;   // nothing to do for rows past W's
-  int c = split * kFewChunk;
-  if (kAhead && c < end) fetch_w(c);
-  if (kXAhead && c < end) fetch_x(c);
-  for (; c < end; c += kSplits * kFewChunk) {
-    if constexpr (!kAhead) fetch_w(c);
-    if constexpr (!kXAhead) fetch_x(c);
-    const Strip<T, VEC, 16> u0 = a0, u1 = a1;
-    Strip<T, VEC, 16> x[TOK];
-#pragma unroll
-    for (int t = 0; t < TOK; ++t) x[t] = ax[t];
-    const int next = c + kSplits * kFewChunk;
-    if (kAhead && next < end) fetch_w(next);
-    if (kXAhead && next < end) fetch_x(next);
+  auto multiply = [&](const Strip<T, VEC, 16>& u0, const Strip<T, VEC, 16>& u1, const Strip<T, VEC, 16> (&x)[TOK], auto finite) {
+    constexpr bool kFinite = decltype(finite)::value;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       if constexpr (sizeof(T) == 2) {
@@ -149,15 +149,15 @@ __global__ void __launch_bounds__(kFewThreads) k9_few_rows(FewArgs g) {
         for (int t = 0; t < TOK; ++t) mma16816(large[t], u0.w[2 * s], u1.w[2 * s], u0.w[2 * s + 1], u1.w[2 * s + 1], x[t].w[2 * s], x[t].w[2 * s + 1], T{});
       } else {
         uint32_t p0[3], p1[3], p2[3], p3[3];
-        split_pair(u0.value(4 * s), u0.value(4 * s + 1), p0);
-        split_pair(u1.value(4 * s), u1.value(4 * s + 1), p1);
-        split_pair(u0.value(4 * s + 2), u0.value(4 * s + 3), p2);
-        split_pair(u1.value(4 * s + 2), u1.value(4 * s + 3), p3);
+        split_pair<kFinite>(u0.value(4 * s), u0.value(4 * s + 1), p0);
+        split_pair<kFinite>(u1.value(4 * s), u1.value(4 * s + 1), p1);
+        split_pair<kFinite>(u0.value(4 * s + 2), u0.value(4 * s + 3), p2);
+        split_pair<kFinite>(u1.value(4 * s + 2), u1.value(4 * s + 3), p3);
 #pragma unroll
         for (int t = 0; t < TOK; ++t) {
           uint32_t q0[3], q1[3];
-          split_pair(x[t].value(4 * s), x[t].value(4 * s + 1), q0);
-          split_pair(x[t].value(4 * s + 2), x[t].value(4 * s + 3), q1);
+          split_pair<kFinite>(x[t].value(4 * s), x[t].value(4 * s + 1), q0);
+          split_pair<kFinite>(x[t].value(4 * s + 2), x[t].value(4 * s + 3), q1);
 #pragma unroll
           for (int i = 2; i >= 0; --i)
 #pragma unroll
@@ -176,6 +176,39 @@ __global__ void __launch_bounds__(kFewThreads) k9_few_rows(FewArgs g) {
           total[t][i] += large[t][i] + small[t][i];
           large[t][i] = small[t][i] = 0.f;
         }
+    }
+  };
+  int c = split * kFewChunk;
+  if (kAhead && c < end) fetch_w(c);
+  if (kXAhead && c < end) fetch_x(c);
+  for (; c < end; c += kSplits * kFewChunk) {
+    if constexpr (!kAhead) fetch_w(c);
+    if constexpr (!kXAhead) fetch_x(c);
+    const Strip<T, VEC, 16> u0 = a0, u1 = a1;
+    Strip<T, VEC, 16> x[TOK];
+#pragma unroll
+    for (int t = 0; t < TOK; ++t) x[t] = ax[t];
+    const int next = c + kSplits * kFewChunk;
+    if (kAhead && next < end) fetch_w(next);
+    if (kXAhead && next < end) fetch_x(next);
+    multiply(u0, u1, x, std::true_type{});
+  }
+  if constexpr (sizeof(T) == 4) {   // a NaN may be an infinity in pieces: once more, with the pieces that keep it one
+    bool none = true;
+#pragma unroll
+    for (int t = 0; t < TOK; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) none = none && !isnan(total[t][i]);
+    if (!__all_sync(0xffffffffu, none)) {
+#pragma unroll
+      for (int t = 0; t < TOK; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) total[t][i] = 0.f;
+      for (c = split * kFewChunk; c < end; c += kSplits * kFewChunk) {
+        fetch_w(c);
+        fetch_x(c);
+        multiply(a0, a1, ax, std::false_type{});
+      }
     }
   }
 #pragma unroll

@@ -318,6 +318,49 @@ def test_linear_not_finite_stays_in_its_row(dtype):
     assert torch.equal(linear_forward(room[:, :96], w)[0][good], y[good])
 
 
+def _infinite(got, want, what):
+    assert torch.equal(got.isnan().cpu(), want.isnan().cpu()), what + ": NaN"
+    assert torch.equal(torch.where(got.isinf(), got, 0).double().cpu(), torch.where(want.isinf(), want, 0).cpu()), what + ": infinities"
+
+
+def _with_infinities(rows, cols, seed):
+    """Infinities, zeros opposite them, values with one, two and three pieces, of both signs and unequal size."""
+    m = _randn(rows, cols, seed=seed) * torch.exp(3 * _randn(rows, cols, seed=seed + 1))
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    pick = torch.rand(rows, cols, device=DEV, generator=gen)
+    m = torch.where(pick < 0.2, m.round(), torch.where(pick < 0.4, m.bfloat16().float(), m))
+    where = torch.rand(rows, cols, device=DEV, generator=gen)
+    m[where < 0.5 / cols] = math.inf
+    m[(where >= 0.5 / cols) & (where < 1 / cols)] = -math.inf
+    return m
+
+
+def _check_infinities(rows, inner, outer):
+    x, w, dy = _with_infinities(rows, inner, 1), _with_infinities(outer, inner, 3), _with_infinities(rows, outer, 5)
+    x[0, 0], w[0, 0], w[0, 1:], dy[0, 0] = math.inf, 1.0, 0.0, -math.inf
+    X, W, D = x.double(), w.double(), dy.double()
+    y = linear_forward(x, w)[0]
+    _infinite(y, X @ W.t(), "y")
+    assert y.isinf().any()
+    dx, dw, _ = linear_backward(dy, x, w)
+    _infinite(dx, D @ W, "dx")
+    _infinite(dw, D.t() @ X, "dw")
+
+
+@pytest.mark.parametrize("rows,inner,outer", [(1, 40, 33), (8, 64, 100), (20, 301, 130), (32, 128, 64), (70, 96, 130), (300, 700, 257)])
+def test_linear_f32_infinities(rows, inner, outer):
+    """An infinity times what is not zero is an infinity of its sign, though operands are multiplied in pieces."""
+    _check_infinities(rows, inner, outer)
+
+
+@pytest.mark.parametrize("rows,inner,outer", [(70, 96, 130), (300, 700, 257)])
+def test_linear_f32_infinities_by_pairs(rows, inner, outer, monkeypatch):
+    from gtopkssgd_b200.ops import linear as module
+    monkeypatch.setattr(module, "PAIRS_FROM_FORWARD", 0)
+    monkeypatch.setattr(module, "PAIRS_FROM_BACKWARD", 0)
+    _check_infinities(rows, inner, outer)
+
+
 @pytest.mark.parametrize("rows,inner,outer", [(1, 40, 33), (20, 1500, 600), (129, 65, 257), (515, 1001, 130), (1000, 8, 1000), (300, 2000, 96)])
 def test_linear_f32_by_pairs(rows, inner, outer, monkeypatch):
     """f32 operands as two scaled f16 pieces, which only large products take, at the sizes where they can go wrong.  What
