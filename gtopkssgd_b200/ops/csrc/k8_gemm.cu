@@ -8,9 +8,9 @@
 // its matrix ("k-major": x and W forward) or the outer one ("mn-major": W for dx, both for dW); the tensor cores
 // take both, so nothing is transposed in memory.  f32 operands come as three bf16 pieces a value (8 + 8 + 8 bits of
 // the significand) and are multiplied piece by piece: the six products down to 2^-18 of the largest; what is left
-// out is below 2^-26.  Or, where the products are long enough to pay for finding the largest magnitude of each row of
-// A and B, as two f16 pieces of 11 + 11 bits, scaled by a power of two so that the row's largest is just under 2^15:
-// three products, and what is left out is below 2^-24.  The tensor cores cut a sum to 24 bits where they add to it instead of rounding it, which over
+// out is below 2^-26.  Or, where a program has chosen it, as two f16 pieces of 11 + 11 bits, scaled by a power of two so
+// that the largest of each row of A and B is just under 2^15: three products, and what is left out is below 2^-24 for
+// entries down to 2^-17 of their row's largest, 2^-40 of that largest for smaller ones.  The tensor cores cut a sum to 24 bits where they add to it instead of rounding it, which over
 // the 6 * 1500 / 16 additions of K = 1500 took 1e-5 off the result (measured; f32 summed in order: 7e-7).  So the large
 // product has an accumulator apart from the five small ones, and every 256 of k both are added to f32 registers of the
 // epilogue's warps and begun again.
@@ -231,7 +231,7 @@ __device__ __forceinline__ int piece_products(int a_pieces, int b_pieces, uint32
     return 3;
   }
   if (a_pieces == 2) {
-    *list = 0x014u;      // (0,1), (1,0), (0,0); what is left out is below 2^-24
+    *list = 0x014u;      // (0,1), (1,0), (0,0)
     return 3;
   }
   *list = 0;

@@ -4,7 +4,9 @@
 ``linear_backward`` are its two directions.  y = act(x W^T + bias) + residual, x
 any shape [..., inner], weight [outer, inner] as in ``nn.Linear``; f32, f16 or bf16,
 one type for all.  Products are summed in f32.  f32 operands are multiplied as three
-bf16 pieces a value, or two scaled f16 ones, which keeps f32's accuracy.  In the 16-bit types the gradient
+bf16 pieces a value, which keeps f32's accuracy entry by entry (what is left out is 2^-22 of
+a product's magnitude at most).  A program may choose two scaled f16 pieces, which are faster and keep it
+relative to a row's largest entry only: ``PAIRS_FROM_FORWARD``.  In the 16-bit types the gradient
 dz = dy * act'(z) is rounded to the type between the products, as their operand.
 """
 from __future__ import annotations
@@ -69,17 +71,20 @@ class Operand:
         self.at, self.ld, self.pieces, self.stride, self.most, self.held = at, row, pieces, stride, most, held
 
 
-# f32 operands as two scaled f16 pieces (three products) from this many multiplications a product on, as three bf16 pieces
-# (six products) below.  Forward the scales are found where the pieces are made; a backward pass's operands, scaled by
-# columns, take two launches more and are read once more.  Both ways, us a pass forward and backward: 512 x 1024 x 1024
-# 18 and 42 against 21 and 39; 2048 x 1024 x 1024 24 and 70 against 32 and 67; 700 x 1500 x 10000 107 and 247 against 138
-# and 286.
-PAIRS_FROM_FORWARD = 500_000_000
-PAIRS_FROM_BACKWARD = 2_200_000_000
+# f32 operands as two f16 pieces (three products instead of six) from this many multiplications a product on; None: never.
+# A vector of an operand along the contracted axis (a row of x or W forward, a column of dz, x or W for the gradients that sum
+# over it) is scaled by a power of two that takes its largest magnitude M just below 2^15, and entries below 2^-17 M lose
+# bits: each is off by 2^-40 M at most, whatever its own size, and a result by that times the sum of its partners'
+# magnitudes.  Where one entry of 2^30 meets a zero weight - a masked token, an unused channel - the others' products are 1e-3
+# off, so that only a program that knows its entries can choose this.  It does from about 500_000_000 forward and
+# 2_200_000_000 backward (whose operands are scaled by columns: two launches more, and read once more).
+PAIRS_FROM_FORWARD: Optional[int] = None
+PAIRS_FROM_BACKWARD: Optional[int] = None
 
 
 def pairs_for(dtype: torch.dtype, backward: bool, m: int, n: int, k: int) -> bool:
-    return dtype is _FLOAT and m * n * k >= (PAIRS_FROM_BACKWARD if backward else PAIRS_FROM_FORWARD)
+    least = PAIRS_FROM_BACKWARD if backward else PAIRS_FROM_FORWARD
+    return least is not None and dtype is _FLOAT and m * n * k >= least
 
 
 def operands(pairs: bool, *specs) -> list:

@@ -318,6 +318,25 @@ def test_linear_not_finite_stays_in_its_row(dtype):
     assert torch.equal(linear_forward(room[:, :96], w)[0][good], y[good])
 
 
+@pytest.mark.parametrize("rows,inner,outer", [(40, 1500, 600), (512, 1024, 1024), (1100, 1500, 1400)])
+def test_linear_f32_entries_of_unequal_size(rows, inner, outer):
+    """One entry of a row may be as large as f32 holds without a loss to the others, where its partner is zero: a masked
+    token's values, an unused channel.  Every entry of a result is held to the sum of its own products' magnitudes."""
+    x, w, dy = _randn(rows, inner), _randn(outer, inner, scale=inner ** -0.5, seed=1), _randn(rows, outer, seed=2)
+    x[:, 7] = 2.0 ** 30                 # a channel of x that no weight reads
+    w[:, 7] = 0
+    w[5] *= 2.0 ** 20                   # an output that no gradient reaches
+    dy[:, 5] = 0
+    x[3] = 2.0 ** 60                    # a token that no gradient reaches
+    dy[3] = 0
+    X, W, D = x.double(), w.double(), dy.double()
+    y = linear_forward(x, w)[0]
+    dx, dw, _ = linear_backward(dy, x, w)
+    _within(y, X @ W.t(), _c(inner, x.dtype) * (X.abs() @ W.abs().t()), "y")
+    _within(dx, D @ W, _c(outer, x.dtype) * (D.abs() @ W.abs()), "dx")
+    _within(dw, D.t() @ X, _c(rows, x.dtype) * (D.abs().t() @ X.abs()), "dw")
+
+
 def _infinite(got, want, what):
     assert torch.equal(got.isnan().cpu(), want.isnan().cpu()), what + ": NaN"
     assert torch.equal(torch.where(got.isinf(), got, 0).double().cpu(), torch.where(want.isinf(), want, 0).cpu()), what + ": infinities"
