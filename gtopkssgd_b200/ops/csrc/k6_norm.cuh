@@ -316,7 +316,7 @@ k6_norm_backward(const T* dy, const S* x, const float* mean, const float* rstd, 
   int turn = 0, slot = 0;
   for (long long left = s.rows - (long long)blockIdx.x * groups; left > 0; left -= step) {   // the whole CTA
     const bool mine = row < s.rows;
-    const float r = nr, mr = -nm * nr;
+    const float r = nr, minus = -0.5f * nm, twice = 2.f * nr;
     float xh[NV][VEC], t[NV][VEC];
     V sum_t = vset<V>(0.f), sum_th = vset<V>(0.f);
     {
@@ -362,7 +362,9 @@ k6_norm_backward(const T* dy, const S* x, const float* mean, const float* rstd, 
             to_f32<T, VEC>(rg.v[i], t[i]);
 #pragma unroll
             for (int j = 0; j < kV; ++j) {
-              const V h = vfma(vget<V>(xh[i], j), vset<V>(r), vset<V>(mr)), g = vget<V>(t[i], j);
+              // (x - mean) rstd by halves, whose difference f32 always holds.  (One multiply-add of x rstd and mean rstd would
+              // leave the rounding of the latter, many times xh where the mean is many deviations.)
+              const V h = vmul(vfma(vget<V>(xh[i], j), vset<V>(0.5f), vset<V>(minus)), vset<V>(twice)), g = vget<V>(t[i], j);
               if constexpr (kShared) {
                 if (partial) {   // this thread's own columns
                   float* own = joined + c;

@@ -121,6 +121,31 @@ def test_layer_norm_special_rows():
     assert y.shape == dx.shape == (0, 1500) and not dw.any() and not db.any()
 
 
+@pytest.mark.parametrize("rows,cols", [(700, 1500), (37, 1021), (20, 64), (3, 9000)])
+@pytest.mark.parametrize("ratio", [100.0, 1e4])
+def test_layer_norm_gradients_of_rows_far_from_zero(rows, cols, ratio):
+    """Means of ``ratio`` standard deviations.  From the statistics given, x - mean is off by a rounding of its own size and
+    so is its product with rstd: xh to 3 * 2^-24 of xh, and no part of it goes by the mean's size."""
+    x = _randn(rows, cols) + ratio
+    dy, w = _randn(rows, cols, seed=1), _randn(cols, seed=2)
+    _, mean, rstd = layer_norm_forward(x, w)
+    dx, dw, db = layer_norm_backward(dy, x, mean, rstd, w)
+    r = rstd.double()[:, None]
+    xh, G, W = (x.double() - mean.double()[:, None]) * r, dy.double(), w.double()
+    t = G * W
+    want = r * (t - t.mean(1, keepdim=True) - xh * (t * xh).mean(1, keepdim=True))
+    _within(dx, want, 70 * EPS32 * r * (t.abs() + t.abs().mean(1, keepdim=True) + xh.abs() * (t * xh).abs().mean(1, keepdim=True)), "dx")
+    _within(dw, (G * xh).sum(0), 70 * EPS32 * (G * xh).abs().sum(0), "dw")
+    # in a block: the norm's output that is made again is the forward pass's
+    p = [w, _randn(cols, seed=3), _randn(24, cols, scale=cols ** -0.5, seed=4), _randn(24, seed=5), _randn(cols, 24, scale=0.2, seed=6), _randn(cols, seed=7)]
+    kept = feed_forward(x, *p)[1]
+    got = feed_forward_backward(dy, kept, *p[:3], p[4])
+    dz = (G @ p[4].double()) * oracle.act_slope("gelu", kept.z.double())
+    da = dz @ p[2].double()
+    for have, want, what in ((got[1], (da * xh).sum(0), "dg"), (got[3], dz.t() @ (xh * W + p[1].double()), "dw1")):
+        assert float((have.double() - want).norm()) <= 2e-6 * float(want.norm()), what
+
+
 # -- 8 bits ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 31), (3, 32), (5, 33), (20, 1500), (7, 1021), (700, 600), (2, 12004)])
