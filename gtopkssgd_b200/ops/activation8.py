@@ -158,6 +158,15 @@ class Activation8:
     def device(self) -> torch.device:
         return self.q.device
 
+    @staticmethod
+    def split(kept):
+        """What autograd saves of a tensor, or of one kept in 8 bits: (two tensors or None, what ``join`` needs besides)."""
+        return ((kept.q, kept.e), (kept.dtype, kept.shape)) if type(kept) is Activation8 else ((kept, None), None)
+
+    @staticmethod
+    def join(first, second, more):
+        return first if more is None else Activation8(first, second, *more)
+
     @property
     def nbytes(self) -> int:
         """Bytes that are held."""

@@ -149,15 +149,16 @@ class _FeedForward(torch.autograd.Function):
         y, kept = feed_forward(x, norm_weight, norm_bias, w1, b1, w2, b2, activation, eps, bits, need)
         if need:
             ctx.activation = activation
-            ctx.codes = (kept.x, kept.z) if bits else None
-            ctx.save_for_backward(kept.mean, kept.rstd, norm_weight, norm_bias, w1, w2, *(() if bits else (kept.x, kept.z)))
+            xs, ctx.x = Activation8.split(kept.x)
+            zs, ctx.z = Activation8.split(kept.z)
+            ctx.save_for_backward(kept.mean, kept.rstd, norm_weight, norm_bias, w1, w2, *xs, *zs)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         mean, rstd, norm_weight, norm_bias, w1, w2, *rest = ctx.saved_tensors
-        x, z = ctx.codes or rest
+        x, z = Activation8.join(*rest[:2], ctx.x), Activation8.join(*rest[2:], ctx.z)
         got = feed_forward_backward(dy, FeedForwardKept(x, mean, rstd, z), norm_weight, norm_bias, w1, w2, ctx.activation)
         return (*(g if n else None for g, n in zip(got, ctx.needs_input_grad)), None, None, None)
 

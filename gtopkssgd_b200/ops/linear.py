@@ -315,23 +315,25 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, activation, residual, bits):
         y, z = linear_forward(x, weight, bias, activation, residual, keep=any(ctx.needs_input_grad[:3]), bits=bits)
-        ctx.activation = activation
-        ctx.z = z if isinstance(z, Activation8) else None
-        kept = Activation8.keep(x) if bits and ctx.needs_input_grad[1] else None
-        ctx.x = kept if kept is not None else x.shape if bits else None
-        ctx.save_for_backward(None if bits else x, weight, None if isinstance(z, Activation8) else z)
+        ctx.activation, ctx.shape = activation, x.shape
+        if bits:   # all that is kept goes through autograd, which lets go of it behind the backward pass
+            x = Activation8.keep(x) if ctx.needs_input_grad[1] else None
+        xs, ctx.x = Activation8.split(x)
+        zs, ctx.z = Activation8.split(z)
+        ctx.save_for_backward(weight, *xs, *zs)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, z = ctx.saved_tensors
+        weight, *kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
         if any(need[:3]):
-            if x is None:   # kept in 8 bits, or not kept at all where the weight has no gradient
-                x = ctx.x if isinstance(ctx.x, Activation8) else dy.new_empty(1).expand(ctx.x)
-            dx, dw, db = linear_backward(dy, x, weight, ctx.activation, z if ctx.z is None else ctx.z, tuple(need[:3]))
+            x, z = Activation8.join(*kept[:2], ctx.x), Activation8.join(*kept[2:], ctx.z)
+            if x is None:   # not kept where the weight has no gradient
+                x = dy.new_empty(1).expand(ctx.shape)
+            dx, dw, db = linear_backward(dy, x, weight, ctx.activation, z, tuple(need[:3]))
         return dx, dw, db, None, dy if need[4] else None, None
 
 

@@ -561,6 +561,37 @@ def test_streams_graphs_and_repetition():
     assert status() == 0
 
 
+def test_what_is_kept_in_8_bits_is_let_go():
+    """The copies, 33 bytes for 32 columns or what is left of them, are held until the backward pass and no longer, though the
+    result is; hooks may move them, and what comes back without the rows' padding is read as well."""
+    def held():
+        return torch.cuda.memory_stats()["requested_bytes.all.current"]
+
+    rows, hidden = 300, 200
+    for width in (1500, 101):
+        x, p = _randn(rows, width), [_randn(width, seed=1), _randn(width, seed=2), _randn(hidden, width, scale=width ** -0.5, seed=3), _randn(hidden, seed=4),
+                                     _randn(width, hidden, scale=hidden ** -0.5, seed=5), _randn(width, seed=6)]
+        leaves = [v.requires_grad_() for v in (x, *p)]
+        copies = sum(33 * rows * -(-n // 32) for n in (width, hidden))
+        for run, more in ((lambda: linear(x, p[2], p[3], "gelu", bits=8), 0), (lambda: feed_forward_block(x, *p, "gelu", 1e-5, 8), 8 * rows)):
+            for v in leaves:
+                v.grad = None
+            run().sum().backward()
+            want = [None if v.grad is None else v.grad.clone() for v in leaves]
+            before = held()
+            y = run()
+            assert held() - before == y.untyped_storage().nbytes() + copies + more
+            y.sum().backward()      # into gradients that are there
+            assert held() - before == y.untyped_storage().nbytes()
+            for v in leaves:
+                v.grad = None
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu().contiguous(), lambda t: t.to(DEV)):
+                run().sum().backward()
+            for v, g in zip(leaves, want):
+                assert (v.grad is None) == (g is None) and (g is None or torch.allclose(v.grad, g, rtol=1e-5, atol=1e-5 * float(g.abs().max())))
+            del y
+
+
 def test_matrices_over_2_31_elements():
     """Offsets past 32 bits: the last rows of 8-bit copies, norms and products."""
     rows, cols = 70001, 32768

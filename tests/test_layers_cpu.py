@@ -236,6 +236,57 @@ def test_language_model_with_feed_forward_blocks_trains_sparsely(bits):
     assert all(math.isfinite(v) for v in losses) and losses[-1] < 0.99 * losses[0]
 
 
+# -- what autograd keeps ----------------------------------------------------------------
+def _passes(bits, device="cpu", rows=6):
+    """(linear, block) under autograd, on leaves of their own."""
+    torch.manual_seed(2)
+    x, w, b = (torch.randn(*s).to(device).requires_grad_() for s in ((rows, 40), (24, 40), (24,)))
+    p = [torch.randn(*s).to(device).requires_grad_() for s in ((rows, 40), (40,), (40,), (24, 40), (24,), (40, 24), (40,))]
+    return [(lambda: linear(x, w, b, "gelu", bits=bits), (x, w, b)), (lambda: feed_forward_block(*p, "gelu", 1e-5, bits), p)]
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("bits", [0, 8])
+def test_what_is_kept_goes_through_autograd(which, bits):
+    """Saved tensors: hooks see the 8-bit copies, may bring them back with other strides, and nothing of them outlives the
+    backward pass, though the result does."""
+    from torch.multiprocessing.reductions import StorageWeakRef
+    run, leaves = _passes(bits)[which]
+    want_y = run()
+    want_y.sum().backward()
+    want = [t.grad.clone() for t in leaves]
+    kinds, codes = [], []
+    keep = oracle.keep8
+
+    def pack(t):
+        kinds.append(t.dtype)
+        return t.clone(memory_format=torch.contiguous_format)
+
+    def watched(x):
+        pair = keep(x)
+        codes.extend(StorageWeakRef(t.untyped_storage()) for t in pair)
+        return pair
+
+    with pytest.MonkeyPatch.context() as patch:
+        patch.setattr(oracle, "keep8", watched)
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            y = run()
+        assert torch.equal(y, want_y)
+        assert kinds.count(torch.int8) == kinds.count(torch.uint8) == (2 if bits else 0)
+        assert len(codes) == (4 if bits else 0) and all(ref.expired() for ref in codes)   # the hook's copies are what is held
+        for t in leaves:
+            t.grad = None
+        y.sum().backward()
+        assert all(torch.equal(t.grad, g) for t, g in zip(leaves, want))
+        codes.clear()   # without hooks: held by the graph until the backward pass, not by the result
+        y = run()
+    assert not any(ref.expired() for ref in codes)
+    y.sum().backward()
+    assert all(ref.expired() for ref in codes) and y.grad_fn is not None
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+
+
 # -- failures -----------------------------------------------------------------------
 def test_a_product_whose_wait_ran_out_stops_the_training(monkeypatch):
     from gtopkssgd_b200 import settings
