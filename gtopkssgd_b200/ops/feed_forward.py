@@ -64,8 +64,8 @@ def feed_forward(x: torch.Tensor, norm_weight: torch.Tensor, norm_bias: torch.Te
 
 
 def feed_forward_backward(dy: torch.Tensor, kept: FeedForwardKept, norm_weight: torch.Tensor, norm_bias: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor,
-                          activation: str = "gelu"):
-    """(dx, dnorm_weight, dnorm_bias, dw1, db1, dw2, db2)."""
+                          activation: str = "gelu", need: Tuple[bool, ...] = (True,) * 7):
+    """(dx, dnorm_weight, dnorm_bias, dw1, db1, dw2, db2), each None where ``need`` says so; what only they take is left out."""
     type_of(dy, "feed_forward")
     code = act_of(activation)
     if code == 0:
@@ -87,45 +87,64 @@ def feed_forward_backward(dy: torch.Tensor, kept: FeedForwardKept, norm_weight: 
         raise ValueError("z has shape %s instead of %s" % (tuple(z.shape), (rows, hidden)))
     if mean.numel() != rows or rstd.numel() != rows or mean.device != dy.device or rstd.device != dy.device:
         raise ValueError("mean and rstd are the forward pass's, one value for each of %d rows" % rows)
+    if len(need) != 7:
+        raise ValueError("need has %d entries instead of 7" % len(need))
     if not g.is_cuda:
-        return _backward_plain(g, FeedForwardKept(x, mean.reshape(-1), rstd.reshape(-1), z), norm_weight, norm_bias, w1, w2, activation, shape)
+        got = _backward_plain(g, FeedForwardKept(x, mean.reshape(-1), rstd.reshape(-1), z), norm_weight, norm_bias, w1, w2, activation, shape)
+        return tuple(v if n else None for v, n in zip(got, need))
     if mean.dtype is not _FLOAT or rstd.dtype is not _FLOAT:
         raise TypeError("mean and rstd are float32")
     new = dy.new_empty
     if rows == 0:
-        return (new(shape), *(new(n).zero_() for n in (dim, dim, (hidden, dim), hidden, (dim, hidden), dim)))
+        zeros = (new(shape), *(new(n).zero_() for n in (dim, dim, (hidden, dim), hidden, (dim, hidden), dim)))
+        return tuple(v if n else None for v, n in zip(zeros, need))
     stream = stream_of(g)
     mean, rstd = mean.contiguous(), rstd.contiguous()
     pairs = pairs_for(dy.dtype, True, rows, hidden, dim)
-    # dz = (dy W2) act'(z) and h = act(z) again, both in the product's epilogue
-    dz, h, db1 = padded_rows(g, rows, hidden), padded_rows(g, rows, hidden), new(hidden)
-    go, w2o = operands(pairs, (g, 1), (matrix(w2), 0))
-    product(rows, hidden, dim, go, False, w2o, True, dz, stream, activation=code, slope=True, z=z, h=h, db=db1)
-    del w2o
-    dw2 = new(dim, hidden)
-    if pairs:
-        go, ho = operands(True, (g, 0), (h, 0))
-    else:
-        ho, = operands(False, (h, 0))
-    product(dim, hidden, rows, go, True, ho, True, dw2, stream)
-    del h, go, ho
-    zo, w1o, *zt = operands(pairs, (dz, 1), (matrix(w1), 0), *(((dz, 0),) if pairs else ()))
-    da = new(rows, dim)
-    product(rows, dim, hidden, zo, False, w1o, True, da, stream)
-    del w1o
+    through_norm, need_w1, need_b1, need_w2, need_b2 = any(need[:3]), *need[3:]
+    dx = dg = db = dw1 = db1 = dw2 = db2 = a = None
+    if through_norm or need_w1 or need_b1 or need_w2:
+        # dz = (dy W2) act'(z) and h = act(z) again, both in the product's epilogue (W2's gradient alone takes h from there, too)
+        dz, h = padded_rows(g, rows, hidden), padded_rows(g, rows, hidden) if need_w2 else None
+        db1 = new(hidden) if need_b1 else None
+        go, w2o = operands(pairs, (g, 1), (matrix(w2), 0))
+        product(rows, hidden, dim, go, False, w2o, True, dz, stream, activation=code, slope=True, z=z, h=h, db=db1)
+        del w2o
+        if need_w2:
+            dw2 = new(dim, hidden)
+            if pairs:
+                go, ho = operands(True, (g, 0), (h, 0))
+            else:
+                ho, = operands(False, (h, 0))
+            product(dim, hidden, rows, go, True, ho, True, dw2, stream)
+            del ho
+        del h, go
+    if through_norm or need_w1:
+        specs = [(dz, 1), (matrix(w1), 0)] if through_norm else [] if pairs else [(dz, 0)]   # (pieces of dz do both ways, pairs one)
+        if pairs and need_w1:
+            specs.append((dz, 0))
+        made = operands(pairs, *specs)
+        zt = made[-1] if pairs or not through_norm else made[0]
     xm = x if isinstance(x, Activation8) else matrix(x)
-    if dim <= MOST_IN_BLOCK:   # the norm's output again and dy's sums on the way
-        dx, dg, db, a, db2 = norm_backward_in_block(da, xm, mean, rstd, norm_weight, norm_bias, g)
-    else:
-        a = normed(xm, mean, rstd, norm_weight, norm_bias)
-        dx, dg, db = layer_norm_backward(da, x.restore().view(rows, dim) if isinstance(x, Activation8) else xm, mean, rstd, norm_weight, add=g)
+    if through_norm:
+        da = new(rows, dim)
+        product(rows, dim, hidden, made[0], False, made[1], True, da, stream)
+        if dim <= MOST_IN_BLOCK:   # the norm's output again and dy's sums on the way
+            dx, dg, db, a, db2 = norm_backward_in_block(da, xm, mean, rstd, norm_weight, norm_bias, g)
+        else:
+            dx, dg, db = layer_norm_backward(da, x.restore().view(rows, dim) if isinstance(x, Activation8) else xm, mean, rstd, norm_weight, add=g,
+                                             want_parameters=need[1] or need[2])
+        if len(shape) != 2:
+            dx = dx.view(shape)
+    if need_b2 and db2 is None:
         _, db2 = colsum(g)
-    dw1 = new(hidden, dim)
-    ao, = operands(pairs, (a, 0))
-    product(hidden, dim, rows, zt[0] if pairs else zo, True, ao, True, dw1, stream)
-    if len(shape) != 2:
-        dx = dx.view(shape)
-    return dx, dg, db, dw1, db1, dw2, db2
+    if need_w1:
+        if a is None:
+            a = normed(xm, mean, rstd, norm_weight, norm_bias)
+        dw1 = new(hidden, dim)
+        ao, = operands(pairs, (a, 0))
+        product(hidden, dim, rows, zt, True, ao, True, dw1, stream)
+    return tuple(v if n else None for v, n in zip((dx, dg, db, dw1, db1, dw2, db2), need))
 
 
 def _backward_plain(g, kept, norm_weight, norm_bias, w1, w2, activation, shape):
@@ -159,8 +178,8 @@ class _FeedForward(torch.autograd.Function):
     def backward(ctx, dy):
         mean, rstd, norm_weight, norm_bias, w1, w2, *rest = ctx.saved_tensors
         x, z = Activation8.join(*rest[:2], ctx.x), Activation8.join(*rest[2:], ctx.z)
-        got = feed_forward_backward(dy, FeedForwardKept(x, mean, rstd, z), norm_weight, norm_bias, w1, w2, ctx.activation)
-        return (*(g if n else None for g, n in zip(got, ctx.needs_input_grad)), None, None, None)
+        got = feed_forward_backward(dy, FeedForwardKept(x, mean, rstd, z), norm_weight, norm_bias, w1, w2, ctx.activation, tuple(ctx.needs_input_grad[:7]))
+        return (*got, None, None, None)
 
 
 def feed_forward_block(x: torch.Tensor, norm_weight: torch.Tensor, norm_bias: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Tensor,

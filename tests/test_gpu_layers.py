@@ -509,6 +509,41 @@ def test_feed_forward_block(dtype, bits, rows, dim, hidden):
     assert torch.equal(out, y) and all(torch.equal(v.grad, a) for v, a in zip(leaves, got))
 
 
+@pytest.mark.parametrize("dtype,bits,by_pairs", [(torch.float32, 0, False), (torch.float32, 8, True), (torch.bfloat16, 8, False)])
+@pytest.mark.parametrize("rows,dim,hidden", [(70, 101, 203), (130, 64, 96), (3, 16400, 16)])
+def test_feed_forward_block_needs(dtype, bits, by_pairs, rows, dim, hidden, monkeypatch):
+    """Any set of gradients is what it is among all of them (sums over rows and the norm's output may be made another way: two
+    roundings of the type), and what nobody wants costs no product."""
+    from gtopkssgd_b200.ops import lib
+    from gtopkssgd_b200.ops import linear as module
+    if by_pairs:
+        monkeypatch.setattr(module, "PAIRS_FROM_BACKWARD", 0)
+    x, dy = _randn(rows, dim, dtype=dtype), _randn(rows, dim, dtype=dtype, seed=7)
+    p = [_randn(dim, dtype=dtype, seed=1), _randn(dim, dtype=dtype, seed=2), _randn(hidden, dim, dtype=dtype, scale=dim ** -0.5, seed=3),
+         _randn(hidden, dtype=dtype, seed=4), _randn(dim, hidden, dtype=dtype, scale=hidden ** -0.5, seed=5), _randn(dim, dtype=dtype, seed=6)]
+    kept = feed_forward(x, *p, bits=bits)[1]
+    full = feed_forward_backward(dy, kept, *p[:3], p[4])
+    limit = max(1e-6, 4 * U[dtype])
+    for i in range(128):
+        need = tuple(bool(i >> j & 1) for j in range(7))
+        for n, a, b in zip(need, feed_forward_backward(dy, kept, *p[:3], p[4], need=need), full):
+            assert (a is None) != n and (a is None or float((a.double() - b.double()).norm()) <= limit * float(b.double().norm())), need
+
+    def products(*trained):
+        leaves = [v.clone().requires_grad_(i in trained) for i, v in enumerate((x, *p))]
+        y = feed_forward_block(*leaves, "gelu", 1e-5, bits)
+        calls = []
+        run = lib.calls()
+        with monkeypatch.context() as patch:
+            patch.setattr(lib, "calls", lambda: type("Calls", (), {"__getattr__": lambda self, name: calls.append(name) or getattr(run, name)})())
+            y.backward(dy)
+        assert all((v.grad is not None) == (i in trained) for i, v in enumerate(leaves))
+        return calls.count("gtk_k8_gemm")
+
+    assert products(*range(7)) == 4 and products(0, 1, 2) == 2 and products(0) == 2 and products(3) == 2 and products(5) == 2 and products(4) == 1
+    assert products(6) == 0
+
+
 def test_gradients_against_differences():
     """Central differences of the 64-bit function along a direction, against the f32 kernels' gradients."""
     rows, dim, hidden = 12, 48, 96

@@ -212,6 +212,21 @@ def test_block_forward_and_backward_parts_agree_with_autograd():
         assert torch.allclose(a, b, rtol=1e-10, atol=1e-12)
 
 
+def test_block_gives_the_gradients_that_are_wanted():
+    x = torch.randn(4, 6)
+    p = [torch.ones(6), torch.zeros(6), torch.randn(8, 6), torch.zeros(8), torch.randn(6, 8), torch.zeros(6)]
+    y, kept = feed_forward(x, *p)
+    full = feed_forward_backward(y, kept, *p[:3], p[4])
+    for rows in (4, 0):
+        some = FeedForwardKept(kept.x[:rows], kept.mean[:rows], kept.rstd[:rows], kept.z[:rows])
+        for i in range(128):
+            need = tuple(bool(i >> j & 1) for j in range(7))
+            got = feed_forward_backward(y[:rows], some, *p[:3], p[4], need=need)
+            assert all((a is None) != n and (a is None or a.shape == (rows, 6) or torch.equal(a, b) or not rows) for n, a, b in zip(need, got, full))
+    with pytest.raises(ValueError):
+        feed_forward_backward(y, kept, *p[:3], p[4], need=(True, True))
+
+
 @pytest.mark.parametrize("bits", [0, 8])
 def test_language_model_with_feed_forward_blocks_trains_sparsely(bits):
     from gtopkssgd_b200.parallel.compression import compressors
