@@ -163,8 +163,8 @@ def _backward_plain(g, kept, norm_weight, norm_bias, w1, w2, activation, shape):
 
 class _FeedForward(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, norm_weight, norm_bias, w1, b1, w2, b2, activation, eps, bits):
-        need = any(ctx.needs_input_grad)
+    def forward(ctx, x, norm_weight, norm_bias, w1, b1, w2, b2, activation, eps, bits, recording):
+        need = recording and any(ctx.needs_input_grad)   # (which goes by the parameters, with gradients off too)
         y, kept = feed_forward(x, norm_weight, norm_bias, w1, b1, w2, b2, activation, eps, bits, need)
         if need:
             ctx.activation = activation
@@ -179,10 +179,10 @@ class _FeedForward(torch.autograd.Function):
         mean, rstd, norm_weight, norm_bias, w1, w2, *rest = ctx.saved_tensors
         x, z = Activation8.join(*rest[:2], ctx.x), Activation8.join(*rest[2:], ctx.z)
         got = feed_forward_backward(dy, FeedForwardKept(x, mean, rstd, z), norm_weight, norm_bias, w1, w2, ctx.activation, tuple(ctx.needs_input_grad[:7]))
-        return (*got, None, None, None)
+        return (*got, None, None, None, None)
 
 
 def feed_forward_block(x: torch.Tensor, norm_weight: torch.Tensor, norm_bias: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Tensor,
                        b2: torch.Tensor, activation: str = "gelu", eps: float = 1e-5, bits: int = 0) -> torch.Tensor:
     """x + W2 act(W1 norm(x) + b1) + b2 under autograd; with ``bits=8`` x and the activation's input are kept in 8 bits."""
-    return _FeedForward.apply(x, norm_weight, norm_bias, w1, b1, w2, b2, activation, eps, bits_of(bits))
+    return _FeedForward.apply(x, norm_weight, norm_bias, w1, b1, w2, b2, activation, eps, bits_of(bits), torch.is_grad_enabled())

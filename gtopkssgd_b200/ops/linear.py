@@ -313,8 +313,11 @@ def linear_backward(dy: torch.Tensor, x: Union[torch.Tensor, Activation8], weigh
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, activation, residual, bits):
-        y, z = linear_forward(x, weight, bias, activation, residual, keep=any(ctx.needs_input_grad[:3]), bits=bits)
+    def forward(ctx, x, weight, bias, activation, residual, bits, recording):
+        # needs_input_grad goes by the parameters, with gradients off too; in here they always are
+        y, z = linear_forward(x, weight, bias, activation, residual, keep=recording and any(ctx.needs_input_grad[:3]), bits=bits)
+        if not recording:
+            return y
         ctx.activation, ctx.shape = activation, x.shape
         if bits:   # all that is kept goes through autograd, which lets go of it behind the backward pass
             x = Activation8.keep(x) if ctx.needs_input_grad[1] else None
@@ -334,11 +337,11 @@ class _Linear(torch.autograd.Function):
             if x is None:   # not kept where the weight has no gradient
                 x = dy.new_empty(1).expand(ctx.shape)
             dx, dw, db = linear_backward(dy, x, weight, ctx.activation, z, tuple(need[:3]))
-        return dx, dw, db, None, dy if need[4] else None, None
+        return dx, dw, db, None, dy if need[4] else None, None, None
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
            residual: Optional[torch.Tensor] = None, bits: int = 0) -> torch.Tensor:
     """act(x W^T + bias) + residual under autograd.  With ``bits=8`` the backward pass reads x and the activation's
     input from 8-bit copies (``Activation8``), and nothing larger of them is held."""
-    return _Linear.apply(x, weight, bias, activation, residual, bits_of(bits))
+    return _Linear.apply(x, weight, bias, activation, residual, bits_of(bits), torch.is_grad_enabled())

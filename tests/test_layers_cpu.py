@@ -302,6 +302,32 @@ def test_what_is_kept_goes_through_autograd(which, bits):
         y.sum().backward()
 
 
+@pytest.mark.parametrize("which", [0, 1])
+def test_nothing_is_kept_where_gradients_are_off(which, monkeypatch):
+    from gtopkssgd_b200.ops import feed_forward as block_module
+    from gtopkssgd_b200.ops import linear as linear_module
+    run, leaves = _passes(8)[which]
+    want = run().detach()
+    copies, asked = [], []
+    keep = oracle.keep8
+    monkeypatch.setattr(oracle, "keep8", lambda x: copies.append(x) or keep(x))
+    for module in (linear_module, block_module):
+        whole = module._forward
+        monkeypatch.setattr(module, "_forward", lambda x, w, b, act, r, kept, *rest, whole=whole: asked.append(kept) or whole(x, w, b, act, r, kept, *rest))
+    with torch.no_grad():
+        y = run()
+    with torch.inference_mode():
+        assert torch.equal(run(), want)
+    assert torch.equal(y, want) and not y.requires_grad and not copies and asked and not any(asked)
+    for t in leaves:
+        t.requires_grad_(False)
+    assert torch.equal(run(), want) and not copies and not any(asked)
+    for t in leaves:
+        t.requires_grad_()
+    run().sum().backward()
+    assert len(copies) == 2 and any(asked) and all(t.grad is not None for t in leaves)
+
+
 # -- failures -----------------------------------------------------------------------
 def test_a_product_whose_wait_ran_out_stops_the_training(monkeypatch):
     from gtopkssgd_b200 import settings
