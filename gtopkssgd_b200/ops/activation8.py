@@ -10,6 +10,7 @@ finite: in the last step, 2^122, codes stop at 63.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -82,7 +83,7 @@ def matrix(t: torch.Tensor) -> torch.Tensor:
             return t
     elif t.dim() == 0:
         raise ValueError("a scalar has no last axis")
-    m = t.reshape(-1, t.size(-1)) if t.size(-1) else t.reshape(0, 0)
+    m = t.reshape(-1, t.size(-1)) if t.size(-1) else t.reshape(math.prod(t.shape[:-1]), 0)
     return m if m.stride(1) == 1 or m.size(1) == 1 else m.contiguous()
 
 
@@ -145,10 +146,7 @@ class Activation8:
         if e.device != q.device:
             raise ValueError("codes are on %s, exponents on %s" % (q.device, e.device))
         shape = tuple(q.shape) if shape is None else tuple(shape)
-        rows = 1
-        for n in shape[:-1]:
-            rows *= n
-        if not shape or shape[-1] != q.size(1) or rows != q.size(0):
+        if not shape or shape[-1] != q.size(1) or math.prod(shape[:-1]) != q.size(0):
             raise ValueError("shape %s is not that of %d rows of %d codes" % (shape, q.size(0), q.size(1)))
         if dtype not in TYPES and not (dtype == torch.float64 and not q.is_cuda):
             raise TypeError("type %s is not supported (float32, float16, bfloat16)" % dtype)

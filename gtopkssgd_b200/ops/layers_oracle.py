@@ -74,7 +74,7 @@ def norm_backward(dy, x, mean, rstd, w, add) -> Tuple[torch.Tensor, torch.Tensor
 def keep8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(codes [rows, cols] int8, exponent bytes [rows, blocks] uint8)."""
     rows, cols = x.shape
-    v = F.pad(wide(x), (0, -cols % BLOCK)).view(rows, -1, BLOCK)
+    v = F.pad(wide(x), (0, -cols % BLOCK)).view(rows, -(-cols // BLOCK), BLOCK)
     most = v.abs().amax(2)
     bad = ~torch.isfinite(v).all(2)
     mantissa, exponent = torch.frexp(torch.where(bad, torch.ones_like(most), most))
@@ -85,15 +85,15 @@ def keep8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     q = torch.where(last, q.clamp(-63, 63), q)
     q = torch.where(bad[..., None], torch.zeros_like(q), q).to(torch.int8)
     byte = torch.where(bad, torch.full_like(e, NAN_BYTE), e + 127).to(torch.uint8)
-    return q.view(rows, -1)[:, :cols].contiguous(), byte
+    return q.flatten(1)[:, :cols].contiguous(), byte
 
 
 def values8(q: torch.Tensor, e: torch.Tensor, dtype=torch.float32) -> torch.Tensor:
     rows, cols = q.shape
-    v = F.pad(q.to(dtype), (0, -cols % BLOCK)).view(rows, -1, BLOCK)
+    v = F.pad(q.to(dtype), (0, -cols % BLOCK)).view(rows, -(-cols // BLOCK), BLOCK)
     v = torch.ldexp(v, e.int()[..., None] - 127)
     v = torch.where((e == NAN_BYTE)[..., None], torch.full_like(v, math.nan), v)
-    return v.view(rows, -1)[:, :cols].contiguous()
+    return v.flatten(1)[:, :cols].contiguous()
 
 
 def restore8(q: torch.Tensor, e: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

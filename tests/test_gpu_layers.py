@@ -655,6 +655,11 @@ def test_matrices_over_2_31_elements():
     assert float((dw[-64:] - want).norm() / want.norm()) < 1e-2
 
 
+def test_empty_axes_on_the_gpu():
+    from test_layers_cpu import _check_empty
+    _check_empty(DEV)
+
+
 def test_refusals_on_the_gpu():
     x, w = _randn(8, 64), _randn(16, 64)
     with pytest.raises(TypeError):

@@ -115,6 +115,33 @@ def test_shapes_lengths_and_strides():
     assert kept.shape == x.shape and kept.restore().shape == x.shape
 
 
+def _check_empty(device):
+    for shape in ((0, 3), (5, 0), (2, 3, 0), (0, 3, 0), (3, 0, 4), (0,), (0, 0)):
+        x = torch.zeros(shape, device=device)
+        kept = Activation8.keep(x)
+        assert kept.restore().shape == x.shape and kept.shape == x.shape
+        dz, db = kept.backward(x, "gelu")
+        assert dz.shape == x.shape and db.shape == shape[-1:] and not db.any()
+    for shape in ((0, 8), (3, 0, 8), (0, 3, 8)):
+        x = torch.zeros(shape, device=device, requires_grad=True)
+        p = [torch.ones(n, device=device, requires_grad=True) for n in (8, 8, (5, 8), 5, (8, 5), 8)]
+        for bits in (0, 8):
+            y = linear(x, p[2], p[3], "gelu", bits=bits)
+            z = feed_forward_block(x, *p, "gelu", 1e-5, bits)
+            assert y.shape == (*shape[:-1], 5) and z.shape == shape
+            (y.sum() + z.sum()).backward()
+        assert x.grad.shape == shape and not any(t.grad.any() for t in p)
+    w = torch.zeros(0, 8, device=device)
+    y, z = linear_forward(torch.ones(3, 8, device=device), w, activation="gelu", keep=True, bits=8)
+    assert y.shape == z.shape == (3, 0)
+    dx, dw, db = linear_backward(y, torch.ones(3, 8, device=device), w, "gelu", z)
+    assert dx.shape == (3, 8) and not dx.any() and dw.shape == (0, 8) and db.shape == (0,)
+
+
+def test_empty_axes():
+    _check_empty("cpu")
+
+
 def test_refusals():
     x, w, b = torch.randn(4, 6), torch.randn(5, 6), torch.randn(5)
     with pytest.raises(TypeError):
