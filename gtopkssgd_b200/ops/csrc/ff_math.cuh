@@ -231,9 +231,9 @@ __device__ __forceinline__ V act_slope(V z, V* value) {
     const V s = sigmoid(tanh_argument(z), 1.f);
     const V h = vmul(z, s);
     *value = h;
-    // s + h (1 - s) du, du = 2 sqrt(2 / pi) (1 + 3 c z^2)
-    const V du = vfma(vmul(z, z), vset<V>(6.f * kSqrt2OverPi * kGeluCubic), vset<V>(2.f * kSqrt2OverPi));
-    return vfma(vmul(h, vfma(s, vset<V>(-1.f), vset<V>(1.f))), du, s);
+    // s + t du, t = h (1 - s), du = 2 sqrt(2 / pi) (1 + 3 c z^2); t first, which is 0 before z^2 leaves f32's range
+    const V t = vmul(h, vfma(s, vset<V>(-1.f), vset<V>(1.f)));
+    return vfma(vmul(vmul(t, z), z), vset<V>(6.f * kSqrt2OverPi * kGeluCubic), vfma(t, vset<V>(2.f * kSqrt2OverPi), s));
   }
   if constexpr (ACT == kActSilu) {
     const V s = sigmoid(z, 1.f);

@@ -43,7 +43,8 @@ def act_slope(name: str, z: torch.Tensor) -> torch.Tensor:
     if name == "gelu_tanh":
         c = math.sqrt(2 / math.pi)
         th = torch.tanh(c * (z + 0.044715 * z ** 3))
-        return 0.5 * (1 + th) + 0.5 * z * (1 - th * th) * c * (1 + 3 * 0.044715 * z * z)
+        t = z * (1 - th * th)      # 0 before z^2 leaves the type's range
+        return 0.5 * (1 + th) + 0.5 * c * (t + 3 * 0.044715 * (t * z * z))
     sg = torch.sigmoid(z)
     return sg * (1 + z * (1 - sg))
 

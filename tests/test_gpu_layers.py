@@ -234,6 +234,19 @@ def test_codes_of_large_values(dtype, cols):
     assert got[0].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("name", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_slopes_of_large_values(dtype, name):
+    """1 and 0, also where the square of z is past f32's range."""
+    from gtopkssgd_b200.ops.activation8 import ACTIVATIONS, colsum
+    z = torch.tensor([1e19, 2e19, 1e25, 3e38, 400.0], device=DEV).repeat_interleave(32)      # a block of 32 each
+    z = torch.stack([z, -z]).to(dtype)
+    dy = _randn(2, 160, dtype=dtype)
+    want = torch.stack([dy[0], torch.zeros_like(dy[1])])
+    for got in (Activation8.keep(z).backward(dy, name)[0], colsum(dy, ACTIVATIONS[name], z, want_dz=True)[0]):
+        assert torch.equal(got, want)
+
+
 # -- linear ---------------------------------------------------------------------------
 SHAPES = [(1, 1, 1), (1, 40, 33), (3, 7, 5), (20, 1500, 600), (64, 64, 128), (129, 65, 257), (128, 1000, 64), (515, 1001, 130), (300, 2000, 96),
           (1, 4096, 1000), (1000, 8, 1000), (257, 200, 1030)]

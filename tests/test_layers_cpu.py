@@ -30,6 +30,12 @@ def test_activations_and_slopes(name):
     assert torch.allclose(oracle.act_slope(name, z), slope, rtol=1e-12, atol=1e-14)
 
 
+@pytest.mark.parametrize("name", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_slopes_of_large_values(name):
+    z = torch.tensor([1e19, 2e19, 1e25, 3e38, 400.0])
+    assert torch.equal(oracle.act_slope(name, z), torch.ones(5)) and torch.equal(oracle.act_slope(name, -z), torch.zeros(5))
+
+
 def test_gradients_against_differences():
     torch.manual_seed(0)
     assert torch.autograd.gradcheck(lambda *a: layer_norm(*a), (_leaf(3, 2, 7), _leaf(7), _leaf(7)))
