@@ -989,7 +989,7 @@ extern "C" int gtk_k8_rehearse_wait(unsigned long long limit_ns, unsigned int* a
 }
 
 // out[m][n] = epilogue(sum_k a[m][k] b[n][k]).  type: of what the epilogue reads and writes.  half: the operands are
-// f16, else bf16; their pieces 1 and 1, 2 and 2, 3 and 3 or 3 and 1.  Leading dimensions and piece strides of operands are multiples of 8 elements, their addresses of
+// f16, else bf16; their pieces 1 and 1 in the 16-bit types, 2 and 2, 3 and 3 or 3 and 1 in f32.  Leading dimensions and piece strides of operands are multiples of 8 elements, their addresses of
 // 16 bytes.  slope: see the top of this file.  sums, room for (m + 31) / 32 lines of n, with db: the sums over all rows of what the slope form stores.
 // limit_ns: how long a wait lasts at most.
 extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long long k, const void* a, long long a_ld, int a_pieces, long long a_stride, int a_mn,
@@ -1000,7 +1000,8 @@ extern "C" int gtk_k8_gemm(int type, int half, long long m, long long n, long lo
   const Operand oa{a, a_ld, a_pieces, a_stride, a_mn != 0, a_most}, ob{b, b_ld, b_pieces, b_stride, b_mn != 0, b_most};
   if (m <= 0 || n <= 0 || k <= 0 || !out || act < 0 || act >= kActCount || !operand_ok(oa) || !operand_ok(ob) || (q && !e8) ||
       (q && !slope && (q_ld < (n + kBlock8 - 1) / kBlock8 * kBlock8 || q_ld % 32 || (uintptr_t)q % 32)) || (sums == nullptr) != (db == nullptr) ||
-      ((a_pieces == 2) != (b_pieces == 2)) || (a_pieces == 2 && (!half || type != kF32)) || ((a_pieces == 3 || b_pieces == 3) && (a_pieces != 3 || half || type != kF32)))
+      ((a_pieces == 2) != (b_pieces == 2)) || (a_pieces == 2 && (!half || type != kF32)) || ((a_pieces == 3 || b_pieces == 3) && (a_pieces != 3 || half || type != kF32)) ||
+      (type == kF32 && a_pieces == 1))   // (f32 has an accumulator for lower pieces, which then nothing would write)
     return GTK_ERR_ARG;
   if (m > 0x7fffff00LL || n > 0x7fffff00LL || k > 0x7fffff00LL) return GTK_ERR_UNSUPPORTED;
   const DeviceInfo* info = gtk_device_info();

@@ -673,6 +673,21 @@ def test_empty_axes_on_the_gpu():
     _check_empty(DEV)
 
 
+def test_products_of_no_known_form_are_refused():
+    """By the host, before anything is launched: f32 results have pieces, pairs their scales, and both operands fit."""
+    from gtopkssgd_b200.ops import lib
+    a, out = torch.zeros(64, 64, dtype=torch.bfloat16, device=DEV), torch.full((64, 64), 7.0, device=DEV)
+
+    def call(code, half, pieces, n=64, ld=64):
+        at = a.data_ptr()
+        return lib.calls().gtk_k8_gemm(code, half, 64, n, 64, at, ld, pieces[0], 0, 0, None, at, ld, pieces[1], 0, 0, None, out.data_ptr(), 64, None, None, 0,
+                                       0, 0, None, 0, None, 0, None, 0, None, 0, None, None, 10 ** 9, torch.cuda.current_stream().cuda_stream)
+
+    for args in ((0, 0, (1, 1)), (0, 1, (1, 1)), (0, 1, (2, 2)), (0, 0, (1, 3)), (0, 0, (3, 3)), (2, 0, (3, 1)), (0, 1, (2, 1)), (2, 0, (1, 1), 0), (2, 0, (1, 1), 64, 60)):
+        assert call(*args) == -1, args
+    assert bool((out == 7).all()) and status() == 0
+
+
 def test_refusals_on_the_gpu():
     x, w = _randn(8, 64), _randn(16, 64)
     with pytest.raises(TypeError):
