@@ -2,7 +2,7 @@
 ``_gtk_calls`` that calls its launch entry points.
 
 Every kernel file is plain CUDA with an ``extern "C"`` launcher, so nothing
-here needs the PyTorch headers and a full rebuild takes seconds.  The library
+here needs the PyTorch headers and a full rebuild takes a minute.  The library
 is written next to this file; a digest of the sources is stored beside it so
 that an up-to-date library is never rebuilt (the GPU box receives the built
 file together with the sources).

@@ -11,8 +11,8 @@
 // With 8 elements a thread the work per thread and row - sums across lanes and warps, addresses - took 37
 // instructions an element forward and 70 backward, and their issue, not memory, set the time.  In the backward pass the column sums of
 // a thread's own columns stay in its registers all along, the groups of a CTA join theirs in shared memory, and
-// col_finish adds up one line per CTA.  16384 x 4096 bf16: forward 72 us (3.7 TB/s, 64 % of the issue slots), backward 118
-// (3.4 TB/s, 59 %): instructions for unpacking and addresses still weigh as much as memory.  700 x 1500 f32: 4.6 and 12 us
+// col_finish adds up one line per CTA.  16384 x 4096 bf16: forward 72 us (3.7 TB/s, 64 % of the issue slots), backward 122
+// (3.3 TB/s, 59 %): instructions for unpacking and addresses still weigh as much as memory.  700 x 1500 f32: 4.6 and 12 us
 // with col_finish.
 #include <atomic>
 

@@ -7,7 +7,7 @@
 //
 // Bound by memory.  A warp takes 32 * VEC neighbouring columns of a row, so that a block of 32 lies in 32 / VEC
 // neighbouring lanes and its maximum takes log2(32 / VEC) shuffles; eight warps of a CTA take rows in turn.  16384 x 8192
-// bf16 (a copy: 6.5 TB/s): keep 69 us (5.8 TB/s), restore 76 (5.3), act_backward from 8 bits 140 (4.8; the activation's
+// bf16 (a copy: 6.5 TB/s): keep 69 us (5.8 TB/s), restore 79 (5.1), act_backward from 8 bits 139 (4.8; the activation's
 // instructions, 61 % of the issue slots), from bf16 142 (5.7), the sums alone 45 (6.0).
 #include "colsum.cuh"
 #include "common.cuh"

@@ -29,8 +29,9 @@
 // a padded buffer in shared memory, so that a warp's accesses run along rows.
 //
 // 8192 x 2048 x 8192 bf16: forward 181 to 190 us (1.45 to 1.52 PFLOP/s, under the power cap), with gelu and its 8-bit input 200 to
-// 216, the input gradient and the weight's 200 to 245 (256 tiles are 3.5 rounds of the 74 pairs); 700 x 1500 x 10000 f32 as
-// pairs 75 us (0.84 PFLOP/s of f16 products: shared memory, read for three products of 128 columns and written, is full).
+// 216, the input gradient and the weight's 200 to 245 (256 tiles are 3.5 rounds of the 74 pairs); 700 x 1500 x 10000 f32
+// 107 us of three pieces (0.59 PFLOP/s of bf16 products), as pairs 75 us (0.84 PFLOP/s of f16 products): shared memory, read
+// for the products of 128 columns and written, is full.
 //
 // Every wait ends: after a time limit the waiter raises the CTA's abort flag and the status word, everybody leaves
 // after its copies and products in flight, and TMEM is freed.

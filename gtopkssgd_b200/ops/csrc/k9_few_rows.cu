@@ -2,7 +2,7 @@
 //
 //   z = x W^T + b ; y = act(z) + r ; z kept in its type or in 8 bits
 //
-// Bound by the bytes of W, each read once, and by latency.  A tile of a matrix product for 256 rows would wait for its
+// Bound by the bytes of W, each read once (f32 above 16 rows: twice, for 16 rows of x each), and by latency.  A tile of a matrix product for 256 rows would wait for its
 // few useful rows as long as for all, and wants rows of W on 16-byte boundaries; here W goes from memory to registers
 // at any alignment and to the tensor cores by mma.sync, whose rate is of no account: W's rows are its rows, x's rows
 // its columns.  Which element of the contracted axis stands at which place of a fragment is free as long as both
@@ -12,7 +12,8 @@
 // their sums through shared memory, in order.  The next 64 of W and x are on their way meanwhile (x, too, comes from L2:
 // no two warps of a half read the same part of it).  f32: three bf16 pieces a value and the six products that count; the
 // large one is summed apart from the small ones, and both go to an f32 sum after every 64 of k, as in K8.  1500 x 6000 bf16
-// (18 MB, 2.8 us at a copy's rate): 1, 8, 20 and 32 rows 7, 8, 12 and 14 us; f32 13, 13, 28 and 30.
+// (18 MB, 2.8 us at a copy's rate): 1, 8, 20 and 32 rows 7, 8, 12 and 14 us; f32 12, 13, 27 and 29 (164 bytes of spills
+// above 8 rows).
 #include "colsum.cuh"
 #include "common.cuh"
 #include "host_api.h"
