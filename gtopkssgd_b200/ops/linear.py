@@ -319,8 +319,10 @@ class _Linear(torch.autograd.Function):
         if not recording:
             return y
         ctx.activation, ctx.shape = activation, x.shape
-        if bits:   # all that is kept goes through autograd, which lets go of it behind the backward pass
-            x = Activation8.keep(x) if ctx.needs_input_grad[1] else None
+        if not ctx.needs_input_grad[1]:
+            x = None
+        elif bits:   # all that is kept goes through autograd, which lets go of it behind the backward pass
+            x = Activation8.keep(x)
         xs, ctx.x = Activation8.split(x)
         zs, ctx.z = Activation8.split(z)
         ctx.save_for_backward(weight, *xs, *zs)

@@ -361,6 +361,18 @@ def test_nothing_is_kept_where_gradients_are_off(which, monkeypatch):
     assert len(copies) == 2 and any(asked) and all(t.grad is not None for t in leaves)
 
 
+@pytest.mark.parametrize("bits", [0, 8])
+def test_a_frozen_weight_keeps_no_input(bits):
+    x, w, b = torch.randn(6, 40), torch.randn(24, 40), torch.randn(24, requires_grad=True)
+    for first in (False, True):
+        saved = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: saved.append(tuple(t.shape)) or t, lambda t: t):
+            y = linear(x.requires_grad_(first), w, b, "gelu", bits=bits)
+        assert (6, 40) not in saved and (6, 24) in saved
+        y.sum().backward()
+        assert (x.grad is not None) == first and b.grad is not None
+
+
 # -- failures -----------------------------------------------------------------------
 def test_a_product_whose_wait_ran_out_stops_the_training(monkeypatch):
     from gtopkssgd_b200 import settings
