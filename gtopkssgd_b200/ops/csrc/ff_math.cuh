@@ -343,23 +343,19 @@ __device__ __forceinline__ int block8_code(float x, uint32_t byte) {
 
 // ---- f32 as three bf16 pieces ---------------------------------------------------------------------------------------
 // Three bf16 pieces whose sum is v to 24 bits: each is the nearest to what the ones before left.  The first is cut
-// instead of rounded where rounding would overflow; a NaN is all in the first.  An infinity is 1, 0 and itself with its
-// sign: the last piece meets the other operand's first one only, which is zero where the operand is and has its sign
-// elsewhere, so that no infinity is multiplied by a lower piece that is zero or of the other sign.
+// instead of rounded where rounding would overflow; a NaN or an infinity is all in the first.
 __device__ __forceinline__ void split3(float v, __nv_bfloat16 (&p)[3]) {
-  if (isinf(v)) {
-    p[0] = __float2bfloat16_rn(copysignf(1.f, v));
-    p[1] = __float2bfloat16_rn(0.f);
-    p[2] = __float2bfloat16_rn(v);
-    return;
-  }
   p[0] = __float2bfloat16_rn(v);
-  if (isinf(__bfloat162float(p[0]))) p[0] = __float2bfloat16_rz(v);
+  if (isinf(__bfloat162float(p[0])) && !isinf(v)) p[0] = __float2bfloat16_rz(v);
   float left = v - __bfloat162float(p[0]);
-  if (isnan(v)) left = 0.f;
+  if (!(fabsf(v) <= 3.402823466e38f)) left = 0.f;
   p[1] = __float2bfloat16_rn(left);
   p[2] = __float2bfloat16_rn(left - __bfloat162float(p[1]));
 }
+// The lower products' sum on top of one that has the first pieces' products.  Where that is no longer finite it is the result:
+// the first piece has its value's sign and is zero only where it is, but an infinity, and what leaves f32's range, may meet
+// lower pieces that are zero or of the other sign.
+__device__ __forceinline__ float add_lower(float sum, float lower) { return fabsf(sum) <= 3.402823466e38f ? sum + lower : sum; }
 
 // ---- f32 as two f16 pieces -----------------------------------------------------------------------------------------
 // The power of two by which values whose largest magnitude has these bits are scaled: it then lies in [2^14, 2^15).

@@ -210,10 +210,9 @@ __device__ __forceinline__ void pack_rows(const PackItem& p, unsigned block) {
   }
 }
 
-// Two f16 pieces of scaled f32 values.  An infinity is 1 and itself with its sign: its second piece meets the other
-// operand's first one only, which has that operand's sign and is zero only where it is (a scaled value too small for that
-// is the smallest number in the first piece and less than nothing in the second).  Beside an infinity, where nothing is
-// scaled, the others count by their signs alone and stop at f16's largest.
+// Two f16 pieces of scaled f32 values.  A NaN or an infinity is all in the first, which has its value's sign and is zero only
+// where it is (a scaled value too small for that is the smallest number in the first piece and less than nothing in the
+// second).  Beside an infinity, where nothing is scaled, the others count by their signs alone and stop at f16's largest.
 template <int VEC>
 __device__ __forceinline__ void store_pairs(__half* out, long long stride, const Vec<float, VEC>& v, const float (&scale)[VEC]) {
   float high[VEC], low[VEC];
@@ -221,10 +220,10 @@ __device__ __forceinline__ void store_pairs(__half* out, long long stride, const
   for (int j = 0; j < VEC; ++j) {
     const float f = v.v[j], x = f * scale[j];
     float first = __half2float(__float2half_rn(x));
-    if (isinf(first)) first = copysignf(isinf(f) ? 1.f : 65504.f, f);
+    if (isinf(first) && !isinf(f)) first = copysignf(65504.f, f);
     if (first == 0.f && f != 0.f) first = copysignf(5.9604644775390625e-8f, f);   // 2^-24
     high[j] = first;
-    low[j] = isinf(f) ? f : fabsf(x) <= 65504.f ? x - first : 0.f;
+    low[j] = fabsf(x) <= 65504.f ? x - first : 0.f;
   }
   store_f32<__half, VEC>(out, high);
   store_f32<__half, VEC>(out + stride, low);

@@ -30,8 +30,8 @@
 //
 // 8192 x 2048 x 8192 bf16: forward 181 to 190 us (1.45 to 1.52 PFLOP/s, under the power cap), with gelu and its 8-bit input 200 to
 // 216, the input gradient and the weight's 200 to 245 (256 tiles are 3.5 rounds of the 74 pairs); 700 x 1500 x 10000 f32
-// 107 us of three pieces (0.59 PFLOP/s of bf16 products), as pairs 75 us (0.84 PFLOP/s of f16 products): shared memory, read
-// for the products of 128 columns and written, is full.
+// 110 us of three pieces (1.15 PFLOP/s of bf16 products), as pairs 75 us (0.84 PFLOP/s of f16 products: shared memory, read
+// for three products of 128 columns and written, is full).
 //
 // Every wait ends: after a time limit the waiter raises the CTA's abort flag and the status word, everybody leaves
 // after its copies and products in flight, and TMEM is freed.
@@ -731,12 +731,12 @@ k8_gemm(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUten
             const int c = side * 32 + j * 64;
             if (c < s.bn) {
               float v[32];   // (one after the other: both at once spill)
-              tmem_load32(lanes + (uint32_t)acc * acc_columns + (uint32_t)(s.bn + c), v);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) sum[j][i] += v[i];
               tmem_load32(lanes + (uint32_t)acc * acc_columns + (uint32_t)c, v);
 #pragma unroll
               for (int i = 0; i < 32; ++i) sum[j][i] += v[i];
+              tmem_load32(lanes + (uint32_t)acc * acc_columns + (uint32_t)(s.bn + c), v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) sum[j][i] = add_lower(sum[j][i], v[i]);
             }
           }
           tc_fence_before();

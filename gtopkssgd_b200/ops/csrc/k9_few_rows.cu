@@ -2,8 +2,9 @@
 //
 //   z = x W^T + b ; y = act(z) + r ; z kept in its type or in 8 bits
 //
-// Bound by the bytes of W, each read once (f32 above 16 rows: twice, for 16 rows of x each), and by latency.  A tile of a matrix product for 256 rows would wait for its
-// few useful rows as long as for all, and wants rows of W on 16-byte boundaries; here W goes from memory to registers
+// Bound by the bytes of W, each read once (f32 above 16 rows: twice, for 16 rows of x each), and by latency.  A tile of a
+// matrix product for 256 rows would wait for its few useful rows as long as for all, and wants rows of W on 16-byte
+// boundaries; here W goes from memory to registers
 // at any alignment and to the tensor cores by mma.sync, whose rate is of no account: W's rows are its rows, x's rows
 // its columns.  Which element of the contracted axis stands at which place of a fragment is free as long as both
 // operands agree: a lane takes 16 neighbours of a row, so that a warp reads whole lines of 16 rows.
@@ -12,8 +13,7 @@
 // their sums through shared memory, in order.  The next 64 of W and x are on their way meanwhile (x, too, comes from L2:
 // no two warps of a half read the same part of it).  f32: three bf16 pieces a value and the six products that count; the
 // large one is summed apart from the small ones, and both go to an f32 sum after every 64 of k, as in K8.  1500 x 6000 bf16
-// (18 MB, 2.8 us at a copy's rate): 1, 8, 20 and 32 rows 7, 8, 12 and 14 us; f32 12, 13, 27 and 29 (164 bytes of spills
-// above 8 rows).
+// (18 MB, 2.8 us at a copy's rate): 1, 8, 20 and 32 rows 7, 8, 12 and 14 us; f32 12, 12, 27 and 29.
 #include "colsum.cuh"
 #include "common.cuh"
 #include "host_api.h"
@@ -87,19 +87,8 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 
 // Three bf16 pieces of two neighbours, a word each: the significand cut after 8, 16 and 24 bits, which takes a third of the
 // instructions of rounding the pieces.  What the products of pieces then leave out is 2^-22 of a product at most, 2^-24
-// on average.  FINITE: infinities come out as NaN; else as 1, 0 and the infinity (see split3).
-template <bool FINITE>
+// on average.  An infinity's lower pieces are NaN, which add_lower leaves out.
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[3]) {
-  if constexpr (!FINITE) {
-    const bool ai = isinf(a), bi = isinf(b);
-    const float ax = a, bx = b;
-    if (ai) a = copysignf(1.f, a);
-    if (bi) b = copysignf(1.f, b);
-    split_pair<true>(a, b, w);
-    if (ai) w[2] = (w[2] & 0xffff0000u) | (__float_as_uint(ax) >> 16);
-    if (bi) w[2] = (w[2] & 0xffffu) | (__float_as_uint(bx) & 0xffff0000u);
-    return;
-  }
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
     w[i] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
@@ -141,8 +130,19 @@ __global__ void __launch_bounds__(kFewThreads) k9_few_rows(FewArgs g) {
     for (int t = 0; t < TOK; ++t) ax[t].load(xr[t], from, quad, g.k, t * 8 + row < rows);
   };
   const int end = n0 < g.n ? g.k : 0;   // nothing to do for rows past W's
-  auto multiply = [&](const Strip<T, VEC, 16>& u0, const Strip<T, VEC, 16>& u1, const Strip<T, VEC, 16> (&x)[TOK], auto finite) {
-    constexpr bool kFinite = decltype(finite)::value;
+  int c = split * kFewChunk;
+  if (kAhead && c < end) fetch_w(c);
+  if (kXAhead && c < end) fetch_x(c);
+  for (; c < end; c += kSplits * kFewChunk) {
+    if constexpr (!kAhead) fetch_w(c);
+    if constexpr (!kXAhead) fetch_x(c);
+    const Strip<T, VEC, 16> u0 = a0, u1 = a1;
+    Strip<T, VEC, 16> x[TOK];
+#pragma unroll
+    for (int t = 0; t < TOK; ++t) x[t] = ax[t];
+    const int next = c + kSplits * kFewChunk;
+    if (kAhead && next < end) fetch_w(next);
+    if (kXAhead && next < end) fetch_x(next);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       if constexpr (sizeof(T) == 2) {
@@ -150,15 +150,15 @@ __global__ void __launch_bounds__(kFewThreads) k9_few_rows(FewArgs g) {
         for (int t = 0; t < TOK; ++t) mma16816(large[t], u0.w[2 * s], u1.w[2 * s], u0.w[2 * s + 1], u1.w[2 * s + 1], x[t].w[2 * s], x[t].w[2 * s + 1], T{});
       } else {
         uint32_t p0[3], p1[3], p2[3], p3[3];
-        split_pair<kFinite>(u0.value(4 * s), u0.value(4 * s + 1), p0);
-        split_pair<kFinite>(u1.value(4 * s), u1.value(4 * s + 1), p1);
-        split_pair<kFinite>(u0.value(4 * s + 2), u0.value(4 * s + 3), p2);
-        split_pair<kFinite>(u1.value(4 * s + 2), u1.value(4 * s + 3), p3);
+        split_pair(u0.value(4 * s), u0.value(4 * s + 1), p0);
+        split_pair(u1.value(4 * s), u1.value(4 * s + 1), p1);
+        split_pair(u0.value(4 * s + 2), u0.value(4 * s + 3), p2);
+        split_pair(u1.value(4 * s + 2), u1.value(4 * s + 3), p3);
 #pragma unroll
         for (int t = 0; t < TOK; ++t) {
           uint32_t q0[3], q1[3];
-          split_pair<kFinite>(x[t].value(4 * s), x[t].value(4 * s + 1), q0);
-          split_pair<kFinite>(x[t].value(4 * s + 2), x[t].value(4 * s + 3), q1);
+          split_pair(x[t].value(4 * s), x[t].value(4 * s + 1), q0);
+          split_pair(x[t].value(4 * s + 2), x[t].value(4 * s + 3), q1);
 #pragma unroll
           for (int i = 2; i >= 0; --i)
 #pragma unroll
@@ -174,42 +174,9 @@ __global__ void __launch_bounds__(kFewThreads) k9_few_rows(FewArgs g) {
       for (int t = 0; t < TOK; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          total[t][i] += large[t][i] + small[t][i];
+          total[t][i] = add_lower(total[t][i] + large[t][i], small[t][i]);
           large[t][i] = small[t][i] = 0.f;
         }
-    }
-  };
-  int c = split * kFewChunk;
-  if (kAhead && c < end) fetch_w(c);
-  if (kXAhead && c < end) fetch_x(c);
-  for (; c < end; c += kSplits * kFewChunk) {
-    if constexpr (!kAhead) fetch_w(c);
-    if constexpr (!kXAhead) fetch_x(c);
-    const Strip<T, VEC, 16> u0 = a0, u1 = a1;
-    Strip<T, VEC, 16> x[TOK];
-#pragma unroll
-    for (int t = 0; t < TOK; ++t) x[t] = ax[t];
-    const int next = c + kSplits * kFewChunk;
-    if (kAhead && next < end) fetch_w(next);
-    if (kXAhead && next < end) fetch_x(next);
-    multiply(u0, u1, x, std::true_type{});
-  }
-  if constexpr (sizeof(T) == 4) {   // a NaN may be an infinity in pieces: once more, with the pieces that keep it one
-    bool none = true;
-#pragma unroll
-    for (int t = 0; t < TOK; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) none = none && !isnan(total[t][i]);
-    if (!__all_sync(0xffffffffu, none)) {
-#pragma unroll
-      for (int t = 0; t < TOK; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) total[t][i] = 0.f;
-      for (c = split * kFewChunk; c < end; c += kSplits * kFewChunk) {
-        fetch_w(c);
-        fetch_x(c);
-        multiply(a0, a1, ax, std::false_type{});
-      }
     }
   }
 #pragma unroll

@@ -22,7 +22,7 @@ from .activation8 import TYPES, Activation8, act_of, bits_of, colsum, ld, matrix
 from .select import _FLOAT, _ptr
 
 # Rows up to which K9 takes a forward pass, us on the device by K9 and by K8, whose operands have to be made first: 1500 x 6000
-# in bf16 1, 8, 20 and 32 rows 7, 8, 12 and 14 against 22, in f32 13, 13, 28 and 30 against 48; and a launch less.
+# in bf16 1, 8, 20 and 32 rows 7, 8, 12 and 14 against 22, in f32 12, 12, 27 and 29 against 48; and a launch less.
 FEW_ROWS = 32
 
 Kept = Union[None, torch.Tensor, Activation8]

@@ -418,6 +418,21 @@ def test_linear_f32_infinities_by_pairs(rows, inner, outer, monkeypatch):
     _check_infinities(rows, inner, outer)
 
 
+@pytest.mark.parametrize("by_pairs", [False, True])
+@pytest.mark.parametrize("rows", [5, 70])
+def test_linear_f32_products_past_the_range(rows, by_pairs, monkeypatch):
+    """An infinity of its sign, as of the sum in f32, whatever the lower pieces' signs."""
+    from gtopkssgd_b200.ops import linear as module
+    if by_pairs:
+        monkeypatch.setattr(module, "PAIRS_FROM_FORWARD", 0)
+    x, w = _randn(rows, 64).abs() + 0.1, _randn(40, 64, seed=1).abs() + 0.1
+    sign = torch.where(torch.arange(40, device=DEV) % 2 == 0, 1.0, -1.0)[:, None]
+    y = linear_forward(x * 1e25, w * sign * 1e25)[0]
+    assert torch.equal(y, torch.full_like(y, math.inf) * sign.t())
+    y = linear_forward(x * 1e15, w * sign * 1e15)[0]
+    assert y.isfinite().all() and torch.equal(y.sign(), sign.t().expand_as(y))
+
+
 @pytest.mark.parametrize("rows,inner,outer", [(1, 40, 33), (20, 1500, 600), (129, 65, 257), (515, 1001, 130), (1000, 8, 1000), (300, 2000, 96)])
 def test_linear_f32_by_pairs(rows, inner, outer, monkeypatch):
     """f32 operands as two scaled f16 pieces, which only large products take, at the sizes where they can go wrong.  What
